@@ -1,0 +1,387 @@
+"""The operators of the 4-bit KV cache, as they are measured: writing K/V rows
+into the cache and reading them back, reading rows of a filled cache, and
+attention over the cache for single tokens (the decode step) and for chunks of
+a prompt.
+
+The cache is a uint8 tensor [slots, layers, kv heads, blocks, 68 * hd]; a block
+holds the K and V records of 64 positions of one kv head:
+
+  [K codes 64 x hd/2][K scales 64 x hd/64 fp16][V codes 64 x hd/2][V scales 64 x hd/64 fp16]
+
+A record is a Q4 record of groups of 64 values: s = fp16(max(max|x|, 1e-12) / 7)
+(at most 65504), code = clip(rint(x / s), -8, 7) + 8, value (code - 8) * s.
+Value d of row r (group d // 64, word u = (d % 64) // 8 of the group, nibble
+d % 8) is in byte u * 4 * (hd / 64) + 4 * (d // 64) + (d % 8) // 2 of the row,
+low nibble first; K rows lie in order, V row r lies at place
+(r & 56) + 4 * (r & 1) + ((r >> 1) & 3) with its word u at u ^ (r & 4).
+
+A case's "op":
+  append  k, v [rows, kv heads, hd] are written at (slot, position) pairs; the
+          pass returns the values that the cache then holds for those rows
+  read    values of given (slot, position) pairs of a filled cache
+  attend  q [batch, T, heads, hd]; query i of sequence b sees the first
+          len[b] - T + 1 + i cached positions; a row that sees none is zero
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+BLOCK = 64
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def listed():
+    return [
+        # one decode step's K/V rows of 64 sequences of the Qwen3 shape, each at its own position
+        {"name": "append step", "op": "append", "rows": 64, "kv": 4, "hd": 128, "type": "f32", "layers": 2, "slots": 64,
+         "cap": 1024, "spread": "slots"},
+        # a whole prompt's rows of one sequence, 16 kv heads (the OLMoE shape), an odd length
+        {"name": "append prompt", "op": "append", "rows": 8179, "kv": 16, "hd": 128, "type": "f32", "layers": 1, "slots": 2,
+         "cap": 8192, "spread": "run"},
+        # some rows of many sequences, heads of 64, 16-bit values
+        {"name": "read rows", "op": "read", "rows": 333, "kv": 8, "hd": 64, "type": "bf16", "layers": 2, "slots": 16,
+         "cap": 1500, "spread": "any"},
+        # one sequence's whole history
+        {"name": "read history", "op": "read", "rows": 30000, "kv": 4, "hd": 128, "type": "f32", "layers": 1, "slots": 2,
+         "cap": 30001, "spread": "run"},
+        # the first tokens of one sequence: launch latency
+        {"name": "step first", "op": "attend", "batch": 1, "T": 1, "heads": 32, "kv": 4, "hd": 128, "type": "f32",
+         "layers": 2, "low": 17, "len": 17, "cap": 4096},
+        # the benchmark's decode step: 64 sequences at context 512
+        {"name": "step 64x512", "op": "attend", "batch": 64, "T": 1, "heads": 32, "kv": 4, "hd": 128, "type": "f32",
+         "layers": 2, "low": 513, "len": 522, "cap": 586},
+        # 64 sequences of ragged lengths, one of them empty, 16-bit activations
+        {"name": "step ragged", "op": "attend", "batch": 64, "T": 1, "heads": 32, "kv": 4, "hd": 128, "type": "bf16",
+         "layers": 1, "low": 0, "len": 8191, "cap": 8192},
+        # one long sequence
+        {"name": "step long", "op": "attend", "batch": 1, "T": 1, "heads": 32, "kv": 4, "hd": 128, "type": "f32",
+         "layers": 1, "low": 131071, "len": 131071, "cap": 131072},
+        # every head has keys of its own (the OLMoE shape)
+        {"name": "step mha", "op": "attend", "batch": 16, "T": 1, "heads": 16, "kv": 16, "hd": 128, "type": "f32",
+         "layers": 1, "low": 1000, "len": 4096, "cap": 4096},
+        # a few drafted tokens of each sequence, groups of five heads of 64
+        {"name": "chunk draft", "op": "attend", "batch": 8, "T": 5, "heads": 10, "kv": 2, "hd": 64, "type": "f16",
+         "layers": 2, "low": 3, "len": 1777, "cap": 2048},
+        # one pass of a prompt through the decoder: 64 positions behind 2000 cached ones
+        {"name": "chunk pass", "op": "attend", "batch": 1, "T": 64, "heads": 32, "kv": 4, "hd": 128, "type": "f32",
+         "layers": 1, "low": 2064, "len": 2064, "cap": 4096},
+        # a long prompt at once, over a cached history of the same length
+        {"name": "chunk prompt", "op": "attend", "batch": 1, "T": 2047, "heads": 32, "kv": 4, "hd": 128, "type": "f32",
+         "layers": 1, "low": 4100, "len": 4100, "cap": 4104},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "read", "attend", "attend", "attend"])
+    hd = rng.choice([64, 128])
+    kind = rng.choice(["f32", "f32", "f16", "bf16"])
+    layers = rng.choice([1, 2, 3])
+    if op != "attend":
+        kv = rng.choice([1, 2, 4, 5, 8, 16])
+        spread = rng.choice(["slots", "run", "any"])
+        rows = _log(rng, 1, 8179 * 16 // kv)
+        slots = rng.randint(1, 9)
+        if spread == "slots":
+            rows = slots = min(rows, 256)
+        cap = max(rows + rng.randint(0, 70) if spread == "run" else -(-rows // slots), rng.randint(1, 600))
+        return {"op": op, "rows": rows, "kv": kv, "hd": hd, "type": kind, "layers": layers if rows < 4000 else 1,
+                "slots": slots, "cap": cap, "spread": spread}
+    kv = rng.choice([1, 2, 3, 4, 8, 16])
+    heads = kv * rng.choice([g for g in (1, 2, 3, 4, 5, 7, 8, 16) if g * kv <= 64])
+    T = 1 if rng.random() < 0.6 else _log(rng, 2, 1500)
+    batch = _log(rng, 1, 96) if T == 1 else _log(rng, 1, 1 + 256 // T)
+    # keys of all sequences and heads, and products, within those of the largest listed cases
+    most = min(64 * 8191 * 4 // (batch * kv), 2047 * 4100 * 32 // (batch * T * heads), 131071)
+    longest = max(T, _log(rng, 1, max(2, most)))
+    low = longest if rng.random() < 0.3 else rng.randint(0, longest)
+    return {"op": op, "batch": batch, "T": T, "heads": heads, "kv": kv, "hd": hd, "type": kind,
+            "layers": layers if batch * kv * longest < 100000 else 1, "low": low, "len": longest,
+            "cap": longest + rng.randint(0, 130)}
+
+
+# ---------------------------------------------------------------------------
+# inputs
+
+
+def _places(hd, device):
+    """Byte offsets in a block of row r's hd/2 code bytes, in the order of their values: K [64, hd/2], V [64, hd/2]."""
+    ng = hd // 64
+    r = torch.arange(BLOCK, device=device)[:, None]
+    b = torch.arange(hd // 2, device=device)[None, :]
+    group, u, byte = b // 32, b % 32 // 4, b % 4
+    inner = 4 * group + byte
+    k = r * (hd // 2) + u * 4 * ng + inner
+    at = (r & 56) + 4 * (r & 1) + ((r >> 1) & 3)
+    v = 34 * hd + at * (hd // 2) + (u ^ (r & 4)) * 4 * ng + inner
+    return k, v
+
+
+def _quantise(x):
+    """fp32 rows [..., hd] -> code bytes [..., hd/2] and fp16 scales [..., hd/64]."""
+    g = x.unflatten(-1, (-1, 64))
+    amax = torch.nan_to_num(g.abs(), nan=0.0, posinf=float("inf")).amax(-1, keepdim=True).clamp_min(1e-12)
+    s = (amax / torch.full_like(amax, 7.0)).clamp_max(65504.0).half()  # a true division: by a number it is a product
+    q = g / s.float()
+    n = torch.where(torch.isnan(q), torch.zeros_like(q), torch.round(q).clamp(-8, 7)).to(torch.int32) + 8
+    n = n.flatten(-2)
+    return (n[..., 0::2] | (n[..., 1::2] << 4)).to(torch.uint8), s.squeeze(-1)
+
+
+def _write(cache, layer, k, v, slots, positions):
+    """Writes fp32 rows k, v [N, kv, hd] at (slots, positions)."""
+    hd, kv = k.shape[-1], k.shape[1]
+    ng = hd // 64
+    pk, pv = _places(hd, cache.device)
+    blk, r = positions.long() // BLOCK, positions.long() % BLOCK
+    flat = cache.view(-1)
+    head = torch.arange(kv, device=cache.device)
+    S, L, H, NB, size = cache.shape
+    base = (((slots.long()[:, None] * L + layer) * H + head[None, :]) * NB + blk[:, None]) * size  # [N, kv]
+    sc = 2 * ng * r[:, None, None] + torch.arange(2 * ng, device=cache.device)
+    for x, place, scales in ((k, pk, 32 * hd), (v, pv, 66 * hd)):
+        codes, s = _quantise(x)
+        flat[base[:, :, None] + place[r][:, None, :]] = codes
+        flat[base[:, :, None] + scales + sc] = s.contiguous().view(torch.uint8).reshape(s.shape[0], kv, 2 * ng)
+
+
+def _read(cache, layer, slots, positions):
+    """fp32 values k, v [N, kv, hd] of the rows at (slots, positions)."""
+    S, L, H, NB, size = cache.shape
+    hd = size // 68
+    ng = hd // 64
+    pk, pv = _places(hd, cache.device)
+    blk, r = positions.long() // BLOCK, positions.long() % BLOCK
+    flat = cache.view(-1)
+    head = torch.arange(H, device=cache.device)
+    base = (((slots.long()[:, None] * L + layer) * H + head[None, :]) * NB + blk[:, None]) * size
+    sc = 2 * ng * r[:, None, None] + torch.arange(2 * ng, device=cache.device)
+    out = []
+    for place, scales in ((pk, 32 * hd), (pv, 66 * hd)):
+        b = flat[base[:, :, None] + place[r][:, None, :]]
+        s = flat[base[:, :, None] + scales + sc].view(torch.float16).float()
+        n = torch.stack((b & 15, b >> 4), -1).flatten(-2).float() - 8.0
+        out.append((n.unflatten(-1, (ng, 64)) * s[..., None]).flatten(-2))
+    return out
+
+
+def _history(cache, layer, slots, n):
+    """fp32 keys and values [batch, kv, n, hd] of the first n positions of each slot."""
+    S, L, H, NB, size = cache.shape
+    hd = size // 68
+    ng, nb = hd // 64, -(-n // BLOCK)
+    pk, pv = _places(hd, cache.device)
+    blocks = cache[slots.long(), layer, :, :nb]  # [batch, kv, nb, size]
+    out = []
+    for place, scales in ((pk, 32 * hd), (pv, 66 * hd)):
+        b = blocks[..., place.reshape(-1)].unflatten(-1, (BLOCK, hd // 2))
+        s = blocks[..., scales:scales + 2 * hd].contiguous().view(torch.float16).float().unflatten(-1, (BLOCK, ng))
+        x = torch.stack((b & 15, b >> 4), -1).flatten(-2).float() - 8.0
+        x = (x.unflatten(-1, (ng, 64)) * s[..., None]).flatten(-2)
+        out.append(x.flatten(2, 3)[:, :, :n])
+    return out
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda", torch.cuda.current_device())
+    g = torch.Generator(device=dev).manual_seed(seed)
+    c, kind = case, TYPES[case["type"]]
+    kv, hd, L = c["kv"], c["hd"], c["layers"]
+    slots_held = c.get("slots") or c["batch"] + 1
+    nb = -(-c["cap"] // BLOCK)
+    layer = L - 1
+    # bytes of a cache whose other layers and rows hold what earlier use left there
+    cache = torch.randint(0, 256, (slots_held, L, kv, nb, 68 * hd), dtype=torch.uint8, device=dev, generator=g)
+    st = {"op": c["op"], "cache": cache, "layer": layer, "type": kind}
+
+    def rows(n):
+        # keys after a norm and a rotation: near unit size, some channels larger; values smaller
+        k = torch.randn(n, kv, hd, device=dev, generator=g)
+        k = k * (1.0 + 2.0 * (torch.rand(1, kv, hd, device=dev, generator=g) < 0.05).float())
+        v = torch.randn(n, kv, hd, device=dev, generator=g) * 0.6
+        return k, v
+
+    if c["op"] == "attend":
+        B, T = c["batch"], c["T"]
+        lens = torch.randint(c["low"], c["len"] + 1, (B,), device=dev, generator=g).to(torch.int32)
+        lens[0] = c["len"]
+        if c["low"] == 0 and B > 1:
+            lens[B - 1] = 0  # a padded entry of the batch
+        slots = torch.randperm(slots_held, device=dev, generator=g)[:B].to(torch.int32)
+        # the history of each slot is written in pieces, as it was in earlier steps
+        piece = max(1, (1 << 24) // (kv * hd))
+        for b in range(B):
+            n = c["len"]
+            for p in range(0, n, piece):
+                m = min(piece, n - p)
+                k, v = rows(m)
+                at = torch.arange(p, p + m, device=dev)
+                _write(cache, layer, k, v, slots[b].expand(m), at)
+        q = (torch.randn(B, T, c["heads"], hd, device=dev, generator=g) * 1.5).to(kind)
+        st.update(q=q, slots=slots, lens=lens, scale=1.0 / math.sqrt(hd), longest=c["len"])
+        return st
+    n = c["rows"]
+    if c["spread"] == "slots":  # one row of each slot, as a decode step writes them
+        slots = torch.randperm(slots_held, device=dev, generator=g)[:n]
+        positions = torch.randint(0, c["cap"], (n,), device=dev, generator=g)
+    elif c["spread"] == "run":  # consecutive rows of one slot, as a prompt has them
+        slots = torch.full((n,), slots_held - 1, device=dev)
+        positions = torch.arange(n, device=dev) + int(torch.randint(0, c["cap"] - n + 1, (1,), device=dev, generator=g))
+    else:
+        at = torch.randperm(slots_held * c["cap"], device=dev, generator=g)[:n]
+        slots, positions = at // c["cap"], at % c["cap"]
+    slots, positions = slots.to(torch.int32), positions.to(torch.int32)
+    k, v = rows(n)
+    if c["op"] == "read":
+        _write(cache, layer, k, v, slots, positions)
+    else:
+        st.update(k=k.to(kind), v=v.to(kind))
+    st.update(slots=slots, positions=positions)
+    return st
+
+
+# ---------------------------------------------------------------------------
+# one pass
+
+
+def run(st):
+    cache, layer, kind, slots = st["cache"], st["layer"], st["type"], st["slots"]
+    if own:
+        from joule_b200 import kv4
+        if st["op"] == "attend":
+            return kv4.kv4_attention(cache, layer, st["q"], slots, st["lens"], scale=st["scale"])
+        if st["op"] == "append":
+            kv4.kv4_append(cache, layer, st["k"], st["v"], slots, st["positions"])
+        return kv4.kv4_read(cache, layer, slots, st["positions"], dtype=kind)
+    if st["op"] == "append":
+        _write(cache, layer, st["k"].float(), st["v"].float(), slots, st["positions"])
+    if st["op"] != "attend":
+        k, v = _read(cache, layer, slots, st["positions"])
+        return k.to(kind), v.to(kind)
+    q = st["q"].float()
+    B, T, H, hd = q.shape
+    n = st["longest"]
+    k, v = _history(cache, layer, slots, n)
+    kv = k.shape[1]
+    q = q.view(B, T, kv, H // kv, hd).permute(0, 2, 1, 3, 4).reshape(B, kv, T * (H // kv), hd)
+    s = torch.matmul(q, k.transpose(2, 3)).view(B, kv, T, H // kv, n) * st["scale"]
+    seen = st["lens"].long()[:, None] - T + 1 + torch.arange(T, device=q.device)  # [B, T]
+    mask = (torch.arange(n, device=q.device) < seen[..., None])[:, None, :, None, :]
+    s = s.masked_fill(~mask, -math.inf)
+    top = s.amax(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).min)
+    p = torch.exp(s - top)
+    del s
+    total = p.sum(-1, keepdim=True)
+    o = torch.matmul(p.view(B, kv, -1, n), v).view(B, kv, T, H // kv, hd)
+    o = torch.where(total > 0, o / total.clamp_min(1e-30), torch.zeros_like(o))
+    return o.permute(0, 2, 1, 3, 4).reshape(B, T, H, hd).to(kind)
+
+
+def work(case):
+    c, esize = case, 4 if case["type"] == "f32" else 2
+    record = 2 * (c["hd"] // 2 + c["hd"] // 32)  # K and V of one (position, kv head)
+    if c["op"] != "attend":
+        values = c["rows"] * c["kv"] * c["hd"] * 2
+        passes = 2 if c["op"] == "append" else 1  # rows in, values out
+        return {"bytes": passes * values * esize + c["rows"] * (c["kv"] * record + 8), "flops": 2 * passes * values}
+    # sequences of mean length (low + len) / 2; query i misses the keys behind it
+    B, T, mean = c["batch"], c["T"], (c["low"] + c["len"]) / 2
+    seen = max(mean - (T - 1) / 2, mean / 2)
+    return {"bytes": B * mean * c["kv"] * record + 2 * B * T * c["heads"] * c["hd"] * esize,
+            "flops": 4 * B * T * c["heads"] * c["hd"] * seen}
+
+
+# ---------------------------------------------------------------------------
+# the definition in 64 bits
+
+
+def _power(e):
+    """2^e in float64 for whole e, built from its bits: torch.pow is not exact on the GPU."""
+    return ((e + 1023) << 52).view(torch.float64)
+
+
+def _value_table(hd):
+    """For each (row, value) of a block: K byte, V byte, nibble, K scale byte, V scale byte."""
+    ng = hd // 64
+    kb, vb, sk, sv = (np.zeros((BLOCK, hd), np.int64) for _ in range(4))
+    for r in range(BLOCK):
+        place = (r // 8) * 8 + (r % 2) * 4 + (r % 8) // 2
+        for d in range(hd):
+            g, u, j = d // 64, d % 64 // 8, d % 8
+            kb[r, d] = r * hd // 2 + u * 4 * ng + 4 * g + j // 2
+            vb[r, d] = 34 * hd + place * hd // 2 + (u + 4 * (1 - 2 * (u // 4)) * ((r // 4) % 2)) * 4 * ng + 4 * g + j // 2
+            sk[r, d] = 32 * hd + 2 * (r * ng + g)
+            sv[r, d] = 66 * hd + 2 * (r * ng + g)
+    return kb, vb, np.tile(np.arange(hd) % 2 * 4, (BLOCK, 1)), sk, sv
+
+
+def _block_values(blocks, hd):
+    """float64 K and V [..., 64, hd] of uint8 blocks [..., 68 * hd]."""
+    kb, vb, sh, sk, sv = (torch.from_numpy(t).to(blocks.device) for t in _value_table(hd))
+
+    def half(at):  # fp16 bits -> float64: sign, exponent and fraction taken apart
+        h = blocks[..., at].to(torch.int64) + 256 * blocks[..., at + 1].to(torch.int64)
+        e, f = (h >> 10) & 31, (h & 1023).double()
+        x = torch.where(e == 0, f * 2.0 ** -24, (1024.0 + f) * _power(e - 25))
+        return torch.where(h >> 15 == 1, -x, x)
+
+    one = lambda at, s: (((blocks[..., at].to(torch.int64) >> sh) & 15) - 8).double() * half(s)  # noqa: E731
+    return one(kb, sk), one(vb, sv)
+
+
+def _held64(x):
+    """What the cache holds of rows x, from the definition."""
+    g = x.double().reshape(*x.shape[:-1], -1, 64)
+    top = torch.clamp(g.abs().amax(-1, keepdim=True), min=1e-12)
+    s = torch.clamp(top / torch.full_like(top, 7.0), max=65504.0)
+    # to the nearest of the fp16 numbers, ties to even: steps of 2^-24 below 2^-14
+    step = _power(torch.clamp((s.view(torch.int64) >> 52) - 1023, min=-14) - 10)
+    s = torch.round(s / step) * step
+    n = torch.where(s > 0, torch.clamp(torch.round(g / torch.where(s > 0, s, torch.ones_like(s))), -8, 7), torch.zeros_like(g))
+    return (n * s).reshape(x.shape)
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    cache, layer = st["cache"], st["layer"]
+    hd = case["hd"]
+    if st["op"] == "append":
+        return _held64(st["k"]), _held64(st["v"])
+    if st["op"] == "read":
+        ks, vs = [], []
+        for i in range(0, case["rows"], 512):
+            slots, pos = st["slots"][i:i + 512].long(), st["positions"][i:i + 512].long()
+            k, v = _block_values(cache[slots, layer, :, pos // BLOCK], hd)  # [N, kv, 64, hd]
+            at = torch.arange(len(pos), device=pos.device)
+            ks.append(k[at, :, pos % BLOCK])
+            vs.append(v[at, :, pos % BLOCK])
+        return torch.cat(ks), torch.cat(vs)
+    B, T, H, kv = case["batch"], case["T"], case["heads"], case["kv"]
+    out = torch.zeros(B, T, H, hd, dtype=torch.float64, device=cache.device)
+    lens = st["lens"].tolist()
+    for b in range(B):
+        n = lens[b]
+        if n == 0:
+            continue
+        for h in range(kv):
+            blocks = cache[int(st["slots"][b]), layer, h, :-(-n // BLOCK)]
+            parts = [_block_values(blocks[i:i + 256], hd) for i in range(0, blocks.shape[0], 256)]
+            k = torch.cat([p[0].reshape(-1, hd) for p in parts])[:n]
+            v = torch.cat([p[1].reshape(-1, hd) for p in parts])[:n]
+            for i0 in range(0, T, 256):
+                i1 = min(T, i0 + 256)
+                q = st["q"][b, i0:i1, h * (H // kv):(h + 1) * (H // kv)].double()
+                s = torch.einsum("tgd,nd->tgn", q, k) * st["scale"]
+                sees = n - T + torch.arange(i0, i1, device=k.device)  # the last key that each query sees
+                hidden = torch.arange(n, device=k.device)[None, None, :] > sees[:, None, None]
+                s = s.masked_fill(hidden, -math.inf)
+                w = torch.softmax(s, -1)
+                w = torch.where((sees < 0)[:, None, None], torch.zeros_like(w), w)
+                out[b, i0:i1, h * (H // kv):(h + 1) * (H // kv)] = torch.einsum("tgn,nd->tgd", w, v)
+    return out
