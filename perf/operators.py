@@ -255,7 +255,7 @@ def run(st):
     if own:
         from joule_b200 import kv4
         if st["op"] == "attend":
-            return kv4.kv4_attention(cache, layer, st["q"], slots, st["lens"], scale=st["scale"])
+            return kv4.kv4_attention(cache, layer, st["q"], slots, st["lens"], scale=st["scale"], longest=st["longest"])
         if st["op"] == "append":
             kv4.kv4_append(cache, layer, st["k"], st["v"], slots, st["positions"])
         return kv4.kv4_read(cache, layer, slots, st["positions"], dtype=kind)
