@@ -489,6 +489,69 @@ void set_lm_threads(int n);
  * counterpart in the reference. */
 int jl_decode_status(void);
 
+/* ------------------------------------------------------------------ */
+/* The 4-bit KV cache: keys and values held as Q4 records (groups of 64 values
+ * along the head, fp16 scales, 4.25 bits per value against the 32 of
+ * jl_dec's fp32 cache), quantised as they are appended, read back, and
+ * attended over. No counterpart in the reference, whose caches are fp32.
+ *
+ * A cache is one caller-owned device buffer of jl_kv4_bytes(c) bytes at
+ * `base` (16-byte aligned): [slots][L][n_kv][ceil(maxT / 64)] blocks of 68 * hd
+ * bytes, each the K and V records of 64 positions of one head,
+ *   [K codes 64 x hd/2][K scales 64 x hd/64][V codes 64 x hd/2][V scales ...].
+ * A record has jl_q4_quantize's values; beyond its rules a scale past fp16
+ * stays at 65504 and a NaN becomes 0, so a cache holds finite values. Word u
+ * (8 values) of group g of a row is at word u * (hd / 64) + g of the row; K rows lie
+ * in order, V row r at place (r & 56) + 4 (r & 1) + ((r >> 1) & 3) with its
+ * word u at u ^ (r & 4). hd is 64 or 128. The buffer needs no initialisation:
+ * only records that were appended are used.
+ *
+ * Value types: */
+#define JL_F32 0
+#define JL_F16 1
+#define JL_BF16 2
+typedef struct {
+    void* base;
+    int slots, L, n_kv, hd, maxT;
+} jl_kv4;
+
+/* Bytes of the buffer behind c (its base is not read), -1 for bad sizes. */
+long long jl_kv4_bytes(const jl_kv4* c);
+
+/* Quantise and append: row n (n < N) of k and v, [n_kv][hd] values of `dtype`
+ * at k + n * k_stride / v + n * v_stride (elements; rows 16-byte aligned), goes
+ * to position positions[n] of slot slots[n] in layer l. The (slot, position)
+ * pairs of one call are distinct. All pointers device; N = 0 does nothing. A
+ * pair outside the cache is skipped and sets bit 8 of dev_status (device int,
+ * nullable, as in the two calls below). */
+int jl_kv4_append(const jl_kv4* c, int l, const void* k, const void* v, int dtype,
+                  long long k_stride, long long v_stride, const int* slots,
+                  const int* positions, int N, int* dev_status, void* stream);
+
+/* Read back: k and v [N][n_kv][hd] of `dtype` receive the cached values of
+ * (slots[n], positions[n]); (code - 8) * scale is exact in fp32 and rounded
+ * once to a 16-bit type. A pair outside the cache reads as zeros. */
+int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* positions, int N,
+                void* k, void* v, int dtype, int* dev_status, void* stream);
+
+/* Attention of T query rows per sequence over layer l: row i of sequence b,
+ * q + (b * T + i) * q_stride elements ([H][hd] of `dtype`, 16-byte aligned),
+ * sees the first lens[b] - T + 1 + i positions of slot slots[b] (its own
+ * position is the last of them: append first). out [B][T][H][hd] of `dtype`:
+ * softmax(scale * q.K) V per head, head h on kv head h / (H / n_kv); a row
+ * that sees nothing is 0. T = 1 is a decode step, T > 1 a piece of a prompt.
+ * `longest` is a bound that the caller knows of the lens (0: maxT); a length
+ * outside [0, longest] or a slot outside the cache gives zeros and the status
+ * bit. ws: jl_kv4_attn_ws(c, B, T, H) bytes of device memory, 16-byte aligned,
+ * used by this call alone until it has run (calls that can run at the same
+ * time, captured graphs among them, need one each). B = 0 does nothing. The
+ * result does not depend on what else runs: no atomics, one order of sums. */
+long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H);
+int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, long long q_stride,
+                const int* slots, const int* lens, int longest, int B, int T, int H,
+                float scale, void* out, void* ws, long long ws_bytes, int* dev_status,
+                void* stream);
+
 /* Bytes of device memory the handle holds (store + workspace). */
 long long jl_moe_device_bytes(const jl_moe* h);
 

@@ -196,3 +196,29 @@ int jl_repack_bf16_part(const uint16_t* src, int p, const jl_moe* h, uint8_t* re
 size_t jl_tc_ws_bytes(int Bmax, int E, int k, int d, int m, size_t* xc_plane, size_t* ac_plane);
 int jl_launch_gateup_tc(const jl_moe* h, const uint8_t* store_l, const float* x, int B, cudaStream_t s);
 int jl_launch_down_tc(const jl_moe* h, const uint8_t* store_l, int B, cudaStream_t s);
+
+// jl_kv4.cu / jl_kv4_attn.cu: the 4-bit KV cache.
+namespace jl {
+struct kv4_dims;
+}
+// The checked view of layer l of a cache (JL_ERR_INVALID for a bad one).
+int jl_kv4_view(const jl_kv4* c, int l, jl::kv4_dims* out);
+
+// One attention call (device pointers). The B sequences' T query rows each are
+// rows q + (b * T + i) * q_stride of [H][hd]; out is [B][T][H][hd] of q's type.
+// lens[b] + len_add positions of slot slots[b] are cached, at most `longest`;
+// query i sees the first lens[b] + len_add - T + 1 + i of them.
+struct jl_kv4_attn_args {
+    const void* q;
+    long long q_stride;
+    const int* slots;
+    const int* lens;
+    void* out;
+    float* outT;   // fp32 column-major copy [H * hd][outT_ld] of the output, or null
+    void* ws;      // jl_kv4_attn_ws_bytes
+    int* err;      // status word (kErrKvIndex), or null
+    float scale;
+    int dtype, len_add, longest, B, T, H, outT_ld;
+};
+long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H);
+int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);

@@ -25,6 +25,7 @@ ERRORS = {
 }
 PATH_AUTO, PATH_EXACT, PATH_TC, PATH_GEMV = 0, 1, 2, 3
 CREATE_ROUTER_ONLY = 1
+F32, F16, BF16 = 0, 1, 2
 
 
 class JouleError(RuntimeError):
@@ -63,6 +64,11 @@ class KernelW(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in _W_PTRS] + [
         ("expert_pk", ctypes.c_void_p * 3), ("expert_sc", ctypes.c_void_p * 3),
         ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("use_i8", ctypes.c_int)]
+
+
+class Kv4(ctypes.Structure):
+    """A 4-bit KV cache (jl_kv4 in joule_moe.h)."""
+    _fields_ = [("base", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in ("slots", "L", "n_kv", "hd", "maxT")]
 
 
 _P, _I, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
@@ -123,6 +129,12 @@ SIGNATURES = {
     "spin_pool_init": ([_I], _I),
     "set_lm_threads": ([_I], None),
     "jl_decode_status": ([], _I),
+    "jl_kv4_bytes": ([ctypes.POINTER(Kv4)], _LL),
+    "jl_kv4_append": ([ctypes.POINTER(Kv4), _I, _P, _P, _I, _LL, _LL, _P, _P, _I, _P, _P], _I),
+    "jl_kv4_read": ([ctypes.POINTER(Kv4), _I, _P, _P, _I, _P, _P, _I, _P, _P], _I),
+    "jl_kv4_attn_ws": ([ctypes.POINTER(Kv4), _I, _I, _I], _LL),
+    "jl_kv4_attn": ([ctypes.POINTER(Kv4), _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _LL,
+                     _P, _P], _I),
     "jl_version": ([], ctypes.c_char_p),
     "jl_last_cuda_error": ([], ctypes.c_char_p),
 }
