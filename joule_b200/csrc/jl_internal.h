@@ -122,7 +122,7 @@ int jl_moe_layer_done(jl_moe* h, int l, cudaStream_t s);
 // callers from several host threads are serialised. key < 32.
 enum {
     kOnceExact = 0, kOnceRouter, kOnceRouterFast, kOnceDispatch, kOnceGemm, kOnceTc, kOnceGemv,
-    kOnceDecode, kOnceEp, kOnceBf16, kOnceMmBf16, kOnceMmF32, kOnceAttn
+    kOnceDecode, kOnceEp, kOnceBf16, kOnceMmBf16, kOnceMmF32, kOnceAttn, kOnceKv4
 };
 int jl_device_once(int key, int (*setup)());
 
