@@ -84,6 +84,18 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     lo = h2bits(__floats2half2_rn((x - f.x) * kLoScale, (y - f.y) * kLoScale));
 }
 
+// n - 8 of the nibbles at bits 0-3 (even) or 4-7 (odd) of both halves, exactly,
+// as fp16: 1024 + n (1024 + 16 n) by its bits, then one packed sum (FMA).
+__device__ __forceinline__ uint32_t code_even(uint32_t x) {
+    x = (x & 0x000F000Fu) | 0x64006400u;
+    return h2bits(__hsub2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(1032.0f, 1032.0f)));
+}
+__device__ __forceinline__ uint32_t code_odd(uint32_t x) {
+    x = (x & 0x00F000F0u) | 0x64006400u;
+    return h2bits(__hfma2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f),
+                          __floats2half2_rn(-72.0f, -72.0f)));
+}
+
 // Blocks of sequence b (0 when its slot or length is outside the cache), and
 // what it counts in the cut: its blocks, or 1 when segments are not cut.
 struct kv4_seqs {
@@ -155,7 +167,6 @@ template <int HD>
 struct kv4_state {
     static constexpr int NG = HD / 64;
     uint32_t qf[NG * 4][4];   // q fragments per k step of 16 values
-    float cinit[NG];          // -8 * sum of the row's q over the group, in units of 2^-24
     float f;                  // accumulator -> score in base 2
     float o[NG][8][4];        // o[g][j][c], [2 + c]: hi, lo sums of value 64 g + 8 (2 t + c) + j
     float m, l;
@@ -181,29 +192,22 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
     int e = (int)(__float_as_uint(mx) >> 23);
     e = e == 0 ? 127 : min(e, 253);
     const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    st.f = scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23) * 16777216.0f;
+    st.f = scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-        float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 2; w++) {
             float (&v)[8] = x[g][w];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[j] *= inv;
-                sum += v[j];
-            }
-            // nibbles j and j + 4 of a word share a half pair; those at bits 4-7 count 16 fold
+            for (int j = 0; j < 8; j++) v[j] *= inv;
+            // nibbles j and j + 4 of a word share a half pair
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 uint32_t (&a)[4] = st.qf[g * 4 + w * 2 + s];
                 split2(v[2 * s], v[2 * s + 4], a[0], a[1]);
-                split2(v[2 * s + 1] * 0.0625f, v[2 * s + 5] * 0.0625f, a[2], a[3]);
+                split2(v[2 * s + 1], v[2 * s + 5], a[2], a[3]);
             }
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        st.cinit[g] = sum * (-8.0f / 16777216.0f);
 #pragma unroll
         for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -215,12 +219,10 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
 
 // One block of 64 positions (j0 = its first) against the tile.
 //
-// Scores: a code nibble n left where it lies is the fp16 subnormal n 2^-24 (or
-// n 2^-20 at bits 4-7, undone in q), so K takes one AND per two values; the
-// code's offset of 8 is the accumulator's start. V: (n - 8) exactly, by one
-// AND-OR into 1024's mantissa and one packed FMA per two values, because the
-// offset's sum would be far larger than the result. K's scale multiplies the
-// accumulated group, V's the weight, both in fp32.
+// Codes become n - 8 exactly, by one AND-OR into 1024's mantissa and one packed
+// fp16 sum per two values (the offset's own sum would be far larger than the
+// results'). K's scale multiplies the accumulated group, V's the weight, both in
+// fp32.
 template <int HD, bool MASK>
 __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0) {
     constexpr int NG = HD / 64, ROW = HD / 2;
@@ -240,8 +242,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
         }
 #pragma unroll
         for (int gr = 0; gr < NG; gr++) {
-            acc[gr][0] = acc[gr][1] = st.cinit[gr];
-            acc[gr][2] = acc[gr][3] = 0.0f;
+            acc[gr][0] = acc[gr][1] = acc[gr][2] = acc[gr][3] = 0.0f;
         }
 #pragma unroll
         for (int w = 0; w < 2; w++)
@@ -251,7 +252,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
                 for (int gr = 0; gr < NG; gr++) {
                     const uint32_t x = sh ? kw[w * NG + gr] >> 8 : kw[w * NG + gr];
                     const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
-                    mma16816(acc[gr], a[0], a[1], a[2], a[3], x & 0x000F000Fu, x & 0x00F000F0u);
+                    mma16816(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
                 }
         // scales of keys 2t, 2t + 1
         float sc[2][NG];
@@ -341,16 +342,6 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
                 vw[r][0] = *reinterpret_cast<const uint32_t*>(p);
             }
         }
-        const __half2 k1032 = __floats2half2_rn(1032.0f, 1032.0f), k72 = __floats2half2_rn(-72.0f, -72.0f),
-                      k16th = __floats2half2_rn(0.0625f, 0.0625f);
-        auto odd = [&](uint32_t x) {  // 1024 + 16 n -> n - 8
-            x = (x & 0x00F000F0u) | 0x64006400u;
-            return h2bits(__hfma2(*reinterpret_cast<__half2*>(&x), k16th, k72));
-        };
-        auto even = [&](uint32_t x) {  // 1024 + n -> n - 8
-            x = (x & 0x000F000Fu) | 0x64006400u;
-            return h2bits(__hsub2(*reinterpret_cast<__half2*>(&x), k1032));
-        };
 #pragma unroll
         for (int gr = 0; gr < NG; gr++)
 #pragma unroll
@@ -359,8 +350,8 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
                 uint32_t y = __byte_perm(vw[2][gr], vw[3][gr], q ? 0x7632 : 0x5410);
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    mma16816(st.o[gr][4 * q + 2 * p], a[gr][0], a[gr][1], a[gr][2], a[gr][3], even(x), even(y));
-                    mma16816(st.o[gr][4 * q + 2 * p + 1], a[gr][0], a[gr][1], a[gr][2], a[gr][3], odd(x), odd(y));
+                    mma16816(st.o[gr][4 * q + 2 * p], a[gr][0], a[gr][1], a[gr][2], a[gr][3], code_even(x), code_even(y));
+                    mma16816(st.o[gr][4 * q + 2 * p + 1], a[gr][0], a[gr][1], a[gr][2], a[gr][3], code_odd(x), code_odd(y));
                     x >>= 8;
                     y >>= 8;
                 }
