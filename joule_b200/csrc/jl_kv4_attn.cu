@@ -20,10 +20,13 @@
 
 namespace jl {
 
-constexpr int kKvWarps = 8;    // warps per block, one block per SM
-constexpr int kKvRing = 3;     // cache blocks in a warp's ring
+constexpr int kKvRing = 2;     // cache blocks in a warp's ring
 constexpr int kKvTile = 8;     // query rows of a tile
 constexpr float kLoScale = 2048.0f;
+// A new reference is 2^kHeadroom above the largest score, so that weights stay
+// at or below 1 without a rescaling of the sums at every new maximum (most blocks
+// of a short run have one in some row).
+constexpr float kHeadroom = 4.0f;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -75,23 +78,46 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// (x, y) as fp16 pairs: hi = the nearest, lo = 2048 times what hi misses, so
+__device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
+
+// A pair as fp16 pairs: hi = the nearest, lo = 2048 times what hi misses, so
 // that hi + lo / 2048 holds 22 bits and lo does not underflow before hi does.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __float22half2_rn(x);
     hi = h2bits(h);
-    lo = h2bits(__floats2half2_rn((x - f.x) * kLoScale, (y - f.y) * kLoScale));
+    lo = h2bits(__float22half2_rn(__ffma2_rn(__half22float2(h), f2(-kLoScale), __fmul2_rn(x, f2(kLoScale)))));
+}
+
+// The scales of positions r, r + 1 of a section: per group a pair over the two.
+template <int NG>
+__device__ __forceinline__ void scale_pairs(const uint8_t* section, int r, float2 (&sc)[NG]) {
+    const uint8_t* p = section + r * 2 * NG;
+    if (NG == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+        sc[0] = make_float2(a.x, b.x);
+        sc[NG - 1] = make_float2(a.y, b.y);
+    } else {
+        sc[0] = __half22float2(*reinterpret_cast<const __half2*>(p));
+    }
 }
 
 // n - 8 of the nibbles at bits 0-3 (even) or 4-7 (odd) of both halves, exactly,
-// as fp16: 1024 + n (1024 + 16 n) by its bits, then one packed sum (FMA).
+// as fp16: 1024 + n (1024 + 16 n) by its bits, then one packed sum (FMA). The
+// and-or is one instruction only when written as lop3 (measured: 256 fewer of
+// 1,590 instructions per block, on the pipe that is busiest).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(m), "r"(o));
+    return y;
+}
 __device__ __forceinline__ uint32_t code_even(uint32_t x) {
-    x = (x & 0x000F000Fu) | 0x64006400u;
+    x = and_or(x, 0x000F000Fu, 0x64006400u);
     return h2bits(__hsub2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(1032.0f, 1032.0f)));
 }
 __device__ __forceinline__ uint32_t code_odd(uint32_t x) {
-    x = (x & 0x00F000F0u) | 0x64006400u;
+    x = and_or(x, 0x00F000F0u, 0x64006400u);
     return h2bits(__hfma2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f),
                           __floats2half2_rn(-72.0f, -72.0f)));
 }
@@ -113,22 +139,22 @@ struct kv4_seqs {
 // The sum of weights over all sequences, and the sequence that holds unit u
 // when a sequence has S segments of its weight: b and the unit's offset in it
 // (b = B when u is past the end). Called by a whole warp.
-__device__ __forceinline__ long long warp_total(const kv4_seqs& q, int B) {
-    long long n = 0;
+__device__ __forceinline__ uint32_t warp_total(const kv4_seqs& q, int B) {
+    uint32_t n = 0;
     for (int b = threadIdx.x & 31; b < B; b += 32) n += q.weight(b);
 #pragma unroll
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
-__device__ __forceinline__ void warp_find(const kv4_seqs& q, int B, int S, long long u, int& b_out, long long& off) {
+__device__ __forceinline__ void warp_find(const kv4_seqs& q, int B, uint32_t S, uint32_t u, int& b_out, uint32_t& off) {
     const int lane = threadIdx.x & 31;
-    long long base = 0;
+    uint32_t base = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
-        const long long n = b0 + lane < B ? (long long)q.weight(b0 + lane) * S : 0;
-        long long inc = n;
+        const uint32_t n = b0 + lane < B ? q.weight(b0 + lane) * S : 0;
+        uint32_t inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         const uint32_t past = __ballot_sync(0xffffffffu, base + inc > u);
@@ -144,19 +170,48 @@ __device__ __forceinline__ void warp_find(const kv4_seqs& q, int B, int S, long 
     off = 0;
 }
 
-// Units per warp: the same on every warp and in k_kv4_merge.
-__device__ __forceinline__ long long units_per_warp(long long U, int W) { return (U + W - 1) / W; }
+// n units in `parts` runs whose sizes differ by one at most, the longer first:
+// run i begins at start(i), and unit u is in run of(u). No run is empty when
+// parts <= n.
+struct kv4_split {
+    uint32_t parts, q, r;
+    __device__ kv4_split(uint32_t n, uint32_t parts_) : parts(parts_), q(n / parts_), r(n - n / parts_ * parts_) {}
+    __device__ uint32_t start(uint32_t i) const { return i * q + min(i, r); }
+    __device__ uint32_t of(uint32_t u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+
+// The cut of U units over at most `blocks` blocks of NW warps: ctas blocks take
+// a share each and nw of a block's warps share that alike, in order (few units
+// spread over all blocks first). U >= 1.
+struct kv4_cut {
+    uint32_t ctas, nw;
+    kv4_split by_block;
+    __device__ kv4_cut(uint32_t U, uint32_t blocks, uint32_t NW)
+        : ctas(min(blocks, U)), nw(min(NW, U / min(blocks, U))), by_block(U, min(blocks, U)) {}
+    __device__ uint32_t start(uint32_t c) const { return by_block.start(c); }
+    __device__ kv4_split by_warp(uint32_t c) const { return kv4_split(start(c + 1) - start(c), nw); }
+    __device__ uint32_t warp_of(uint32_t u) const {  // nw * block + warp
+        const uint32_t c = by_block.of(u);
+        return c * nw + by_warp(c).of(u - start(c));
+    }
+};
 
 // A partial result in the workspace: O [8][HD], m [8], l [8] (fp32, base-2
 // exponents). Warp w's part 0 belongs to the segment that began before its run,
-// part 1 to the one that goes on past it.
+// part 1 to the one that begins in it and goes on past it. Where all warps of a
+// block are inside one segment, the block's first warp holds their sum.
 __host__ __device__ constexpr int kv4_part_floats(int hd) { return kKvTile * hd + 2 * kKvTile; }
 
+// Warps of a block (one block per SM): as many as the registers of a tile's
+// sums and the ring of whole blocks allow. 128: 12 warps of 168 registers, 209 KB.
+__host__ __device__ constexpr int kv4_warps(int hd) { return hd == 128 ? 12 : 16; }
 template <int HD>
 struct kv4_smem {
-    static constexpr int BLK = 68 * HD;
-    static constexpr int bars = kKvWarps * kKvRing * BLK;
-    static constexpr int total = bars + kKvWarps * kKvRing * 8;
+    static constexpr int BLK = 68 * HD, NW = kv4_warps(HD);
+    static constexpr int bars = NW * kKvRing * BLK;
+    static constexpr int stat = bars + NW * kKvRing * 8;      // m, l [NW][8] of the block's sum
+    static constexpr int total = stat + NW * 2 * kKvTile * 4;
+    static_assert(kKvRing * BLK >= kKvTile * HD * 4, "a warp's ring holds its sums");
 };
 
 // One warp's running state for the segment it is in. The matrix instruction's
@@ -167,9 +222,10 @@ template <int HD>
 struct kv4_state {
     static constexpr int NG = HD / 64;
     uint32_t qf[NG * 4][4];   // q fragments per k step of 16 values
-    float f;                  // accumulator -> score in base 2
+    float f;                  // accumulator -> score in base 2 (a power of two)
     float o[NG][8][4];        // o[g][j][c], [2 + c]: hi, lo sums of value 64 g + 8 (2 t + c) + j
-    float m, l;
+    float m;                  // reference of the exponents, in the accumulator's units: no score is above it
+    float2 l;                 // this thread's sum of weights
     int n;                    // positions that row g sees
 };
 
@@ -184,7 +240,10 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
         for (int w = 0; w < 2; w++) {
             load8(q + g * 64 + 16 * t + 8 * w, x[g][w]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[g][w][j]));
+            for (int j = 0; j < 8; j++) {
+                x[g][w][j] *= scale * 1.4426950408889634f;
+                mx = fmaxf(mx, fabsf(x[g][w][j]));
+            }
         }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -192,7 +251,7 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
     int e = (int)(__float_as_uint(mx) >> 23);
     e = e == 0 ? 127 : min(e, 253);
     const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    st.f = scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23);
+    st.f = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
 #pragma unroll
@@ -204,8 +263,8 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 uint32_t (&a)[4] = st.qf[g * 4 + w * 2 + s];
-                split2(v[2 * s], v[2 * s + 4], a[0], a[1]);
-                split2(v[2 * s + 1], v[2 * s + 5], a[2], a[3]);
+                split2(make_float2(v[2 * s], v[2 * s + 4]), a[0], a[1]);
+                split2(make_float2(v[2 * s + 1], v[2 * s + 5]), a[2], a[3]);
             }
         }
 #pragma unroll
@@ -214,7 +273,7 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
             for (int c = 0; c < 4; c++) st.o[g][j][c] = 0.0f;
     }
     st.m = -INFINITY;
-    st.l = 0.0f;
+    st.l = f2(0.0f);
 }
 
 // One block of 64 positions (j0 = its first) against the tile.
@@ -223,13 +282,19 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
 // fp16 sum per two values (the offset's own sum would be far larger than the
 // results'). K's scale multiplies the accumulated group, V's the weight, both in
 // fp32.
+// MASK: the block reaches past what some row sees; pieces of it that no row sees
+// (n_max) are passed over.
 template <int HD, bool MASK>
-__device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0) {
+__device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_max) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float s[8][2];
+    float2 s[8];
 #pragma unroll
     for (int nt = 0; nt < 8; nt++) {
+        if (MASK && j0 + nt * 8 >= n_max) {
+            s[nt] = f2(-INFINITY);
+            continue;
+        }
         float acc[NG][4];
         uint32_t kw[NG * 2];
         const uint8_t* kp = blk + (nt * 8 + g) * ROW + t * 8 * NG;
@@ -241,9 +306,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
             kw[0] = w.x, kw[1] = w.y;
         }
 #pragma unroll
-        for (int gr = 0; gr < NG; gr++) {
-            acc[gr][0] = acc[gr][1] = acc[gr][2] = acc[gr][3] = 0.0f;
-        }
+        for (int gr = 0; gr < NG; gr++) acc[gr][0] = acc[gr][1] = acc[gr][2] = acc[gr][3] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 2; w++)
 #pragma unroll
@@ -254,82 +317,65 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
                     const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
                     mma16816(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
                 }
-        // scales of keys 2t, 2t + 1
-        float sc[2][NG];
-        const uint8_t* sp = blk + kv4_kscale(HD) + (nt * 8 + 2 * t) * 2 * NG;
-        if (NG == 2) {
-            const uint2 w = *reinterpret_cast<const uint2*>(sp);
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-            sc[0][0] = a.x, sc[0][NG - 1] = a.y, sc[1][0] = b.x, sc[1][NG - 1] = b.y;
-        } else {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(sp));
-            sc[0][0] = a.x, sc[1][0] = a.y;
-        }
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            float v = sc[c][0] * fmaf(acc[0][2 + c], 1.0f / kLoScale, acc[0][c]);
-            if (NG == 2) v = fmaf(sc[c][NG - 1], fmaf(acc[NG - 1][2 + c], 1.0f / kLoScale, acc[NG - 1][c]), v);
-            v *= st.f;
-            if (MASK && j0 + nt * 8 + 2 * t + c >= st.n) v = -INFINITY;
-            s[nt][c] = v;
+        float2 sc[NG];
+        scale_pairs<NG>(blk + kv4_kscale(HD), nt * 8 + 2 * t, sc);
+        s[nt] = __fmul2_rn(sc[0], __ffma2_rn(make_float2(acc[0][2], acc[0][3]), f2(1.0f / kLoScale),
+                                             make_float2(acc[0][0], acc[0][1])));
+        if (NG == 2)
+            s[nt] = __ffma2_rn(sc[NG - 1], __ffma2_rn(make_float2(acc[NG - 1][2], acc[NG - 1][3]), f2(1.0f / kLoScale),
+                                                      make_float2(acc[NG - 1][0], acc[NG - 1][1])), s[nt]);
+        if (MASK) {
+            if (j0 + nt * 8 + 2 * t >= st.n) s[nt].x = -INFINITY;
+            if (j0 + nt * 8 + 2 * t + 1 >= st.n) s[nt].y = -INFINITY;
         }
     }
-    float m = s[0][0];
+    float m = fmaxf(s[0].x, s[0].y);
 #pragma unroll
-    for (int nt = 0; nt < 8; nt++) m = fmaxf(m, fmaxf(s[nt][0], s[nt][1]));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = fmaxf(m, st.m);
-    if (__any_sync(0xffffffffu, m > st.m)) {
-        const float al = m > st.m ? ex2(st.m - m) : 1.0f;  // st.m = -inf: 0
-        st.l *= al;
+    for (int nt = 1; nt < 8; nt++) m = fmaxf(m, fmaxf(s[nt].x, s[nt].y));
+    if (__any_sync(0xffffffffu, m > st.m)) {  // a score past the reference: all lanes of the row take a new one
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        if (m > st.m) {
+            m = fmaf(kHeadroom, 1.0f / st.f, m);
+            const float al = ex2((st.m - m) * st.f);  // st.m = -inf: 0
+            st.l = __fmul2_rn(st.l, f2(al));
 #pragma unroll
-        for (int gr = 0; gr < NG; gr++)
+            for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+                for (int j = 0; j < 8; j++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) st.o[gr][j][c] *= al;
-        st.m = m;
-    }
-    const float mu = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int nt = 0; nt < 8; nt++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            s[nt][c] = ex2(s[nt][c] - mu);
-            st.l += s[nt][c];
+                    for (int c = 0; c < 4; c++) st.o[gr][j][c] *= al;
+            st.m = m;
         }
+    }
+    const float2 mf = f2(st.m == -INFINITY ? 0.0f : -st.m * st.f), ff = f2(st.f);
+#pragma unroll
+    for (int nt = 0; nt < 8; nt++) {
+        s[nt] = __ffma2_rn(s[nt], ff, mf);
+        s[nt].x = ex2(s[nt].x);
+        s[nt].y = ex2(s[nt].y);
+        st.l = __fadd2_rn(st.l, s[nt]);
+    }
     const uint8_t* vp = blk + kv4_vcode(HD) + t * ROW + (g ^ ((t & 2) << 1)) * 4 * NG;
 #pragma unroll
     for (int kk = 0; kk < 4; kk++) {
+        if (MASK && j0 + kk * 16 >= n_max) break;
         // weights times scales of positions 2t, 2t + 1 (nt even), 2t + 8, 2t + 9 (nt odd)
         uint32_t a[NG][4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int nt = 2 * kk + h;
-            float sc[2][NG];
-            const uint8_t* sp = blk + kv4_vscale(HD) + (nt * 8 + 2 * t) * 2 * NG;
-            if (NG == 2) {
-                const uint2 w = *reinterpret_cast<const uint2*>(sp);
-                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-                sc[0][0] = x.x, sc[0][NG - 1] = x.y, sc[1][0] = y.x, sc[1][NG - 1] = y.y;
-            } else {
-                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(sp));
-                sc[0][0] = x.x, sc[1][0] = x.y;
-            }
+            float2 sc[NG];
+            scale_pairs<NG>(blk + kv4_vscale(HD), nt * 8 + 2 * t, sc);
             if (MASK) {  // rows never written may hold any scale
 #pragma unroll
-                for (int c = 0; c < 2; c++)
-                    if (j0 + nt * 8 + 2 * t + c >= st.n) {
-#pragma unroll
-                        for (int gr = 0; gr < NG; gr++) sc[c][gr] = 0.0f;
-                    }
+                for (int gr = 0; gr < NG; gr++) {
+                    if (j0 + nt * 8 + 2 * t >= st.n) sc[gr].x = 0.0f;
+                    if (j0 + nt * 8 + 2 * t + 1 >= st.n) sc[gr].y = 0.0f;
+                }
             }
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++)
-                split2(s[nt][0] * sc[0][gr], s[nt][1] * sc[1][gr], a[gr][2 * h], a[gr][2 * h + 1]);
+            for (int gr = 0; gr < NG; gr++) split2(__fmul2_rn(s[nt], sc[gr]), a[gr][2 * h], a[gr][2 * h + 1]);
         }
         uint32_t vw[4][NG];  // rows 2t, 2t + 1, 2t + 8, 2t + 9 at places t, 4 + t, 8 + t, 12 + t
 #pragma unroll
@@ -360,13 +406,13 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
 }
 
 // Bound by HBM for long caches (the codes and scales are read once, 4.25 bits
-// per value) and by launch and load latency for short ones. Eight warps per
-// SM, each with a ring of three whole blocks filled by one bulk copy each, and
-// no barrier between warps.
+// per value) and by launch and load latency for short ones. Each warp has a ring
+// of two whole blocks, filled by one bulk copy each; no barrier between warps
+// but for the sum of a block that is inside one segment.
 template <int HD, typename T>
-__global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
+__global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int BLK = kv4_smem<HD>::BLK, NG = HD / 64;
+    constexpr int BLK = kv4_smem<HD>::BLK, NG = HD / 64, NW = kv4_warps(HD);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kKvRing * BLK;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kv4_smem<HD>::bars) + warp * kKvRing;
@@ -377,11 +423,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     __syncwarp();
     griddep_wait();
     griddep_launch_dependents();
-    const int W = gridDim.x * kKvWarps, wid = warp * gridDim.x + blockIdx.x;
     const int gsz = a.H / c.KH, rows = a.T * gsz, S = R * c.KH;
     const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, whole};
     // sequences without positions: zeros (and the status bit for those outside the cache)
-    for (int b = wid; b < a.B; b += W) {
+    for (int b = warp * gridDim.x + blockIdx.x; b < a.B; b += NW * gridDim.x) {
         const int n = seqs.len(b);
         if (n > 0) continue;
         if (n < 0 && lane == 0 && a.err) atomicOr(a.err, kErrKvIndex);
@@ -392,11 +437,16 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             for (long long i = lane; i < 8 * n8; i += 32)
                 a.outT[(size_t)(i % (a.H * HD)) * a.outT_ld + r0 + i / (a.H * HD)] = 0.0f;
     }
-    const long long U = warp_total(seqs, a.B) * S, per = units_per_warp(U, W), u0 = wid * per;
-    if (u0 >= U) return;
-    int units = (int)min(per, U - u0);  // blocks of this warp's run
+    const uint32_t U = warp_total(seqs, a.B) * S;
+    if (U == 0) return;
+    const kv4_cut cut(U, gridDim.x, NW);
+    if (warp >= cut.nw || blockIdx.x >= cut.ctas) return;
+    const int wid = blockIdx.x * cut.nw + warp;
+    const kv4_split mine = cut.by_warp(blockIdx.x);
+    const uint32_t c0 = cut.start(blockIdx.x), c1 = cut.start(blockIdx.x + 1), u0 = c0 + mine.start(warp);
+    int units = mine.start(warp + 1) - mine.start(warp);  // blocks of this warp's run
     int b;
-    long long off;
+    uint32_t off;
     warp_find(seqs, a.B, S, u0, b, off);
     struct cursor {
         int b, s, j, nb;
@@ -432,6 +482,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         }
     };
     cursor co = pr;
+    // the block's run is inside one segment: its warps' sums meet here
+    const uint32_t seg0 = u0 - pr.j;
+    const bool joined = !whole && cut.nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nb;
     int issued = 0;
     auto issue = [&]() {
         if (lane == 0) {
@@ -457,18 +510,19 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             n_max = max(0, len - a.T + 1 + min(rt * kKvTile + kKvTile - 1, rows - 1) / gsz);
             began = true;
         }
-        if (!mbar_wait_bounded(bar + slot_k, phase, a.err)) return;
+        if (!mbar_wait_bounded(bar + slot_k, phase, a.err)) break;  // flagged; the block's sum still meets
         const uint8_t* blk = ring + slot_k * BLK;
         const int j0 = co.j * kKv4Rows;
-        if (j0 + kKv4Rows <= n_min) kv4_block<HD, false>(st, blk, j0);
-        else if (j0 < n_max) kv4_block<HD, true>(st, blk, j0);
+        if (j0 + kKv4Rows <= n_min) kv4_block<HD, false>(st, blk, j0, n_max);
+        else if (j0 < n_max) kv4_block<HD, true>(st, blk, j0, n_max);
         fence_proxy_async_smem();
         __syncwarp();
         if (issued < units) issue();
         if (++slot_k == kKvRing) slot_k = 0, phase ^= 1;
         const bool ends = co.j == co.nb - 1;
         if (ends || i == units - 1) {
-            float lsum = st.l + __shfl_xor_sync(0xffffffffu, st.l, 1);
+            float lsum = st.l.x + st.l.y;
+            lsum += __shfl_xor_sync(0xffffffffu, lsum, 1);
             lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
             const bool from_start = i >= co.j;  // the segment's first block is in this warp's run
             if (ends && from_start) {
@@ -493,7 +547,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
                         }
                 }
             } else {
-                float* part = static_cast<float*>(a.ws) + ((size_t)wid * 2 + from_start) * kv4_part_floats(HD);
+                float* part = joined ? reinterpret_cast<float*>(ring)
+                                     : static_cast<float*>(a.ws) + ((size_t)wid * 2 + from_start) * kv4_part_floats(HD);
+                float* ml = joined ? reinterpret_cast<float*>(smem + kv4_smem<HD>::stat) + warp * 2 * kKvTile
+                                   : part + kKvTile * HD;
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++)
 #pragma unroll
@@ -504,30 +561,53 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
                         put8(part + g * HD + gr * 64 + 8 * (2 * t + cc), x);
                     }
                 if (t == 0) {
-                    part[kKvTile * HD + g] = st.m;
-                    part[kKvTile * HD + kKvTile + g] = lsum;
+                    ml[g] = st.m == -INFINITY ? st.m : st.m * st.f;
+                    ml[kKvTile + g] = lsum;
                 }
             }
             began = false;
         }
         if (i + 1 < units) advance(co);
     }
+    if (!joined) return;
+    // all cut.nw warps of the block come here: the warps' sums, in their order
+    asm volatile("bar.sync 1, %0;" ::"r"(cut.nw * 32) : "memory");
+    const float* ml = reinterpret_cast<const float*>(smem + kv4_smem<HD>::stat);
+    float* part = static_cast<float*>(a.ws) +
+                  ((size_t)blockIdx.x * cut.nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
+    for (int x = threadIdx.x; x < kKvTile * HD / 4; x += cut.nw * 32) {
+        const int r = x / (HD / 4);
+        float m = -INFINITY, lsum = 0.0f;
+        for (int w = 0; w < (int)cut.nw; w++) m = fmaxf(m, ml[w * 2 * kKvTile + r]);
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < (int)cut.nw; w++) {
+            const float f = ex2(ml[w * 2 * kKvTile + r] - mu);
+            const float4 v = reinterpret_cast<const float4*>(smem + w * kKvRing * BLK)[x];
+            lsum = fmaf(ml[w * 2 * kKvTile + kKvTile + r], f, lsum);
+            o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+        }
+        reinterpret_cast<float4*>(part)[x] = o;
+        if (x % (HD / 4) == 0) {
+            part[kKvTile * HD + r] = m;
+            part[kKvTile * HD + kKvTile + r] = lsum;
+        }
+    }
 }
 
 // Adds up the parts of segments that several warps shared: block = RB rows of
 // one segment, 8 / RB warps per row, each adding every (8 / RB)-th part.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int W, int RB) {
-    constexpr int V = HD / 32;  // values per lane
-    __shared__ float sums[8][HD];
+__global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int ctas, int RB) {
+    constexpr int V = HD / 32, NW = kv4_warps(HD), PF = kv4_part_floats(HD);  // V values per lane
+    __shared__ float sums[8][HD], stat[8][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    griddep_wait();
-    griddep_launch_dependents();
     const int gsz = a.H / c.KH, rows = a.T * gsz, S = R * c.KH;
     const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, 0};
+    // The attention's blocks have all passed their own wait when this kernel
+    // starts, so lens and slots are there before this kernel's wait.
     const int b = blockIdx.x / S, s = blockIdx.x % S, nb = seqs.blocks(b);
-    if (nb == 0) return;
-    long long before = 0, U = 0;
+    uint32_t before = 0, U = 0;
     for (int i = lane; i < a.B; i += 32) {
         const int n = seqs.blocks(i);
         U += n;
@@ -538,39 +618,77 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
         U += __shfl_xor_sync(0xffffffffu, U, o);
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    const long long per = units_per_warp(U * S, W), first = before * S + (long long)s * nb;
-    const int w0 = (int)(first / per), w1 = (int)((first + nb - 1) / per);
-    if (w0 == w1) return;  // one warp had it all
+    const kv4_cut cut(max(1u, U * S), ctas, NW);
+    const uint32_t first = before * S + s * nb, last = first + nb;
+    const int w0 = nb ? cut.warp_of(first) : 0, w1 = nb ? cut.warp_of(last - 1) : 0, nw = cut.nw;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (w0 == w1) return;  // nothing to add, or one warp had it all
+    // Parts: one per warp of the first and last block where these reach out of
+    // the segment, one per block in between.
+    int b0 = w0 / nw, b1 = w1 / nw + 1;  // joined blocks [b0, b1)
+    if (cut.start(b0) < first) b0++;
+    if (cut.start(b1) > last) b1--;
+    if (nw == 1 || b1 <= b0) b0 = b1 = w1 / nw + 1;
+    const int head = min(w1 + 1, b0 * nw) - w0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
     const int g = blockIdx.y * RB + warp % RB, lanes = 8 / RB, pl = warp / RB;
-    const float* ws = static_cast<const float*>(a.ws);
-    // warp w0 began the segment (its part 1), unless its run begins just there: part 1 all the same
-    auto part = [&](int w) { return ws + ((size_t)w * 2 + (w == w0)) * kv4_part_floats(HD); };
-    float m = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, part(w)[kKvTile * HD + g]);
+    const float* ws = static_cast<const float*>(a.ws) + g * HD;
+    // warp w0 began the segment: its part 1
+    auto part = [&](int i) {
+        const int w = i < head ? w0 + i : i < head + b1 - b0 ? (b0 + i - head) * nw : b1 * nw + i - head - (b1 - b0);
+        return ws + ((size_t)w * 2 + (w == w0)) * PF;
+    };
+    const int so = kKvTile * HD + g - g * HD;  // m from the row's values; l is kKvTile further
+    float m = -INFINITY, lsum = 0.0f, x[V] = {};
+    for (int i0 = pl; i0 < n; i0 += 4 * lanes) {
+        float v[4][V], pm[4], pl4[4], mx = m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mu = m == -INFINITY ? 0.0f : m;
-    float lsum = 0.0f;
-    for (int w = w0 + lane; w <= w1; w += 32)
-        lsum += part(w)[kKvTile * HD + kKvTile + g] * ex2(part(w)[kKvTile * HD + g] - mu);
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * lanes;
+            pm[k] = -INFINITY, pl4[k] = 0.0f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
-    float x[V] = {};
-#pragma unroll 4
-    for (int w = w0 + pl; w <= w1; w += lanes) {
-        const float* p = part(w);
-        const float f = ex2(p[kKvTile * HD + g] - mu);
+            for (int e = 0; e < V; e++) v[k][e] = 0.0f;
+            if (i < n) {
+                const float* p = part(i);
+                pm[k] = p[so];
+                pl4[k] = p[so + kKvTile];
 #pragma unroll
-        for (int e = 0; e < V; e++) x[e] = fmaf(p[g * HD + lane + 32 * e], f, x[e]);
+                for (int e = 0; e < V; e++) v[k][e] = p[lane + 32 * e];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) mx = fmaxf(mx, pm[k]);
+        const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
+        lsum *= al;
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] *= al;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = ex2(pm[k] - mu);
+            lsum = fmaf(pl4[k], f, lsum);
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] = fmaf(v[k][e], f, x[e]);
+        }
+        m = mx;
     }
     if (lanes > 1) {
 #pragma unroll
         for (int e = 0; e < V; e++) sums[warp][lane + 32 * e] = x[e];
+        if (lane == 0) stat[warp][0] = m, stat[warp][1] = lsum;
         __syncthreads();
         if (pl) return;
-        for (int w = 1; w < lanes; w++)
+        float mx = m;
+        for (int w = 1; w < lanes; w++) mx = fmaxf(mx, stat[warp + w * RB][0]);
+        const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
+        lsum *= al;
 #pragma unroll
-            for (int e = 0; e < V; e++) x[e] += sums[warp + w * RB][lane + 32 * e];
+        for (int e = 0; e < V; e++) x[e] *= al;
+        for (int w = 1; w < lanes; w++) {
+            const float f = ex2(stat[warp + w * RB][0] - mu);
+            lsum = fmaf(stat[warp + w * RB][1], f, lsum);
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] = fmaf(sums[warp + w * RB][lane + 32 * e], f, x[e]);
+        }
     }
     const int row = s % R * kKvTile + g;
     if (row >= rows) return;
@@ -616,16 +734,15 @@ int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream
     const int sms = std::min(sm_count(), kMaxSms), R = row_tiles(c, a.T, a.H);
     if (sms < 1) return JL_ERR_CUDA;
     const long long segs = (long long)a.B * R * c.KH;
-    if (segs > INT_MAX) return JL_ERR_INVALID;
+    if (segs > INT_MAX || segs * c.nb > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
     // Segments of at most 4 blocks are not cut: a warp takes that many sooner
     // than a second kernel starts.
     const int whole = a.longest <= 4 * kKv4Rows;
-    const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kKvWarps * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
+    const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kv4_warps(HD) * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
                           whole);
     if (rc || whole) return rc;
-    const int RB = segs >= 2 * sms ? 8 : segs * 4 >= 2 * sms ? 2 : 1;
-    return launch(k_kv4_merge<HD, T>, dim3((unsigned)segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms * kKvWarps,
-                  RB);
+    const int RB = segs >= sms ? 8 : segs * 4 >= sms ? 2 : 1;
+    return launch(k_kv4_merge<HD, T>, dim3((unsigned)segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB);
 }
 
 template <int HD>
@@ -639,7 +756,7 @@ int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStrea
 
 // Two parts for each warp that has blocks.
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
-    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kKvWarps;
+    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kv4_warps(c.hd);
     const long long n = segs >= warps ? warps : std::min(warps, segs * c.nb);
     return n * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float);
 }
