@@ -20,13 +20,13 @@
 
 namespace jl {
 
-constexpr int kKvRing = 2;     // cache blocks in a warp's ring
+constexpr int kKvUnit = kKv4Rows;  // positions that a warp takes at a time: a cache block
+constexpr int kKvRing = 2;     // units in a warp's ring
 constexpr int kKvTile = 8;     // query rows of a tile
-constexpr float kLoScale = 2048.0f;
-// A new reference is 2^kHeadroom above the largest score, so that weights stay
-// at or below 1 without a rescaling of the sums at every new maximum (most blocks
-// of a short run have one in some row).
-constexpr float kHeadroom = 4.0f;
+// Weights times V's scales are kept at or below 2^kTop in fp16; a new reference
+// puts the largest at 2^(kTop - kHeadroom), so that the sums are not rescaled at
+// every new maximum (most units of a short run have one in some row).
+constexpr float kTop = 15.0f, kHeadroom = 4.0f;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -76,17 +76,26 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same onto zeros.
+__device__ __forceinline__ void mma16816_0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                           uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-__device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
-
-// A pair as fp16 pairs: hi = the nearest, lo = 2048 times what hi misses, so
-// that hi + lo / 2048 holds 22 bits and lo does not underflow before hi does.
+// A pair as fp16 pairs, hi the nearest and lo what hi misses: 22 bits down to
+// fp16's smallest steps of 2^-24 (callers scale what they split to 2^10 and more).
 __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __float22half2_rn(x);
+    const float2 f = __half22float2(h);
     hi = h2bits(h);
-    lo = h2bits(__float22half2_rn(__ffma2_rn(__half22float2(h), f2(-kLoScale), __fmul2_rn(x, f2(kLoScale)))));
+    lo = h2bits(__float22half2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y))));
 }
+
+__device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
 
 // The scales of positions r, r + 1 of a section: per group a pair over the two.
 template <int NG>
@@ -122,8 +131,8 @@ __device__ __forceinline__ uint32_t code_odd(uint32_t x) {
                           __floats2half2_rn(-72.0f, -72.0f)));
 }
 
-// Blocks of sequence b (0 when its slot or length is outside the cache), and
-// what it counts in the cut: its blocks, or 1 when segments are not cut.
+// Units of sequence b (0 when its slot or length is outside the cache), and
+// what it counts in the cut: its units, or 1 when segments are not cut.
 struct kv4_seqs {
     const int* slots;
     const int* lens;
@@ -132,8 +141,8 @@ struct kv4_seqs {
         const int n = __ldg(lens + b) + len_add, s = __ldg(slots + b);
         return s >= 0 && s < nslots && n >= 0 && n <= longest ? n : -1;
     }
-    __device__ int blocks(int b) const { return (max(0, len(b)) + kKv4Rows - 1) / kKv4Rows; }
-    __device__ int weight(int b) const { return whole ? len(b) > 0 : blocks(b); }
+    __device__ int units(int b) const { return (max(0, len(b)) + kKvUnit - 1) / kKvUnit; }
+    __device__ int weight(int b) const { return whole ? len(b) > 0 : units(b); }
 };
 
 // The sum of weights over all sequences, and the sequence that holds unit u
@@ -196,37 +205,40 @@ struct kv4_cut {
     }
 };
 
-// A partial result in the workspace: O [8][HD], m [8], l [8] (fp32, base-2
-// exponents). Warp w's part 0 belongs to the segment that began before its run,
-// part 1 to the one that begins in it and goes on past it. Where all warps of a
-// block are inside one segment, the block's first warp holds their sum.
+// A partial result in the workspace: O [8][HD], then per row the reference of its
+// exponents (base 2) and its sum of weights. Warp w's part 0 belongs to the segment
+// that began before its run, part 1 to the one that begins in it and goes on past
+// it. Where all warps of a block are inside one segment, the block's first warp
+// holds their sum.
 __host__ __device__ constexpr int kv4_part_floats(int hd) { return kKvTile * hd + 2 * kKvTile; }
 
-// Warps of a block (one block per SM): as many as the registers of a tile's
-// sums and the ring of whole blocks allow. 128: 12 warps of 168 registers, 209 KB.
-__host__ __device__ constexpr int kv4_warps(int hd) { return hd == 128 ? 12 : 16; }
+constexpr int kKvWarps = 12;  // warps per block, one block per SM (168 registers a thread, 209 KB at hd = 128)
 template <int HD>
 struct kv4_smem {
-    static constexpr int BLK = 68 * HD, NW = kv4_warps(HD);
-    static constexpr int bars = NW * kKvRing * BLK;
-    static constexpr int stat = bars + NW * kKvRing * 8;      // m, l [NW][8] of the block's sum
-    static constexpr int total = stat + NW * 2 * kKvTile * 4;
-    static_assert(kKvRing * BLK >= kKvTile * HD * 4, "a warp's ring holds its sums");
+    static constexpr int UNIT = kv4_block_bytes(HD);
+    static constexpr int bars = kKvWarps * kKvRing * UNIT;
+    static constexpr int stat = bars + kKvWarps * kKvRing * 8;     // reference, sum [warps][2][8] of the block's sum
+    static constexpr int total = stat + kKvWarps * 2 * kKvTile * 4;
+    static_assert(kKvRing * UNIT >= kKvTile * HD * 4, "a warp's ring holds its sums");
 };
 
-// One warp's running state for the segment it is in. The matrix instruction's
-// 16 rows are the tile's 8 query rows twice: rows 0-7 the hi parts of q (and of
-// the weights), rows 8-15 the lo parts, so a 22-bit operand costs no further
-// instruction. Thread (g, t) = (lane / 4, lane % 4) holds row g.
+// One warp's running state for the segment it is in. Both operands that are not
+// codes enter as hi and lo parts of 11 bits each. Scores are S = q K^T with q's hi
+// parts in the instruction's rows 0-7 and its lo parts in rows 8-15 (one instruction
+// for both); values are O^T = V^T P^T with the 8 rows of the tile as the columns (an
+// instruction each for hi and lo, onto the same 32 registers of sums). A thread's
+// scores are then where the second product wants its weights: thread (g, t) =
+// (lane / 4, lane % 4) has row g at positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, and
+// sums of rows 2 t and 2 t + 1.
 template <int HD>
 struct kv4_state {
     static constexpr int NG = HD / 64;
-    uint32_t qf[NG * 4][4];   // q fragments per k step of 16 values
-    float f;                  // accumulator -> score in base 2 (a power of two)
-    float o[NG][8][4];        // o[g][j][c], [2 + c]: hi, lo sums of value 64 g + 8 (2 t + c) + j
-    float m;                  // reference of the exponents, in the accumulator's units: no score is above it
-    float2 l;                 // this thread's sum of weights
-    int n;                    // positions that row g sees
+    uint32_t qf[NG * 4][4];  // q of row g per step of 16 values
+    float f;                 // accumulator -> score in base 2 (a power of two)
+    float ref;               // reference of row g's exponents, base 2
+    float2 l;                // this thread's sum of row g's weights
+    float o[NG][4][4];       // o[gr][i][c]: value 64 gr + 8 g + 2 i + c / 2 of row 2 t + c % 2
+    int n;                   // positions that row g sees
 };
 
 template <int HD, typename T>
@@ -247,11 +259,11 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
         }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // q by a power of two so that its largest value is in [1, 2): fp16 has room for the rest
+    // q by a power of two so that its largest value is in [2^10, 2^11)
     int e = (int)(__float_as_uint(mx) >> 23);
-    e = e == 0 ? 127 : min(e, 253);
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    st.f = __uint_as_float((uint32_t)e << 23);
+    e = min(max(e, 11), 253);
+    const float inv = __uint_as_float((uint32_t)(264 - e) << 23);
+    st.f = __uint_as_float((uint32_t)(e - 10) << 23);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
 #pragma unroll
@@ -268,154 +280,187 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) st.o[g][j][c] = 0.0f;
+            for (int c = 0; c < 4; c++) st.o[g][i][c] = 0.0f;
     }
-    st.m = -INFINITY;
+    st.ref = -INFINITY;
     st.l = f2(0.0f);
 }
 
-// One block of 64 positions (j0 = its first) against the tile.
-//
-// Codes become n - 8 exactly, by one AND-OR into 1024's mantissa and one packed
-// fp16 sum per two values (the offset's own sum would be far larger than the
-// results'). K's scale multiplies the accumulated group, V's the weight, both in
-// fp32.
-// MASK: the block reaches past what some row sees; pieces of it that no row sees
-// (n_max) are passed over.
-template <int HD, bool MASK>
-__device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_max) {
+// Scores in base 2 of positions r0 .. r0 + 7 of a block: s = those of r0 + 2 t and
+// r0 + 2 t + 1. Codes become n - 8 exactly, by one AND-OR into 1024's mantissa and
+// one packed fp16 sum per two values (the offset's own sum would be far larger than
+// the results'). K's scale multiplies the accumulated group in fp32.
+template <int HD>
+__device__ __forceinline__ float2 kv4_scores(const kv4_state<HD>& st, const uint8_t* blk, int r0) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float2 s[8];
+    float acc[NG][4];
+    uint32_t kw[NG * 2];
+    const uint8_t* kp = blk + (r0 + g) * ROW + t * 8 * NG;
+    if (NG == 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(kp);
+        kw[0] = w.x, kw[1] = w.y, kw[NG] = w.z, kw[2 * NG - 1] = w.w;
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(kp);
+        kw[0] = w.x, kw[1] = w.y;
+    }
 #pragma unroll
-    for (int nt = 0; nt < 8; nt++) {
-        if (MASK && j0 + nt * 8 >= n_max) {
-            s[nt] = f2(-INFINITY);
-            continue;
-        }
-        float acc[NG][4];
-        uint32_t kw[NG * 2];
-        const uint8_t* kp = blk + (nt * 8 + g) * ROW + t * 8 * NG;
-        if (NG == 2) {
-            const uint4 w = *reinterpret_cast<const uint4*>(kp);
-            kw[0] = w.x, kw[1] = w.y, kw[NG] = w.z, kw[2 * NG - 1] = w.w;
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(kp);
-            kw[0] = w.x, kw[1] = w.y;
-        }
+    for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int gr = 0; gr < NG; gr++) acc[gr][0] = acc[gr][1] = acc[gr][2] = acc[gr][3] = 0.0f;
+        for (int sh = 0; sh < 2; sh++)
 #pragma unroll
-        for (int w = 0; w < 2; w++)
+            for (int gr = 0; gr < NG; gr++) {
+                const uint32_t x = sh ? kw[w * NG + gr] >> 8 : kw[w * NG + gr];
+                const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
+                if (w + sh == 0) mma16816_0(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
+                else mma16816(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
+            }
+    float2 sc[NG];
+    scale_pairs<NG>(blk + kv4_kscale(HD), r0 + 2 * t, sc);
+    float2 s = __fmul2_rn(sc[0], __fadd2_rn(make_float2(acc[0][0], acc[0][1]), make_float2(acc[0][2], acc[0][3])));
+    if (NG == 2)
+        s = __ffma2_rn(sc[NG - 1], __fadd2_rn(make_float2(acc[NG - 1][0], acc[NG - 1][1]),
+                                              make_float2(acc[NG - 1][2], acc[NG - 1][3])), s);
+    return __fmul2_rn(s, f2(st.f));
+}
+
+// A weight past the limit (or the first of a row): its row takes a new reference,
+// and its sums are brought to it. mx: this thread's largest score of row g.
+template <int HD>
+__device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, float top) {
+    const int t = threadIdx.x & 3;
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    float al = 1.0f;
+    if (mx - st.ref > kTop - top) {
+        mx += top - (kTop - kHeadroom);
+        al = ex2(st.ref - mx);  // the first time: 0
+        st.ref = mx;
+    }
+    st.l = __fmul2_rn(st.l, f2(al));
+    const float2 ac = make_float2(__shfl_sync(0xffffffffu, al, 8 * t), __shfl_sync(0xffffffffu, al, 8 * t + 4));
 #pragma unroll
-            for (int sh = 0; sh < 2; sh++)
+    for (int gr = 0; gr < HD / 64; gr++)
 #pragma unroll
-                for (int gr = 0; gr < NG; gr++) {
-                    const uint32_t x = sh ? kw[w * NG + gr] >> 8 : kw[w * NG + gr];
-                    const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
-                    mma16816(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
-                }
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) st.o[gr][i][c] *= c & 1 ? ac.y : ac.x;
+}
+
+// Weights of positions r0 .. r0 + 15 from their scores, and the weighted values
+// onto the sums. V's scale multiplies the weight in fp32. MASK: row g does not see
+// positions from n on (in the block's numbering); those may hold any scale.
+template <int HD, bool MASK>
+__device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], float ref, int n) {
+    constexpr int NG = HD / 64, ROW = HD / 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t bh[NG][2], bl[NG][2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
         float2 sc[NG];
-        scale_pairs<NG>(blk + kv4_kscale(HD), nt * 8 + 2 * t, sc);
-        s[nt] = __fmul2_rn(sc[0], __ffma2_rn(make_float2(acc[0][2], acc[0][3]), f2(1.0f / kLoScale),
-                                             make_float2(acc[0][0], acc[0][1])));
-        if (NG == 2)
-            s[nt] = __ffma2_rn(sc[NG - 1], __ffma2_rn(make_float2(acc[NG - 1][2], acc[NG - 1][3]), f2(1.0f / kLoScale),
-                                                      make_float2(acc[NG - 1][0], acc[NG - 1][1])), s[nt]);
-        if (MASK) {
-            if (j0 + nt * 8 + 2 * t >= st.n) s[nt].x = -INFINITY;
-            if (j0 + nt * 8 + 2 * t + 1 >= st.n) s[nt].y = -INFINITY;
+        scale_pairs<NG>(blk + kv4_vscale(HD), r0 + 8 * h + 2 * t, sc);
+        s[h] = __fadd2_rn(s[h], f2(ref));
+        s[h].x = ex2(s[h].x);
+        s[h].y = ex2(s[h].y);
+        st.l = __fadd2_rn(st.l, s[h]);
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+            float2 w = __fmul2_rn(s[h], sc[gr]);
+            if (MASK) {
+                if (r0 + 8 * h + 2 * t >= n) w.x = 0.0f;
+                if (r0 + 8 * h + 2 * t + 1 >= n) w.y = 0.0f;
+            }
+            split2(w, bh[gr][h], bl[gr][h]);
         }
     }
-    float m = fmaxf(s[0].x, s[0].y);
+    // thread (g, t) unpacks values 8 g .. 8 g + 7 of each group at positions 2t, 2t + 1, 2t + 8, 2t + 9
+    // (places t, 4 + t, 8 + t, 12 + t)
+    uint32_t vw[4][NG];
+    const uint8_t* vp = blk + kv4_vcode(HD) + (r0 + t) * ROW + (g ^ ((t & 2) << 1)) * 4 * NG;
 #pragma unroll
-    for (int nt = 1; nt < 8; nt++) m = fmaxf(m, fmaxf(s[nt].x, s[nt].y));
-    if (__any_sync(0xffffffffu, m > st.m)) {  // a score past the reference: all lanes of the row take a new one
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        if (m > st.m) {
-            m = fmaf(kHeadroom, 1.0f / st.f, m);
-            const float al = ex2((st.m - m) * st.f);  // st.m = -inf: 0
-            st.l = __fmul2_rn(st.l, f2(al));
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) st.o[gr][j][c] *= al;
-            st.m = m;
+    for (int r = 0; r < 4; r++) {
+        if (NG == 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(vp + 4 * r * ROW);
+            vw[r][0] = w.x, vw[r][NG - 1] = w.y;
+        } else {
+            vw[r][0] = *reinterpret_cast<const uint32_t*>(vp + 4 * r * ROW);
         }
     }
-    const float2 mf = f2(st.m == -INFINITY ? 0.0f : -st.m * st.f), ff = f2(st.f);
 #pragma unroll
-    for (int nt = 0; nt < 8; nt++) {
-        s[nt] = __ffma2_rn(s[nt], ff, mf);
-        s[nt].x = ex2(s[nt].x);
-        s[nt].y = ex2(s[nt].y);
-        st.l = __fadd2_rn(st.l, s[nt]);
+    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // values 2i, 2i + 1 of the words
+            uint32_t x = __byte_perm(vw[0][gr], vw[1][gr], i < 2 ? 0x5410 : 0x7632);
+            uint32_t y = __byte_perm(vw[2][gr], vw[3][gr], i < 2 ? 0x5410 : 0x7632);
+            if (i & 1) x >>= 8, y >>= 8;
+            const uint32_t a0 = code_even(x), a1 = code_odd(x), a2 = code_even(y), a3 = code_odd(y);
+            mma16816(st.o[gr][i], a0, a1, a2, a3, bh[gr][0], bh[gr][1]);
+            mma16816(st.o[gr][i], a0, a1, a2, a3, bl[gr][0], bl[gr][1]);
+        }
+}
+
+// One block (j0 = its first position's number): rows see all positions below n_min
+// and none from n_max on. A block that all rows see whole is one stretch of code
+// with one branch; others go by 16 positions.
+template <int HD>
+__device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_min, int n_max) {
+    constexpr int NG = HD / 64;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    // 2^top: the power of two above the block's largest V scale that a row sees
+    uint32_t bits = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if (j0 + 32 * h + lane < n_max) {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(blk + kv4_vscale(HD)) + (32 * h + lane) * NG;
+            bits = max(bits, (uint32_t)(NG == 2 ? max(p[0], p[NG - 1]) : p[0]));
+        }
+    const float top = (float)((int)(__reduce_max_sync(0xffffffffu, bits) >> 10) - 14);
+    if (j0 + kKv4Rows <= n_min) {
+        float2 s[4][2];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                s[k][h] = kv4_scores<HD>(st, blk, 16 * k + 8 * h);
+                mx = fmaxf(mx, fmaxf(s[k][h].x, s[k][h].y));
+            }
+        if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
+        const float ref = st.ref == -INFINITY ? 0.0f : -st.ref;
+#pragma unroll
+        for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], ref, 0);
+        return;
     }
-    const uint8_t* vp = blk + kv4_vcode(HD) + t * ROW + (g ^ ((t & 2) << 1)) * 4 * NG;
-#pragma unroll
-    for (int kk = 0; kk < 4; kk++) {
-        if (MASK && j0 + kk * 16 >= n_max) break;
-        // weights times scales of positions 2t, 2t + 1 (nt even), 2t + 8, 2t + 9 (nt odd)
-        uint32_t a[NG][4];
+    const int n = st.n - j0;
+#pragma unroll 1
+    for (int r0 = 0; r0 < min(kKv4Rows, n_max - j0); r0 += 16) {
+        float2 s[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int nt = 2 * kk + h;
-            float2 sc[NG];
-            scale_pairs<NG>(blk + kv4_vscale(HD), nt * 8 + 2 * t, sc);
-            if (MASK) {  // rows never written may hold any scale
-#pragma unroll
-                for (int gr = 0; gr < NG; gr++) {
-                    if (j0 + nt * 8 + 2 * t >= st.n) sc[gr].x = 0.0f;
-                    if (j0 + nt * 8 + 2 * t + 1 >= st.n) sc[gr].y = 0.0f;
-                }
-            }
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++) split2(__fmul2_rn(s[nt], sc[gr]), a[gr][2 * h], a[gr][2 * h + 1]);
+            s[h] = kv4_scores<HD>(st, blk, r0 + 8 * h);
+            if (r0 + 8 * h + 2 * t >= n) s[h].x = -INFINITY;
+            if (r0 + 8 * h + 2 * t + 1 >= n) s[h].y = -INFINITY;
         }
-        uint32_t vw[4][NG];  // rows 2t, 2t + 1, 2t + 8, 2t + 9 at places t, 4 + t, 8 + t, 12 + t
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint8_t* p = vp + (kk * 16 + 4 * r) * ROW;
-            if (NG == 2) {
-                const uint2 w = *reinterpret_cast<const uint2*>(p);
-                vw[r][0] = w.x, vw[r][NG - 1] = w.y;
-            } else {
-                vw[r][0] = *reinterpret_cast<const uint32_t*>(p);
-            }
-        }
-#pragma unroll
-        for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-            for (int q = 0; q < 2; q++) {  // values 4q .. 4q + 3 of the words
-                uint32_t x = __byte_perm(vw[0][gr], vw[1][gr], q ? 0x7632 : 0x5410);
-                uint32_t y = __byte_perm(vw[2][gr], vw[3][gr], q ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    mma16816(st.o[gr][4 * q + 2 * p], a[gr][0], a[gr][1], a[gr][2], a[gr][3], code_even(x), code_even(y));
-                    mma16816(st.o[gr][4 * q + 2 * p + 1], a[gr][0], a[gr][1], a[gr][2], a[gr][3], code_odd(x), code_odd(y));
-                    x >>= 8;
-                    y >>= 8;
-                }
-            }
+        const float mx = fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[1].x, s[1].y));
+        if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
+        kv4_values<HD, true>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
     }
 }
 
 // Bound by HBM for long caches (the codes and scales are read once, 4.25 bits
 // per value) and by launch and load latency for short ones. Each warp has a ring
-// of two whole blocks, filled by one bulk copy each; no barrier between warps
+// of two whole cache blocks, filled by one bulk copy each; no barrier between warps
 // but for the sum of a block that is inside one segment.
 template <int HD, typename T>
-__global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
+__global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int BLK = kv4_smem<HD>::BLK, NG = HD / 64, NW = kv4_warps(HD);
+    using SM = kv4_smem<HD>;
+    constexpr int UNIT = SM::UNIT, NG = HD / 64, NW = kKvWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = smem + warp * kKvRing * BLK;
-    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kv4_smem<HD>::bars) + warp * kKvRing;
+    uint8_t* ring = smem + warp * kKvRing * UNIT;
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SM::bars) + warp * kKvRing;
     if (lane == 0) {
         for (int i = 0; i < kKvRing; i++) mbar_init(bar + i, 1);
         mbar_fence_init();
@@ -444,39 +489,38 @@ __global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, 
     const int wid = blockIdx.x * cut.nw + warp;
     const kv4_split mine = cut.by_warp(blockIdx.x);
     const uint32_t c0 = cut.start(blockIdx.x), c1 = cut.start(blockIdx.x + 1), u0 = c0 + mine.start(warp);
-    int units = mine.start(warp + 1) - mine.start(warp);  // blocks of this warp's run
+    int units = mine.start(warp + 1) - mine.start(warp);  // units of this warp's run
     int b;
     uint32_t off;
     warp_find(seqs, a.B, S, u0, b, off);
     struct cursor {
-        int b, s, j, nb;
-        const uint8_t* p;
+        int b, s, j, nu;  // sequence, segment, unit of nu
+        const uint8_t* p;  // the unit
     } pr;
     pr.b = b;
-    pr.nb = seqs.blocks(b);
-    pr.s = (int)(whole ? off : off / pr.nb);
-    pr.j = (int)(whole ? 0 : off % pr.nb);
-    if (whole) {  // so many segments, each with its sequence's blocks
+    pr.nu = seqs.units(b);
+    pr.s = (int)(whole ? off : off / pr.nu);
+    pr.j = (int)(whole ? 0 : off % pr.nu);
+    if (whole) {  // so many segments, each with its sequence's units
         int segs = units, bb = b, ss = pr.s;
         for (units = 0; segs; segs--) {
-            units += seqs.blocks(bb);
+            units += seqs.units(bb);
             if (++ss == S && segs > 1) {
                 ss = 0;
                 do bb++;
-                while (seqs.blocks(bb) == 0);
+                while (seqs.units(bb) == 0);
             }
         }
     }
-    pr.p = c.run(a.slots[b], l, pr.s / R) + (size_t)pr.j * BLK;
+    pr.p = c.run(a.slots[b], l, pr.s / R) + (size_t)pr.j * UNIT;
     auto advance = [&](cursor& x) {  // not past the last unit
-        x.j++;
-        x.p += BLK;
-        if (x.j == x.nb) {
+        x.p += UNIT;
+        if (++x.j == x.nu) {
             x.j = 0;
             if (++x.s == S) {
                 x.s = 0;
-                do x.nb = seqs.blocks(++x.b);
-                while (x.nb == 0);
+                do x.nu = seqs.units(++x.b);
+                while (x.nu == 0);
             }
             x.p = c.run(a.slots[x.b], l, x.s / R);
         }
@@ -484,85 +528,87 @@ __global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, 
     cursor co = pr;
     // the block's run is inside one segment: its warps' sums meet here
     const uint32_t seg0 = u0 - pr.j;
-    const bool joined = !whole && cut.nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nb;
+    const bool joined = !whole && cut.nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nu;
     int issued = 0;
     auto issue = [&]() {
         if (lane == 0) {
             const int k = issued % kKvRing;
-            mbar_expect_tx(bar + k, BLK);
-            bulk_g2s(ring + k * BLK, pr.p, BLK, bar + k);
+            mbar_expect_tx(bar + k, UNIT);
+            bulk_g2s(ring + k * UNIT, pr.p, UNIT, bar + k);
         }
         if (++issued < units) advance(pr);
     };
-    while (issued < min(units, kKvRing)) issue();
+    issue();  // all warps' first units before anyone's others
     kv4_state<HD> st;
-    int slot_k = 0, phase = 0, n_min = 0, n_max = 0, row = 0;
+    int slot_k = 0, phase = 0, n_min = 0, n_max = 0;
     bool began = false;
     for (int i = 0; i < units; i++) {
         if (!began) {  // a new segment: its rows (those past the last repeat it and are not written)
-            const int kh = co.s / R, rt = co.s % R, r = min(rt * kKvTile + g, rows - 1);
-            const int tok = r / gsz, h = kh * gsz + r % gsz, len = seqs.len(co.b);
-            row = rt * kKvTile + g;
+            const int kh = co.s / R, rt = co.s % R, len = seqs.len(co.b);
+            auto row_of = [&](int r) { return min(rt * kKvTile + r, rows - 1); };
+            auto sees = [&](int r) { return max(0, len - a.T + 1 + row_of(r) / gsz); };
+            const int r = row_of(g), tok = r / gsz, h = kh * gsz + r % gsz;
             kv4_load_q<HD, T>(st, static_cast<const T*>(a.q) + ((long long)co.b * a.T + tok) * a.q_stride + h * HD,
                               a.scale);
-            st.n = max(0, len - a.T + 1 + tok);
-            n_min = max(0, len - a.T + 1 + rt * kKvTile / gsz);
-            n_max = max(0, len - a.T + 1 + min(rt * kKvTile + kKvTile - 1, rows - 1) / gsz);
+            st.n = sees(g);
+            n_min = sees(0), n_max = sees(kKvTile - 1);
             began = true;
+            if (i == 0) {
+                while (issued < min(units, kKvRing)) issue();
+            }
         }
         if (!mbar_wait_bounded(bar + slot_k, phase, a.err)) break;  // flagged; the block's sum still meets
-        const uint8_t* blk = ring + slot_k * BLK;
-        const int j0 = co.j * kKv4Rows;
-        if (j0 + kKv4Rows <= n_min) kv4_block<HD, false>(st, blk, j0, n_max);
-        else if (j0 < n_max) kv4_block<HD, true>(st, blk, j0, n_max);
+        const int j0 = co.j * kKvUnit;
+        if (j0 < n_max) kv4_block<HD>(st, ring + slot_k * UNIT, j0, n_min, n_max);
         fence_proxy_async_smem();
         __syncwarp();
         if (issued < units) issue();
         if (++slot_k == kKvRing) slot_k = 0, phase ^= 1;
-        const bool ends = co.j == co.nb - 1;
+        const bool ends = co.j == co.nu - 1;
         if (ends || i == units - 1) {
-            float lsum = st.l.x + st.l.y;
-            lsum += __shfl_xor_sync(0xffffffffu, lsum, 1);
-            lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
-            const bool from_start = i >= co.j;  // the segment's first block is in this warp's run
+            float lrow = st.l.x + st.l.y;
+            lrow += __shfl_xor_sync(0xffffffffu, lrow, 1);
+            lrow += __shfl_xor_sync(0xffffffffu, lrow, 2);
+            const float2 lsum = make_float2(__shfl_sync(0xffffffffu, lrow, 8 * t), __shfl_sync(0xffffffffu, lrow, 8 * t + 4));
+            const bool from_start = i >= co.j;  // the segment's first unit is in this warp's run
             if (ends && from_start) {
-                const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-                if (row < rows) {
-                    const int tok = row / gsz, h = co.s / R * gsz + row % gsz;
-                    const long long orow = (long long)co.b * a.T + tok;
+#pragma unroll
+                for (int cc = 0; cc < 2; cc++) {
+                    const int row = co.s % R * kKvTile + 2 * t + cc;
+                    if (row >= rows) continue;
+                    const float ls = cc ? lsum.y : lsum.x, inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                    const int h = co.s / R * gsz + row % gsz;
+                    const long long orow = (long long)co.b * a.T + row / gsz;
                     T* out = static_cast<T*>(a.out) + (orow * a.H + h) * HD;
 #pragma unroll
-                    for (int gr = 0; gr < NG; gr++)
+                    for (int gr = 0; gr < NG; gr++) {
+                        float x[8];
 #pragma unroll
-                        for (int cc = 0; cc < 2; cc++) {
-                            float x[8];
+                        for (int j = 0; j < 8; j++) x[j] = st.o[gr][j / 2][j % 2 * 2 + cc] * inv;
+                        const int d = gr * 64 + 8 * g;
+                        put8(out + d, x);
+                        if (a.outT)
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                x[j] = fmaf(st.o[gr][j][2 + cc], 1.0f / kLoScale, st.o[gr][j][cc]) * inv;
-                            const int d = gr * 64 + 8 * (2 * t + cc);
-                            put8(out + d, x);
-                            if (a.outT)
-#pragma unroll
-                                for (int j = 0; j < 8; j++) a.outT[(size_t)(h * HD + d + j) * a.outT_ld + orow] = x[j];
-                        }
+                            for (int j = 0; j < 8; j++) a.outT[(size_t)(h * HD + d + j) * a.outT_ld + orow] = x[j];
+                    }
                 }
             } else {
                 float* part = joined ? reinterpret_cast<float*>(ring)
                                      : static_cast<float*>(a.ws) + ((size_t)wid * 2 + from_start) * kv4_part_floats(HD);
-                float* ml = joined ? reinterpret_cast<float*>(smem + kv4_smem<HD>::stat) + warp * 2 * kKvTile
-                                   : part + kKvTile * HD;
+                float* ml = joined ? reinterpret_cast<float*>(smem + SM::stat) + warp * 2 * kKvTile : part + kKvTile * HD;
 #pragma unroll
-                for (int gr = 0; gr < NG; gr++)
+                for (int cc = 0; cc < 2; cc++) {
 #pragma unroll
-                    for (int cc = 0; cc < 2; cc++) {
+                    for (int gr = 0; gr < NG; gr++) {
                         float x[8];
 #pragma unroll
-                        for (int j = 0; j < 8; j++) x[j] = fmaf(st.o[gr][j][2 + cc], 1.0f / kLoScale, st.o[gr][j][cc]);
-                        put8(part + g * HD + gr * 64 + 8 * (2 * t + cc), x);
+                        for (int j = 0; j < 8; j++) x[j] = st.o[gr][j / 2][j % 2 * 2 + cc];
+                        put8(part + (2 * t + cc) * HD + gr * 64 + 8 * g, x);
                     }
+                }
                 if (t == 0) {
-                    ml[g] = st.m == -INFINITY ? st.m : st.m * st.f;
-                    ml[kKvTile + g] = lsum;
+                    ml[g] = st.ref;
+                    ml[kKvTile + g] = lrow;
                 }
             }
             began = false;
@@ -572,7 +618,7 @@ __global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, 
     if (!joined) return;
     // all cut.nw warps of the block come here: the warps' sums, in their order
     asm volatile("bar.sync 1, %0;" ::"r"(cut.nw * 32) : "memory");
-    const float* ml = reinterpret_cast<const float*>(smem + kv4_smem<HD>::stat);
+    const float* ml = reinterpret_cast<const float*>(smem + SM::stat);
     float* part = static_cast<float*>(a.ws) +
                   ((size_t)blockIdx.x * cut.nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
     for (int x = threadIdx.x; x < kKvTile * HD / 4; x += cut.nw * 32) {
@@ -583,7 +629,7 @@ __global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, 
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int w = 0; w < (int)cut.nw; w++) {
             const float f = ex2(ml[w * 2 * kKvTile + r] - mu);
-            const float4 v = reinterpret_cast<const float4*>(smem + w * kKvRing * BLK)[x];
+            const float4 v = reinterpret_cast<const float4*>(smem + w * kKvRing * UNIT)[x];
             lsum = fmaf(ml[w * 2 * kKvTile + kKvTile + r], f, lsum);
             o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
         }
@@ -599,17 +645,17 @@ __global__ void __launch_bounds__(kv4_warps(HD) * 32, 1) k_kv4_attn(kv4_dims c, 
 // one segment, 8 / RB warps per row, each adding every (8 / RB)-th part.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int ctas, int RB) {
-    constexpr int V = HD / 32, NW = kv4_warps(HD), PF = kv4_part_floats(HD);  // V values per lane
+    constexpr int V = HD / 32, NW = kKvWarps, PF = kv4_part_floats(HD);  // V values per lane
     __shared__ float sums[8][HD], stat[8][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gsz = a.H / c.KH, rows = a.T * gsz, S = R * c.KH;
     const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, 0};
     // The attention's blocks have all passed their own wait when this kernel
     // starts, so lens and slots are there before this kernel's wait.
-    const int b = blockIdx.x / S, s = blockIdx.x % S, nb = seqs.blocks(b);
+    const int b = blockIdx.x / S, s = blockIdx.x % S, nu = seqs.units(b);
     uint32_t before = 0, U = 0;
     for (int i = lane; i < a.B; i += 32) {
-        const int n = seqs.blocks(i);
+        const int n = seqs.units(i);
         U += n;
         if (i < b) before += n;
     }
@@ -619,8 +665,8 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const kv4_cut cut(max(1u, U * S), ctas, NW);
-    const uint32_t first = before * S + s * nb, last = first + nb;
-    const int w0 = nb ? cut.warp_of(first) : 0, w1 = nb ? cut.warp_of(last - 1) : 0, nw = cut.nw;
+    const uint32_t first = before * S + s * nu, last = first + nu;
+    const int w0 = nu ? cut.warp_of(first) : 0, w1 = nu ? cut.warp_of(last - 1) : 0, nw = cut.nw;
     griddep_wait();
     griddep_launch_dependents();
     if (w0 == w1) return;  // nothing to add, or one warp had it all
@@ -735,10 +781,10 @@ int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream
     if (sms < 1) return JL_ERR_CUDA;
     const long long segs = (long long)a.B * R * c.KH;
     if (segs > INT_MAX || segs * c.nb > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
-    // Segments of at most 4 blocks are not cut: a warp takes that many sooner
+    // Segments of at most 256 positions are not cut: a warp takes that many sooner
     // than a second kernel starts.
     const int whole = a.longest <= 4 * kKv4Rows;
-    const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kv4_warps(HD) * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
+    const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kKvWarps * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
                           whole);
     if (rc || whole) return rc;
     const int RB = segs >= sms ? 8 : segs * 4 >= sms ? 2 : 1;
@@ -756,7 +802,7 @@ int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStrea
 
 // Two parts for each warp that has blocks.
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
-    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kv4_warps(c.hd);
+    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kKvWarps;
     const long long n = segs >= warps ? warps : std::min(warps, segs * c.nb);
     return n * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float);
 }
