@@ -288,42 +288,52 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
     st.l = f2(0.0f);
 }
 
-// Scores in base 2 of positions r0 .. r0 + 7 of a block: s = those of r0 + 2 t and
-// r0 + 2 t + 1. Codes become n - 8 exactly, by one AND-OR into 1024's mantissa and
-// one packed fp16 sum per two values (the offset's own sum would be far larger than
-// the results'). K's scale multiplies the accumulated group in fp32.
+// Scores in base 2 of positions r0 .. r0 + 15 of a block: s[h] = those of
+// r0 + 8 h + 2 t and the next. Codes become n - 8 exactly, by one AND-OR into
+// 1024's mantissa and one packed fp16 sum per two values (the offset's own sum would
+// be far larger than the results'). K's scale multiplies the accumulated group in
+// fp32. Four sums take turns, since an instruction's result is there 20 cycles
+// later and the next one can start after 8.
 template <int HD>
-__device__ __forceinline__ float2 kv4_scores(const kv4_state<HD>& st, const uint8_t* blk, int r0) {
+__device__ __forceinline__ void kv4_scores(const kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2]) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float acc[NG][4];
-    uint32_t kw[NG * 2];
+    float acc[2][NG][4];
+    uint32_t kw[2][NG * 2];
     const uint8_t* kp = blk + (r0 + g) * ROW + t * 8 * NG;
-    if (NG == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(kp);
-        kw[0] = w.x, kw[1] = w.y, kw[NG] = w.z, kw[2 * NG - 1] = w.w;
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(kp);
-        kw[0] = w.x, kw[1] = w.y;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (NG == 2) {
+            const uint4 w = *reinterpret_cast<const uint4*>(kp + 8 * h * ROW);
+            kw[h][0] = w.x, kw[h][1] = w.y, kw[h][NG] = w.z, kw[h][2 * NG - 1] = w.w;
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(kp + 8 * h * ROW);
+            kw[h][0] = w.x, kw[h][1] = w.y;
+        }
     }
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
         for (int sh = 0; sh < 2; sh++)
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                const uint32_t x = sh ? kw[w * NG + gr] >> 8 : kw[w * NG + gr];
-                const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
-                if (w + sh == 0) mma16816_0(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
-                else mma16816(acc[gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
-            }
-    float2 sc[NG];
-    scale_pairs<NG>(blk + kv4_kscale(HD), r0 + 2 * t, sc);
-    float2 s = __fmul2_rn(sc[0], __fadd2_rn(make_float2(acc[0][0], acc[0][1]), make_float2(acc[0][2], acc[0][3])));
-    if (NG == 2)
-        s = __ffma2_rn(sc[NG - 1], __fadd2_rn(make_float2(acc[NG - 1][0], acc[NG - 1][1]),
-                                              make_float2(acc[NG - 1][2], acc[NG - 1][3])), s);
-    return __fmul2_rn(s, f2(st.f));
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t x = sh ? kw[h][w * NG + gr] >> 8 : kw[h][w * NG + gr];
+                    const uint32_t (&a)[4] = st.qf[gr * 4 + w * 2 + sh];
+                    if (w + sh == 0) mma16816_0(acc[h][gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
+                    else mma16816(acc[h][gr], a[0], a[1], a[2], a[3], code_even(x), code_odd(x));
+                }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float2 sc[NG];
+        scale_pairs<NG>(blk + kv4_kscale(HD), r0 + 8 * h + 2 * t, sc);
+        s[h] = __fmul2_rn(sc[0], __fadd2_rn(make_float2(acc[h][0][0], acc[h][0][1]), make_float2(acc[h][0][2], acc[h][0][3])));
+        if (NG == 2)
+            s[h] = __ffma2_rn(sc[NG - 1], __fadd2_rn(make_float2(acc[h][NG - 1][0], acc[h][NG - 1][1]),
+                                                     make_float2(acc[h][NG - 1][2], acc[h][NG - 1][3])), s[h]);
+        s[h] = __fmul2_rn(s[h], f2(st.f));
+    }
 }
 
 // A weight past the limit (or the first of a row): its row takes a new reference,
@@ -351,8 +361,10 @@ __device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, f
 
 // Weights of positions r0 .. r0 + 15 from their scores, and the weighted values
 // onto the sums. V's scale multiplies the weight in fp32. MASK: row g does not see
-// positions from n on (in the block's numbering); those may hold any scale.
-template <int HD, bool MASK>
+// positions from n on (in the block's numbering); those may hold any scale. LO: the
+// weights' lo parts too; without them a weight is off by 2^-12 of itself at most,
+// random from weight to weight, which a 16-bit output (2^-11, 2^-8) does not show.
+template <int HD, bool MASK, bool LO>
 __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], float ref, int n) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -372,7 +384,8 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
                 if (r0 + 8 * h + 2 * t >= n) w.x = 0.0f;
                 if (r0 + 8 * h + 2 * t + 1 >= n) w.y = 0.0f;
             }
-            split2(w, bh[gr][h], bl[gr][h]);
+            if (LO) split2(w, bh[gr][h], bl[gr][h]);
+            else bh[gr][h] = h2bits(__float22half2_rn(w));
         }
     }
     // thread (g, t) unpacks values 8 g .. 8 g + 7 of each group at positions 2t, 2t + 1, 2t + 8, 2t + 9
@@ -389,22 +402,33 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
         }
     }
 #pragma unroll
-    for (int gr = 0; gr < NG; gr++)
+    for (int q = 0; q < 2; q++) {  // values 4q .. 4q + 3 of the words, 2 per instruction: four sums take turns
+        uint32_t f[NG][2][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {  // values 2i, 2i + 1 of the words
-            uint32_t x = __byte_perm(vw[0][gr], vw[1][gr], i < 2 ? 0x5410 : 0x7632);
-            uint32_t y = __byte_perm(vw[2][gr], vw[3][gr], i < 2 ? 0x5410 : 0x7632);
-            if (i & 1) x >>= 8, y >>= 8;
-            const uint32_t a0 = code_even(x), a1 = code_odd(x), a2 = code_even(y), a3 = code_odd(y);
-            mma16816(st.o[gr][i], a0, a1, a2, a3, bh[gr][0], bh[gr][1]);
-            mma16816(st.o[gr][i], a0, a1, a2, a3, bl[gr][0], bl[gr][1]);
+        for (int gr = 0; gr < NG; gr++) {
+            const uint32_t x = __byte_perm(vw[0][gr], vw[1][gr], q ? 0x7632 : 0x5410);
+            const uint32_t y = __byte_perm(vw[2][gr], vw[3][gr], q ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                f[gr][i][0] = code_even(i ? x >> 8 : x), f[gr][i][1] = code_odd(i ? x >> 8 : x);
+                f[gr][i][2] = code_even(i ? y >> 8 : y), f[gr][i][3] = code_odd(i ? y >> 8 : y);
+            }
         }
+#pragma unroll
+        for (int part = 0; part < (LO ? 2 : 1); part++)
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    mma16816(st.o[gr][2 * q + i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3],
+                             part ? bl[gr][0] : bh[gr][0], part ? bl[gr][1] : bh[gr][1]);
+    }
 }
 
 // One block (j0 = its first position's number): rows see all positions below n_min
 // and none from n_max on. A block that all rows see whole is one stretch of code
 // with one branch; others go by 16 positions.
-template <int HD>
+template <int HD, bool LO>
 __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_min, int n_max) {
     constexpr int NG = HD / 64;
     const int lane = threadIdx.x & 31, t = lane & 3;
@@ -421,31 +445,29 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
         float2 s[4][2];
         float mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                s[k][h] = kv4_scores<HD>(st, blk, 16 * k + 8 * h);
-                mx = fmaxf(mx, fmaxf(s[k][h].x, s[k][h].y));
-            }
+        for (int k = 0; k < 4; k++) {
+            kv4_scores<HD>(st, blk, 16 * k, s[k]);
+            mx = fmaxf(mx, fmaxf(fmaxf(s[k][0].x, s[k][0].y), fmaxf(s[k][1].x, s[k][1].y)));
+        }
         if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
         const float ref = st.ref == -INFINITY ? 0.0f : -st.ref;
 #pragma unroll
-        for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], ref, 0);
+        for (int k = 0; k < 4; k++) kv4_values<HD, false, LO>(st, blk, 16 * k, s[k], ref, 0);
         return;
     }
     const int n = st.n - j0;
 #pragma unroll 1
     for (int r0 = 0; r0 < min(kKv4Rows, n_max - j0); r0 += 16) {
         float2 s[2];
+        kv4_scores<HD>(st, blk, r0, s);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            s[h] = kv4_scores<HD>(st, blk, r0 + 8 * h);
             if (r0 + 8 * h + 2 * t >= n) s[h].x = -INFINITY;
             if (r0 + 8 * h + 2 * t + 1 >= n) s[h].y = -INFINITY;
         }
         const float mx = fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[1].x, s[1].y));
         if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
-        kv4_values<HD, true>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
+        kv4_values<HD, true, LO>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
     }
 }
 
@@ -559,7 +581,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         }
         if (!mbar_wait_bounded(bar + slot_k, phase, a.err)) break;  // flagged; the block's sum still meets
         const int j0 = co.j * kKvUnit;
-        if (j0 < n_max) kv4_block<HD>(st, ring + slot_k * UNIT, j0, n_min, n_max);
+        if (j0 < n_max) kv4_block<HD, sizeof(T) == 4>(st, ring + slot_k * UNIT, j0, n_min, n_max);
         fence_proxy_async_smem();
         __syncwarp();
         if (issued < units) issue();
