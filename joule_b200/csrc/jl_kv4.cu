@@ -2,6 +2,7 @@
 // entry points of the attention over it (jl_kv4_attn.cu). Layout: jl_kv4.cuh.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -25,79 +26,110 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
                        bf16_to_f32(w.y >> 16));
 }
 
-// Append: 16 lanes per (row, head, K or V, group) read 4 values each, reduce
-// the group's maximum by shuffles and store its record. Bound by HBM (each
-// value read once, an eighth of its fp32 size written).
-template <typename T>
+// Append and read back: block (row chunk, K or V of a head), a row's head by
+// HD / values-per-lane lanes, STEPS rows of a lane in flight. (An index of one
+// flat item per lane took three times the instructions and bound both kernels by
+// issue: 8,179 rows x 16 heads 65 + 47 us under ncu.)
+constexpr int kKvSteps = 4;
+
+// Append: a lane has one code word (8 values); the 8 lanes of a group reduce its
+// maximum by shuffles and store its record. Bound by HBM (each value read once, an
+// eighth of its fp32 size written).
+template <int HD, typename T, int STEPS>
 __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, const T* __restrict__ k,
                                                            const T* __restrict__ v, long long ks, long long vs,
                                                            const int* __restrict__ slots,
-                                                           const int* __restrict__ positions, long long ntask,
-                                                           int* err) {
+                                                           const int* __restrict__ positions, int N, int* err) {
+    constexpr int LPR = HD / 8, ROWS = kKvThreads / LPR;  // lanes per row, rows per step
     griddep_wait();
     griddep_launch_dependents();
-    const int i = threadIdx.x & 15, ng = c.hd / 64, per = c.KH * 2 * ng;
-    const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);
-    const long long task = ((long long)blockIdx.x * kKvThreads + threadIdx.x) >> 4;
-    if (task >= ntask) return;
-    const long long n = task / per;
-    const int rest = (int)(task - n * per), is_v = rest / (c.KH * ng), h = rest % (c.KH * ng) / ng, g = rest % ng;
-    const int slot = slots[n], pos = positions[n];
-    if (slot < 0 || slot >= c.slots || pos < 0 || pos >= c.maxT) {
-        if (rest == 0 && i == 0 && err) atomicOr(err, kErrKvIndex);
-        return;
+    const int is_v = blockIdx.y & 1, h = blockIdx.y >> 1, w = threadIdx.x % LPR, g = w / 8, u = w % 8;
+    const long long stride = is_v ? vs : ks;
+    const int n0 = blockIdx.x * ROWS * STEPS + threadIdx.x / LPR;
+    const T* src = (is_v ? v : k) + n0 * stride + h * HD + 8 * w;
+    float4 x[STEPS], y[STEPS];
+    int slot[STEPS], pos[STEPS];
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        const int n = n0 + j * ROWS;
+        slot[j] = -1;
+        x[j] = y[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (n < N) {
+            slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
+            const T* p = src + j * ROWS * stride;
+            x[j] = load4(p), y[j] = load4(p + 4);
+        }
     }
-    const T* src = (is_v ? v + n * vs : k + n * ks) + h * c.hd + g * 64 + 4 * i;
-    uint8_t* blk = c.run(slot, l, h) + (size_t)(pos / kKv4Rows) * kv4_block_bytes(c.hd);
-    kv4_store_group(blk, c.hd, is_v, pos % kKv4Rows, g, load4(src), i, mask);
+    uint8_t* base = c.run(0, l, h);
+    const size_t per_slot = (size_t)c.L * c.KH * c.nb * kv4_block_bytes(HD);
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        const bool ok = (unsigned)slot[j] < (unsigned)c.slots && (unsigned)pos[j] < (unsigned)c.maxT;
+        if (!ok && n0 + j * ROWS < N && blockIdx.y == 0 && w == 0 && err) atomicOr(err, kErrKvIndex);
+        uint8_t* blk = base + slot[j] * per_slot + (size_t)(pos[j] / kKv4Rows) * kv4_block_bytes(HD);
+        kv4_store_group(blk, HD, is_v, pos[j] % kKv4Rows, g, u, x[j], y[j], ok);
+    }
 }
 
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+// VPT values of a code word from value v0 on, one 16-byte store.
+__device__ __forceinline__ void store_values(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
 }
-__device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
+__device__ __forceinline__ void store_values(__half* p, const float* x) {
     __half2 h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+__device__ __forceinline__ void store_values(__nv_bfloat16* p, const float* x) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
 }
 
-// Read back: thread = one code word (8 values) of (row, head, K or V, group);
-// (n - 8) * s is exact in fp32 (4 by 11 bits), rounded once to a 16-bit type.
-// A row outside the cache reads as zeros. Bound by HBM (the values written).
-template <typename T>
+// Read back: a lane writes 16 bytes (half a code word's values in fp32, a word's in
+// 16 bits); (n - 8) * s is exact in fp32 (4 by 11 bits), rounded once to a 16-bit
+// type. A row outside the cache reads as zeros. Bound by HBM (the values written).
+template <int HD, typename T, int STEPS>
 __global__ void __launch_bounds__(kKvThreads) k_kv4_read(kv4_dims c, int l, T* __restrict__ k, T* __restrict__ v,
                                                          const int* __restrict__ slots,
-                                                         const int* __restrict__ positions, long long ntask,
-                                                         int* err) {
+                                                         const int* __restrict__ positions, int N, int* err) {
+    constexpr int VPT = 16 / sizeof(T), LPR = HD / VPT, ROWS = kKvThreads / LPR;
     griddep_wait();
     griddep_launch_dependents();
-    const int ng = c.hd / 64, per = c.KH * 2 * ng * 8;
-    const long long task = (long long)blockIdx.x * kKvThreads + threadIdx.x;
-    if (task >= ntask) return;
-    const long long n = task / per;
-    const int rest = (int)(task - n * per), is_v = rest / (c.KH * ng * 8), hg = rest % (c.KH * ng * 8) / 8;
-    const int u = rest % 8, h = hg / ng, g = hg % ng;
-    const int slot = slots[n], pos = positions[n];
-    float x[8] = {};
-    if (slot < 0 || slot >= c.slots || pos < 0 || pos >= c.maxT) {
-        if (rest == 0 && err) atomicOr(err, kErrKvIndex);
-    } else {
-        const uint8_t* blk = c.run(slot, l, h) + (size_t)(pos / kKv4Rows) * kv4_block_bytes(c.hd);
-        const int r = pos % kKv4Rows;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + kv4_word_off(c.hd, is_v, r, g, u));
-        const float s = half_bits_to_f32(*reinterpret_cast<const uint16_t*>(blk + kv4_scale_off(c.hd, is_v, r, g)));
+    const int is_v = blockIdx.y & 1, h = blockIdx.y >> 1, e = threadIdx.x % LPR * VPT, g = e / 64, u = e % 64 / 8;
+    const int n0 = blockIdx.x * ROWS * STEPS + threadIdx.x / LPR;
+    const uint8_t* base = c.run(0, l, h);
+    const size_t per_slot = (size_t)c.L * c.KH * c.nb * kv4_block_bytes(HD);
+    uint32_t word[STEPS];
+    float s[STEPS];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = __fmul_rn((float)((int)(w >> (4 * j) & 15u) - 8), s);
+    for (int j = 0; j < STEPS; j++) {
+        const int n = n0 + j * ROWS;
+        word[j] = 0, s[j] = 0.0f;
+        if (n >= N) continue;
+        const int slot = __ldg(slots + n), pos = __ldg(positions + n);
+        if ((unsigned)slot < (unsigned)c.slots && (unsigned)pos < (unsigned)c.maxT) {
+            const uint8_t* blk = base + slot * per_slot + (size_t)(pos / kKv4Rows) * kv4_block_bytes(HD);
+            const int row = pos % kKv4Rows;
+            word[j] = *reinterpret_cast<const uint32_t*>(blk + kv4_word_off(HD, is_v, row, g, u));
+            s[j] = half_bits_to_f32(*reinterpret_cast<const uint16_t*>(blk + kv4_scale_off(HD, is_v, row, g)));
+        } else if (blockIdx.y == 0 && e == 0 && err) {
+            atomicOr(err, kErrKvIndex);
+        }
     }
-    store8((is_v ? v : k) + (n * c.KH + h) * c.hd + g * 64 + 8 * u, x);
+    T* dst = (is_v ? v : k) + ((size_t)n0 * c.KH + h) * HD + e;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+        if (n0 + j * ROWS >= N) break;
+        if (VPT == 4) word[j] >>= e % 8 * 4;
+        float x[VPT];
+#pragma unroll
+        for (int q = 0; q < VPT; q++)  // n in the low bits of 2^23
+            x[q] = __fmul_rn(__uint_as_float((word[j] >> (4 * q) & 15u) | 0x4B000000u) - 8388616.0f, s[j]);
+        store_values(dst + (size_t)j * ROWS * c.KH * HD, x);
+    }
 }
 
 }  // namespace jl
@@ -111,7 +143,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int jl_kv4_view(const jl_kv4* c, int l, jl::kv4_dims* out) {
     if (!c || !c->base || !aligned16(c->base) || (c->hd != 64 && c->hd != 128)) return JL_ERR_INVALID;
     if (c->slots < 1 || c->L < 1 || c->n_kv < 1 || c->maxT < 1 || l < 0 || l >= c->L) return JL_ERR_INVALID;
-    if (c->maxT > INT_MAX - jl::kKv4Rows) return JL_ERR_INVALID;
+    if (c->maxT > INT_MAX - jl::kKv4Rows || c->n_kv > 4096) return JL_ERR_INVALID;
     out->base = static_cast<uint8_t*>(c->base);
     out->slots = c->slots, out->L = c->L, out->KH = c->n_kv, out->hd = c->hd, out->maxT = c->maxT;
     out->nb = (c->maxT + jl::kKv4Rows - 1) / jl::kKv4Rows;
@@ -130,26 +162,32 @@ extern "C" long long jl_kv4_bytes(const jl_kv4* c) {
 
 namespace {
 
-template <typename T>
+// Several rows of a lane in flight for calls that fill the device with blocks all
+// the same, one row for short ones.
+template <int HD, typename T, int VPT, typename K1, typename K4, typename... Args>
+int launch_rows(K1 one, K4 many, int KH, int N, cudaStream_t s, Args... args) {
+    using namespace jl;
+    const int rows = kKvThreads / (HD / VPT);
+    const bool big = (long long)N * KH >= (long long)rows * 1024;
+    const int per = big ? rows * kKvSteps : rows;
+    const dim3 grid((N + per - 1) / per, 2 * KH);
+    return big ? launch(many, grid, dim3(kKvThreads), 0, s, args...) : launch(one, grid, dim3(kKvThreads), 0, s, args...);
+}
+
+template <int HD, typename T>
 int launch_append(const jl::kv4_dims& c, int l, const void* k, const void* v, long long ks, long long vs,
                   const int* slots, const int* positions, int N, int* err, cudaStream_t s) {
     using namespace jl;
-    const long long ntask = (long long)N * c.KH * 2 * (c.hd / 64);
-    const long long blocks = (ntask * 16 + kKvThreads - 1) / kKvThreads;
-    if (blocks > INT_MAX) return JL_ERR_INVALID;
-    return launch(k_kv4_append<T>, dim3((unsigned)blocks), dim3(kKvThreads), 0, s, c, l, (const T*)k, (const T*)v, ks,
-                  vs, slots, positions, ntask, err);
+    return launch_rows<HD, T, 8>(k_kv4_append<HD, T, 1>, k_kv4_append<HD, T, kKvSteps>, c.KH, N, s, c, l, (const T*)k,
+                                 (const T*)v, ks, vs, slots, positions, N, err);
 }
 
-template <typename T>
+template <int HD, typename T>
 int launch_read(const jl::kv4_dims& c, int l, const int* slots, const int* positions, int N, void* k, void* v,
                 int* err, cudaStream_t s) {
     using namespace jl;
-    const long long ntask = (long long)N * c.KH * 2 * (c.hd / 64) * 8;
-    const long long blocks = (ntask + kKvThreads - 1) / kKvThreads;
-    if (blocks > INT_MAX) return JL_ERR_INVALID;
-    return launch(k_kv4_read<T>, dim3((unsigned)blocks), dim3(kKvThreads), 0, s, c, l, (T*)k, (T*)v, slots, positions,
-                  ntask, err);
+    return launch_rows<HD, T, 16 / sizeof(T)>(k_kv4_read<HD, T, 1>, k_kv4_read<HD, T, kKvSteps>, c.KH, N, s, c, l, (T*)k,
+                                              (T*)v, slots, positions, N, err);
 }
 
 }  // namespace
@@ -167,9 +205,10 @@ extern "C" int jl_kv4_append(const jl_kv4* c, int l, const void* k, const void* 
         (N > 1 && (k_stride < row || v_stride < row)))
         return JL_ERR_INVALID;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == JL_F32) return launch_append<float>(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
-    if (dtype == JL_F16) return launch_append<__half>(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
-    return launch_append<__nv_bfloat16>(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
+    const bool wide = d.hd == 128;
+    if (dtype == JL_F32) return (wide ? launch_append<128, float> : launch_append<64, float>)(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
+    if (dtype == JL_F16) return (wide ? launch_append<128, __half> : launch_append<64, __half>)(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
+    return (wide ? launch_append<128, __nv_bfloat16> : launch_append<64, __nv_bfloat16>)(d, l, k, v, k_stride, v_stride, slots, positions, N, dev_status, s);
 }
 
 extern "C" int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* positions, int N, void* k, void* v,
@@ -181,9 +220,10 @@ extern "C" int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* 
     if (N == 0) return JL_OK;
     if (!k || !v || !slots || !positions || !aligned16(k) || !aligned16(v)) return JL_ERR_INVALID;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == JL_F32) return launch_read<float>(d, l, slots, positions, N, k, v, dev_status, s);
-    if (dtype == JL_F16) return launch_read<__half>(d, l, slots, positions, N, k, v, dev_status, s);
-    return launch_read<__nv_bfloat16>(d, l, slots, positions, N, k, v, dev_status, s);
+    const bool wide = d.hd == 128;
+    if (dtype == JL_F32) return (wide ? launch_read<128, float> : launch_read<64, float>)(d, l, slots, positions, N, k, v, dev_status, s);
+    if (dtype == JL_F16) return (wide ? launch_read<128, __half> : launch_read<64, __half>)(d, l, slots, positions, N, k, v, dev_status, s);
+    return (wide ? launch_read<128, __nv_bfloat16> : launch_read<64, __nv_bfloat16>)(d, l, slots, positions, N, k, v, dev_status, s);
 }
 
 extern "C" long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H) {

@@ -49,30 +49,53 @@ struct kv4_dims {
     }
 };
 
-// Quantises one group of 64 values held by 16 consecutive lanes (lane i of the
-// 16 holds values 4i..4i+3) and stores it as (row r, group g) of block `blk`.
-// The quotient is an IEEE division, so a code is the nearest step to the exact
-// x / s. Beyond the record's own rules: a scale that fp16 cannot hold stays at
-// its largest number (values past 7 * 65504 saturate) and a NaN becomes zero,
-// so what the cache holds is always finite. All 16 lanes of the group call it.
-__device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, int r, int g, float4 x, int i,
-                                                uint32_t mask) {
-    float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-    for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-    const __half sh = __float2half_rn(fminf(__fdiv_rn(fmaxf(amax, 1e-12f), 7.0f), 65504.0f));
-    const float s = __half2float(sh);
-    const float v[4] = {x.x, x.y, x.z, x.w};
+// Codes of eight values of a group with scale s (the nearest steps of the exact
+// quotients, ties to even): an IEEE division each.
+inline __device__ __noinline__ uint32_t kv4_codes_div(float4 x, float4 y, float s) {
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < 8; j++) {
         const float q = rintf(__fdiv_rn(v[j], s));
         const int n = q != q ? 8 : (int)fminf(fmaxf(q, -8.0f), 7.0f) + 8;
         w |= (uint32_t)n << (4 * j);
     }
-    w |= __shfl_down_sync(mask, w, 1) << 16;  // the odd lane's four values
-    if ((i & 1) == 0) *reinterpret_cast<uint32_t*>(blk + kv4_word_off(hd, is_v, r, g, i >> 1)) = w;
-    if (i == 0) *reinterpret_cast<uint16_t*>(blk + kv4_scale_off(hd, is_v, r, g)) = __half_as_ushort(sh);
+    return w;
+}
+
+// Quantises a group of 64 values held by 8 consecutive lanes (lane u of the 8 has
+// word u: values 8u .. 8u + 7, x then y) and stores it as (row r, group g) of block
+// `blk` when `store`. A code is the step nearest to the exact x / s. Its first guess
+// is the product with 1 / s, rounded by adding 1.5 * 2^23 + 8; the guess n stands when
+// what is left, x - (n - 8) s (exact: 11 by 4 bits from a value of the same size), is
+// clearly below half a step, and the lane divides when it is not (a tie or nearly one,
+// a NaN, an infinity, a scale of 0, a value past the largest scale). Beyond the
+// record's own rules: a scale that fp16 cannot hold stays at its largest number
+// (values past 7 * 65504 saturate) and a NaN becomes zero, so what the cache holds is
+// always finite. All lanes of the warp call it.
+__device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, int r, int g, int u, float4 x, float4 y,
+                                                bool store) {
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(v[j]));
+#pragma unroll
+    for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const __half sh = __float2half_rn(fminf(__fdiv_rn(fmaxf(amax, 1e-12f), 7.0f), 65504.0f));
+    const float s = __half2float(sh), inv = __frcp_rn(s), bound = 0.4999f * s;
+    uint32_t w = 0;
+    bool sure = true;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float q = fmaf(v[j], inv, 12582920.0f);
+        const float left = fmaf(12582920.0f - q, s, v[j]);
+        sure = sure && fabsf(left) <= bound;
+        w |= (__float_as_uint(q) & 15u) << (4 * j);
+    }
+    if (!sure) w = kv4_codes_div(x, y, s);
+    if (!store) return;
+    *reinterpret_cast<uint32_t*>(blk + kv4_word_off(hd, is_v, r, g, u)) = w;
+    if (u == 0) *reinterpret_cast<uint16_t*>(blk + kv4_scale_off(hd, is_v, r, g)) = __half_as_ushort(sh);
 }
 
 }  // namespace jl
