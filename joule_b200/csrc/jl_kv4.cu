@@ -13,17 +13,31 @@ namespace jl {
 
 constexpr int kKvThreads = 256;
 
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
+// Eight values as fp32. STREAM: first to leave L2 (a long call's rows, read once).
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_from(const void* p) {
+    return STREAM ? __ldcs(static_cast<const V*>(p)) : *static_cast<const V*>(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void load8(const float* p, float4& x, float4& y) {
+    x = load_from<STREAM, float4>(p);
+    y = load_from<STREAM, float4>(p + 4);
+}
+template <bool STREAM>
+__device__ __forceinline__ void load8(const __half* p, float4& x, float4& y) {
+    const uint4 w = load_from<STREAM, uint4>(p);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
+    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&w.z));
+    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&w.w));
+    x = make_float4(a.x, a.y, b.x, b.y);
+    y = make_float4(c.x, c.y, d.x, d.y);
 }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    return make_float4(bf16_to_f32(w.x & 0xFFFFu), bf16_to_f32(w.x >> 16), bf16_to_f32(w.y & 0xFFFFu),
-                       bf16_to_f32(w.y >> 16));
+template <bool STREAM>
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float4& x, float4& y) {
+    const uint4 w = load_from<STREAM, uint4>(p);
+    x = make_float4(bf16_to_f32(w.x & 0xFFFFu), bf16_to_f32(w.x >> 16), bf16_to_f32(w.y & 0xFFFFu), bf16_to_f32(w.y >> 16));
+    y = make_float4(bf16_to_f32(w.z & 0xFFFFu), bf16_to_f32(w.z >> 16), bf16_to_f32(w.w & 0xFFFFu), bf16_to_f32(w.w >> 16));
 }
 
 // Append and read back: block (row chunk, K or V of a head), a row's head by
@@ -56,8 +70,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, co
         x[j] = y[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (n < N) {
             slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
-            const T* p = src + j * ROWS * stride;
-            x[j] = load4(p), y[j] = load4(p + 4);
+            load8<(STEPS > 1)>(src + j * ROWS * stride, x[j], y[j]);
         }
     }
     uint8_t* base = c.run(0, l, h);
@@ -71,21 +84,30 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, co
     }
 }
 
-// VPT values of a code word from value v0 on, one 16-byte store.
-__device__ __forceinline__ void store_values(float* p, const float* x) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+// 16 bytes of values. STREAM: first to leave L2 (outputs of long calls, which would
+// push out the cache's records and one another: 30,000 rows x 4 heads 33 -> 26 us).
+template <bool STREAM>
+__device__ __forceinline__ void store16(void* p, uint4 v) {
+    if (STREAM) __stcs(reinterpret_cast<uint4*>(p), v);
+    else *reinterpret_cast<uint4*>(p) = v;
 }
-__device__ __forceinline__ void store_values(__half* p, const float* x) {
+template <bool STREAM>
+__device__ __forceinline__ void store_values(float* p, const float (&x)[4]) {
+    store16<STREAM>(p, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
+}
+template <bool STREAM>
+__device__ __forceinline__ void store_values(__half* p, const float (&x)[8]) {
     __half2 h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+    store16<STREAM>(p, *reinterpret_cast<uint4*>(h));
 }
-__device__ __forceinline__ void store_values(__nv_bfloat16* p, const float* x) {
+template <bool STREAM>
+__device__ __forceinline__ void store_values(__nv_bfloat16* p, const float (&x)[8]) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+    store16<STREAM>(p, *reinterpret_cast<uint4*>(h));
 }
 
 // Read back: a lane writes 16 bytes (half a code word's values in fp32, a word's in
@@ -123,12 +145,15 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_read(kv4_dims c, int l, T* _
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
         if (n0 + j * ROWS >= N) break;
-        if (VPT == 4) word[j] >>= e % 8 * 4;
+        // nibble q of a half word left in place in 2^23's mantissa: 2^23 + 16^q n, then n - 8 by an exact FMA
         float x[VPT];
 #pragma unroll
-        for (int q = 0; q < VPT; q++)  // n in the low bits of 2^23
-            x[q] = __fmul_rn(__uint_as_float((word[j] >> (4 * q) & 15u) | 0x4B000000u) - 8388616.0f, s[j]);
-        store_values(dst + (size_t)j * ROWS * c.KH * HD, x);
+        for (int q = 0; q < VPT; q++) {
+            const uint32_t half = VPT == 4 ? word[j] >> (e % 8 * 4) : q < 4 ? word[j] : word[j] >> 16;
+            const float unit = q % 4 == 0 ? 1.0f : q % 4 == 1 ? 0.0625f : q % 4 == 2 ? 0.00390625f : 0.000244140625f;
+            x[q] = __fmul_rn(fmaf(__uint_as_float((half & (15u << (4 * (q % 4)))) | 0x4B000000u), unit, -8388608.0f * unit - 8.0f), s[j]);
+        }
+        store_values<(STEPS > 1)>(dst + (size_t)j * ROWS * c.KH * HD, x);
     }
 }
 
@@ -247,7 +272,7 @@ extern "C" int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, lon
     if (!q || !slots || !lens || !out || !aligned16(q) || !aligned16(out) || q_stride % unit ||
         ((long long)B * T > 1 && q_stride < row))
         return JL_ERR_INVALID;
-    const long long need = jl_kv4_attn_ws_bytes(d, B, T, H);
+    const long long need = longest && longest <= 256 ? 0 : jl_kv4_attn_ws_bytes(d, B, T, H);
     if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need)) return JL_ERR_INVALID;
     jl_kv4_attn_args a;
     a.q = q, a.dtype = dtype, a.q_stride = q_stride, a.slots = slots, a.lens = lens, a.len_add = 0;

@@ -803,9 +803,9 @@ int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream
     if (sms < 1) return JL_ERR_CUDA;
     const long long segs = (long long)a.B * R * c.KH;
     if (segs > INT_MAX || segs * c.nb > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
-    // Segments of at most 256 positions are not cut: a warp takes that many sooner
-    // than a second kernel starts.
-    const int whole = a.longest <= 4 * kKv4Rows;
+    // Segments of at most 256 positions are not cut (and need no workspace): a warp
+    // takes that many sooner than a second kernel starts.
+    const int whole = a.longest <= 256;
     const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kKvWarps * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
                           whole);
     if (rc || whole) return rc;

@@ -17,7 +17,7 @@ length outside it skips the row (append) or reads as zeros, and sets bit 8 of
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
 
 import torch
@@ -42,108 +42,124 @@ def kv4_cache(slots: int, L: int, n_kv: int, hd: int, maxT: int, device=None) ->
     return torch.empty(slots, L, n_kv, -(-maxT // KV4_BLOCK), 68 * hd, dtype=torch.uint8, device=device)
 
 
-def _view(cache: torch.Tensor, l: int) -> Kv4:
-    if cache.dtype != torch.uint8 or cache.dim() != 5 or not cache.is_cuda or not cache.is_contiguous():
+_lib = None
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object
+
+
+def _dll():
+    global _lib
+    if _lib is None:
+        _lib = get_dll()
+    return _lib
+
+
+def _view(cache: torch.Tensor, l: int) -> tuple[Kv4, int]:
+    """The cache as the library takes it, and its device's index."""
+    shape = cache.shape
+    if len(shape) != 5 or cache.dtype is not torch.uint8 or not cache.is_cuda or not cache.is_contiguous():
         raise ValueError("kv4: the cache is a contiguous uint8 CUDA tensor [slots, L, n_kv, blocks, 68 * hd]")
-    slots, L, kh, nb, size = cache.shape
-    if size not in (68 * 64, 68 * 128) or cache.numel() == 0:
+    slots, L, kh, nb, size = shape
+    if size != 68 * 64 and size != 68 * 128 or not slots or not kh or not nb:
         raise ValueError(f"kv4: block size {size} is not 68 * hd with hd 64 or 128, or the cache is empty")
     if not 0 <= l < L:
         raise ValueError(f"kv4: layer {l} outside [0, {L})")
-    return Kv4(cache.data_ptr(), slots, L, kh, size // 68, nb * KV4_BLOCK)
+    return Kv4(cache.data_ptr(), slots, L, kh, size // 68, nb * KV4_BLOCK), cache.get_device()
 
 
-def _index(t: torch.Tensor, n: int, dev, name: str) -> int:
-    if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"kv4: {name} is a contiguous int32 tensor [{n}] on {dev}")
+def _index(t: torch.Tensor, n: int, dev: int, name: str) -> int:
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"kv4: {name} is a contiguous int32 tensor [{n}] on cuda:{dev}")
     return t.data_ptr()
 
 
-def _status(t, dev) -> int | None:
+def _status(t, dev: int) -> int | None:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != dev or t.numel() < 1:
-        raise ValueError(f"kv4: status is an int32 tensor on {dev}")
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.numel() < 1:
+        raise ValueError(f"kv4: status is an int32 tensor on cuda:{dev}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [rows, heads, hd] with whole rows at a 16-byte aligned stride; others are copied."""
-    _, h, d = t.shape
-    es = t.element_size()
-    s = t.stride()
-    if s[2] != 1 or (h > 1 and s[1] != d) or (t.shape[0] > 1 and (s[0] < h * d or s[0] * es % 16)) \
-            or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
-class _on:
-    """The device and stream of a call: tensors it allocates belong to that
-    stream, and the current device is the cache's."""
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t [rows, heads, hd] with its row stride, when whole rows lie at a 16-byte aligned stride; else a copy."""
+    n, h, d = t.shape
+    sn, sh, sd = t.stride()
+    if sd == 1 and (sh == d or h == 1) and (n <= 1 or sn >= h * d and sn * t.element_size() % 16 == 0) \
+            and t.data_ptr() % 16 == 0:
+        return t, sn if n > 1 else h * d
+    return _aligned(t), h * d
 
-    __slots__ = ("guard", "handle")
 
-    def __init__(self, dev, stream):
-        if stream is None and torch.cuda.current_device() == dev.index:
-            self.guard = None
-            self.handle = torch.cuda.current_stream(dev.index).cuda_stream
-            return
-        if stream is None:
-            stream = torch.cuda.current_stream(dev)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=dev)
-        if stream.device != dev:
-            raise ValueError(f"kv4: the stream is on {stream.device}, the cache on {dev}")
-        self.guard = torch.cuda.stream(stream)
-        self.handle = stream.cuda_stream
+def _on(dev: int, stream):
+    """The stream's handle when the call can go to it as things are (the current
+    device's current stream), else None."""
+    return _raw_stream(dev) if stream is None and torch._C._cuda_getDevice() == dev else None
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.handle
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _other(dev: int, stream) -> torch.cuda.Stream:
+    """A stream given by the caller, or the current one of another device: to be
+    made current for the call, so that what the call allocates belongs to it."""
+    device = torch.device("cuda", dev)
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        return torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        raise ValueError(f"kv4: the stream is on {stream.device}, the cache on {device}")
+    return stream
 
 
 def kv4_append(cache: torch.Tensor, l: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
                positions: torch.Tensor, status: torch.Tensor | None = None, stream=None) -> None:
     """Quantise k, v [N, n_kv, hd] (fp32, fp16 or bf16; rows of any stride)
     into positions[n] of slot slots[n] (int32 [N], distinct pairs) of layer l."""
-    c = _view(cache, l)
-    dev = cache.device
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (c.n_kv, c.hd):
+    c, dev = _view(cache, l)
+    shape = k.shape
+    if shape != v.shape or len(shape) != 3 or shape[1] != c.n_kv or shape[2] != c.hd:
         raise ValueError(f"kv4_append: k and v are [N, {c.n_kv}, {c.hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype not in _TYPES or v.dtype != k.dtype or k.device != dev or v.device != dev:
-        raise ValueError(f"kv4_append: k and v are fp32, fp16 or bf16, of one type, on {dev}")
-    n = k.shape[0]
+    kind = _TYPES.get(k.dtype)
+    if kind is None or v.dtype is not k.dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"kv4_append: k and v are fp32, fp16 or bf16, of one type, on cuda:{dev}")
+    n = shape[0]
     ps, pp, st = _index(slots, n, dev, "slots"), _index(positions, n, dev, "positions"), _status(status, dev)
-    with _on(dev, stream) as s:
-        k, v = _rows(k), _rows(v)
-        check(get_dll().jl_kv4_append(ctypes.byref(c), l, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.stride(0),
-                                      v.stride(0), ps, pp, n, st, s), "jl_kv4_append")
+    handle = _on(dev, stream)
+    if handle is None:
+        with torch.cuda.stream(_other(dev, stream)):
+            return kv4_append(cache, l, k, v, slots, positions, status)
+    k, sk = _rows(k)
+    v, sv = _rows(v)
+    check(_dll().jl_kv4_append(c, l, k.data_ptr(), v.data_ptr(), kind, sk, sv, ps, pp, n, st, handle), "jl_kv4_append")
 
 
 def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.Tensor,
              dtype: torch.dtype = torch.float32, status: torch.Tensor | None = None,
              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values [N, n_kv, hd] of (slots[n], positions[n])."""
-    c = _view(cache, l)
-    dev = cache.device
-    if dtype not in _TYPES:
+    c, dev = _view(cache, l)
+    kind = _TYPES.get(dtype)
+    if kind is None:
         raise ValueError(f"kv4_read: dtype is fp32, fp16 or bf16, got {dtype}")
     n = slots.numel()
     ps, pp, st = _index(slots, n, dev, "slots"), _index(positions, n, dev, "positions"), _status(status, dev)
-    with _on(dev, stream) as s:
-        k = torch.empty(n, c.n_kv, c.hd, dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        check(get_dll().jl_kv4_read(ctypes.byref(c), l, ps, pp, n, k.data_ptr(), v.data_ptr(), _TYPES[dtype], st, s),
-              "jl_kv4_read")
+    handle = _on(dev, stream)
+    if handle is None:
+        with torch.cuda.stream(_other(dev, stream)):
+            return kv4_read(cache, l, slots, positions, dtype, status)
+    k = torch.empty(n, c.n_kv, c.hd, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    check(_dll().jl_kv4_read(c, l, ps, pp, n, k.data_ptr(), v.data_ptr(), kind, st, handle), "jl_kv4_read")
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(slots: int, L: int, n_kv: int, hd: int, maxT: int, B: int, T: int, H: int) -> int:
+    """jl_kv4_attn_ws for these sizes."""
+    return max(0, get_dll().jl_kv4_attn_ws(Kv4(16, slots, L, n_kv, hd, maxT), B, T, H))
 
 
 def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Tensor, lens: torch.Tensor,
@@ -156,34 +172,46 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     longest: a bound of the lens that the caller knows (by default the cache's
     length); a longer entry counts as outside the cache. Rows that see nothing
     are zero. Returns out, of q's shape and type."""
-    c = _view(cache, l)
-    dev = cache.device
-    if q.dim() not in (3, 4) or q.shape[-1] != c.hd or q.shape[-2] < 1 or q.shape[-2] % c.n_kv:
-        raise ValueError(f"kv4_attention: q is [B, T, H, {c.hd}] or [B, H, {c.hd}] with H a multiple of {c.n_kv}, "
+    c, dev = _view(cache, l)
+    shape = q.shape
+    hd, H = c.hd, shape[-2] if len(shape) >= 3 else 0
+    if len(shape) not in (3, 4) or shape[-1] != hd or H < 1 or H % c.n_kv:
+        raise ValueError(f"kv4_attention: q is [B, T, H, {hd}] or [B, H, {hd}] with H a multiple of {c.n_kv}, "
                          f"got {tuple(q.shape)}")
-    if q.dtype not in _TYPES or q.device != dev:
-        raise ValueError(f"kv4_attention: q is fp32, fp16 or bf16 on {dev}")
-    B, T, H = q.shape[0], 1 if q.dim() == 3 else q.shape[1], q.shape[-2]
+    kind = _TYPES.get(q.dtype)
+    if kind is None or q.get_device() != dev:
+        raise ValueError(f"kv4_attention: q is fp32, fp16 or bf16 on cuda:{dev}")
+    B, T = shape[0], 1 if len(shape) == 3 else shape[1]
     if T < 1:
         raise ValueError("kv4_attention: T is 1 or more")
     if longest is None:
         longest = 0
     elif not 1 <= longest <= c.maxT:
         raise ValueError(f"kv4_attention: longest {longest} outside [1, {c.maxT}]")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != dev
+    if out is not None and (out.shape != shape or out.dtype is not q.dtype or out.get_device() != dev
                             or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("kv4_attention: out is contiguous, 16-byte aligned, of q's shape, type and device")
     ps, pl, st = _index(slots, B, dev, "slots"), _index(lens, B, dev, "lens"), _status(status, dev)
-    if scale is None:
-        scale = 1.0 / math.sqrt(c.hd)
-    L = get_dll()
-    with _on(dev, stream) as s:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        rows = _rows(q if q.dim() == 3 else q.flatten(0, 1))
-        n = L.jl_kv4_attn_ws(ctypes.byref(c), B, T, H)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
-        check(L.jl_kv4_attn(ctypes.byref(c), l, rows.data_ptr(), _TYPES[q.dtype], rows.stride(0), ps, pl, longest,
-                            B, T, H, scale, out.data_ptr(), ws.data_ptr() if ws is not None else None, max(n, 0),
-                            st, s), "jl_kv4_attn")
+    handle = _on(dev, stream)
+    if handle is None:
+        with torch.cuda.stream(_other(dev, stream)):
+            return kv4_attention(cache, l, q, slots, lens, scale, longest or None, out, status)
+    row = H * hd
+    if q.is_contiguous() and q.data_ptr() % 16 == 0:
+        rows = q
+    elif len(shape) == 3:
+        rows, row = _rows(q)
+    else:  # one stride between all rows, or a copy
+        s = q.stride()
+        if B == 1 or T == 1 or s[0] == T * s[1]:
+            rows, row = _rows(q.as_strided((B * T, H, hd), (s[1] if T > 1 else s[0], s[2], s[3])))
+        else:
+            rows = _aligned(q)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    n = 0 if 0 < longest <= 256 else _ws_bytes(c.slots, c.L, c.n_kv, hd, c.maxT, B, T, H)
+    ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+    check(_dll().jl_kv4_attn(c, l, rows.data_ptr(), kind, row, ps, pl, longest, B, T, H,
+                             1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(),
+                             ws.data_ptr() if n else None, n, st, handle), "jl_kv4_attn")
     return out
