@@ -407,10 +407,21 @@ int jl_dec_create(const KernelCfg* c, const KernelW* W, int max_batch, int slots
                   int src_on_device, jl_dec** out);
 int jl_dec_destroy(jl_dec* h);
 
+/* jl_dec_create with flags. JL_DEC_KV4 keeps the sequences' keys and values in
+ * a 4-bit cache (jl_kv4 below) in place of the fp32 one, about a 7.5th of its
+ * bytes: steps and prefill chunks quantise the new rows as they write them and
+ * attend over the cached values by jl_kv4_attn's kernels. Contexts are bound by
+ * maxT alone. hd must be 64 or 128. Logits are then those of the cached values,
+ * not the reference's bits. No counterpart in the reference. */
+#define JL_DEC_KV4 1
+int jl_dec_create_ex(const KernelCfg* c, const KernelW* W, int max_batch, int slots,
+                     int src_on_device, int flags, jl_dec** out);
+
 /* The decoder's MoE handle (to upload experts, or set its path). */
 int jl_dec_moe(jl_dec* h, jl_moe** moe);
 
-/* Device base pointers of the K and V caches, [slots][L][maxT][n_kv*hd] fp32. */
+/* Device base pointers of the K and V caches, [slots][L][maxT][n_kv*hd] fp32
+ * (JL_ERR_INVALID for a handle with the 4-bit cache). */
 int jl_dec_kv(jl_dec* h, float** k, float** v);
 
 /* x[b] = bf16 embed[tokens[b]] as fp32 (embed_lookup, decode_kernel.c:1597-1600);
@@ -552,6 +563,10 @@ int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, long long q_st
                 const int* slots, const int* lens, int longest, int B, int T, int H,
                 float scale, void* out, void* ws, long long ws_bytes, int* dev_status,
                 void* stream);
+
+/* The cache of a decoder created with JL_DEC_KV4 (its buffer stays the
+ * decoder's), for jl_kv4_read and the like. */
+int jl_dec_kv4(jl_dec* h, jl_kv4* out);
 
 /* Bytes of device memory the handle holds (store + workspace). */
 long long jl_moe_device_bytes(const jl_moe* h);

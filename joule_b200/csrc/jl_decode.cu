@@ -9,7 +9,9 @@
 //
 // Per layer: k_rms (h += previous residual, norm1) -> k_mv (QKV, + bias) ->
 // k_attn_qk (QK-norm, RoPE, KV append, scores) -> k_attn_pv (softmax, values)
-// -> k_mv (o_proj) ->
+// -> k_mv (o_proj) -> (with the 4-bit cache, JL_DEC_KV4: k_qk_prep, which
+// quantises the rows as it writes them, -> the attention of jl_kv4_attn.cu; that
+// one keeps no order of the reference's sums) ->
 // k_rms (h += o, norm2) -> the MoE layer (jl_moe_forward) -> next layer.
 // Then k_rms (final norm) -> k_mv (fp32 lm_head) -> k_argmax.
 //
@@ -34,6 +36,7 @@
 
 #include "jl_common.cuh"
 #include "jl_internal.h"
+#include "jl_kv4.cuh"
 #include "jl_mv.cuh"
 
 namespace jl {
@@ -49,6 +52,15 @@ constexpr int kErrPosition = 8;       // a position outside [0, maxT) (error wor
 __device__ __forceinline__ float sqrtf_fast(float x) {
     const float y = __uint_as_float((__float_as_uint(x) + 0x3F800000u) >> 1);
     return __fmul_rn(0.5f, __fadd_rn(y, __fdiv_rn(x, y)));
+}
+// The same on the host (the 4-bit cache's attention takes its scale as a number).
+inline float sqrtf_fast_host(float x) {
+    uint32_t b;
+    memcpy(&b, &x, 4);
+    b = (b + 0x3F800000u) >> 1;
+    float y;
+    memcpy(&y, &b, 4);
+    return 0.5f * (y + x / y);
 }
 
 // 1 / sqrtf_fast(ss / n + eps) (decode_kernel.c:227, 1168, 1181)
@@ -286,7 +298,8 @@ struct attn_args {
     int sqn;                 // floats per squares buffer of k_kv_append: max(qn, kn) for whole-vector norms, else hd
     float eps;
     int* err;
-    float* qr;               // [B][H][hd] q after QK-norm and RoPE (register-tiled attention)
+    float* qr;               // [B][H][hd] q after QK-norm and RoPE (register-tiled attention, 4-bit cache)
+    kv4_dims kv4;            // the 4-bit cache, or base = null: kc and vc
 };
 
 // Squares of v[0..n) into sq (n % 4 == 0, 16-byte aligned), loads batched.
@@ -716,6 +729,15 @@ __global__ void __launch_bounds__(kAttnThreads) k_qk_prep(attn_args a) {
     for (int hh = 0; hh < gsz; hh++)
         for (int c = tid; c < hd / 4; c += blockDim.x)
             reinterpret_cast<float4*>(dst + hh * hd)[c] = reinterpret_cast<const float4*>(q_s + hh * QS)[c];
+    if (a.kv4.base) {  // quantised as they are written: 8 lanes per group of K, then of V (hd 64 or 128: one warp)
+        if (tid < 32) {
+            const int ng = hd / 64, gr = tid / 8 % ng, u = tid % 8, is_v = tid / 8 / ng;
+            const float4* src = reinterpret_cast<const float4*>((is_v ? v_s : k_s) + gr * 64 + 8 * u);
+            uint8_t* blk = a.kv4.run(slot, a.l, g) + (size_t)(pos / kKv4Rows) * kv4_block_bytes(hd);
+            kv4_store_group(blk, hd, is_v, pos % kKv4Rows, gr, u, src[0], src[1], tid < 16 * ng);
+        }
+        return;
+    }
     const size_t off = (((size_t)slot * a.L + a.l) * a.maxT + pos) * kn + g * hd;
     for (int i = tid; i < hd; i += blockDim.x) {
         a.kc[off + i] = k_s[i];
@@ -1120,6 +1142,9 @@ struct jl_dec {
     float* sinb;
     float* kc;         // [slots][L][maxT][kn]
     float* vc;
+    jl_kv4 kv4;        // JL_DEC_KV4: the 4-bit cache in kc's and vc's place (base = null without it)
+    void* kv4_ws;      // its attention's workspace, for the step and for prefill chunks
+    long long kv4_ws_bytes;
     // workspace
     float* h;          // [max_batch, d]
     float* t;          // [max_batch, d]
@@ -1271,7 +1296,7 @@ extern "C" int jl_dec_destroy(jl_dec* h) {
     if (!h) return JL_OK;
     if (h->moe) jl_moe_destroy(h->moe);
     void* ptrs[] = {h->embed, h->norm1, h->norm2, h->fnorm, h->qnw, h->knw, h->wqkv, h->wo, h->bqkv, h->lm,
-                    h->cosb, h->sinb, h->kc, h->vc, h->h, h->t, h->h2, h->qkv, h->att, h->tT, h->attT, h->scores, h->qr,
+                    h->cosb, h->sinb, h->kc, h->vc, h->kv4.base, h->kv4_ws, h->h, h->t, h->h2, h->qkv, h->att, h->tT, h->attT, h->scores, h->qr,
                     h->logits, h->tok, h->arg_v, h->arg_i, h->pre_pos, h->pre_slot, h->err, h->stage};
     for (void* p : ptrs)
         if (p) cudaFree(p);
@@ -1281,11 +1306,20 @@ extern "C" int jl_dec_destroy(jl_dec* h) {
 
 extern "C" int jl_dec_create(const KernelCfg* c, const KernelW* W, int max_batch, int slots, int src_on_device,
                              jl_dec** out) {
+    return jl_dec_create_ex(c, W, max_batch, slots, src_on_device, 0, out);
+}
+
+extern "C" int jl_dec_create_ex(const KernelCfg* c, const KernelW* W, int max_batch, int slots, int src_on_device,
+                                int flags, jl_dec** out) {
     using namespace jl;
-    if (!out || !W || max_batch < 1 || slots < max_batch) return JL_ERR_INVALID;
+    if (!out || !W || max_batch < 1 || slots < max_batch || (flags & ~JL_DEC_KV4)) return JL_ERR_INVALID;
     *out = nullptr;
     int rc = check_dec_cfg(c);
     if (rc) return rc;
+    const bool kv4 = flags & JL_DEC_KV4;
+    jl_kv4 cache = {nullptr, slots, c->L, c->n_kv, c->hd, c->maxT};
+    const long long kv4_bytes = kv4 ? jl_kv4_bytes(&cache) : 0;
+    if (kv4_bytes < 0) return JL_ERR_INVALID;  // head dims other than 64 and 128
     if (c->qk_norm_type && (!W->qn || !W->kn)) return JL_ERR_INVALID;
     if (c->bias_qkv && (!W->bq || !W->bk || !W->bv)) return JL_ERR_INVALID;
     if (!W->embed || !W->lm_head || !W->final_norm || !W->norm1 || !W->norm2 || !W->wq || !W->wk || !W->wv ||
@@ -1310,7 +1344,14 @@ extern "C" int jl_dec_create(const KernelCfg* c, const KernelW* W, int max_batch
     }
     const size_t L = h->L, d = h->d, V = h->V;
     const size_t qnw_n = h->qk_type == 2 ? (size_t)h->qn : h->hd, knw_n = h->qk_type == 2 ? (size_t)h->kn : h->hd;
-    const size_t kvb = (size_t)slots * L * h->maxT * h->kn * sizeof(float);
+    const size_t kvb = kv4 ? 0 : (size_t)slots * L * h->maxT * h->kn * sizeof(float);
+    h->kv4 = cache;
+    if (kv4) {
+        kv4_dims d4;
+        d4.slots = slots, d4.L = h->L, d4.KH = h->KH, d4.hd = h->hd, d4.maxT = h->maxT;
+        d4.nb = (h->maxT + kKv4Rows - 1) / kKv4Rows;
+        h->kv4_ws_bytes = std::max(jl_kv4_attn_ws_bytes(d4, max_batch, 1, h->H), jl_kv4_attn_ws_bytes(d4, 1, max_batch, h->H));
+    }
     h->stage_bytes = std::max({V * d * sizeof(float), (size_t)h->nqkv * d * 2, d * (size_t)h->qn * 2});
     struct alloc { void** p; size_t n; } al[] = {
         {(void**)&h->embed, V * d * 2},
@@ -1332,7 +1373,9 @@ extern "C" int jl_dec_create(const KernelCfg* c, const KernelW* W, int max_batch
         {(void**)&h->h2, (size_t)max_batch * d * 4},
         {(void**)&h->qkv, (size_t)max_batch * h->nqkv * 4},
         {(void**)&h->att, (size_t)max_batch * h->qn * 4},
-        {(void**)&h->scores, (size_t)max_batch * h->H * h->maxT * 4},
+        {&h->kv4.base, (size_t)kv4_bytes},
+        {&h->kv4_ws, (size_t)h->kv4_ws_bytes},
+        {(void**)&h->scores, kv4 ? 0 : (size_t)max_batch * h->H * h->maxT * 4},
         {(void**)&h->qr, (size_t)max_batch * h->qn * 4},
         {(void**)&h->tT, max_batch >= kMmMinB ? (size_t)d * h->Bp * 4 : 0},
         {(void**)&h->attT, max_batch >= kMmMinB ? (size_t)h->qn * h->Bp * 4 : 0},
@@ -1360,8 +1403,8 @@ extern "C" int jl_dec_create(const KernelCfg* c, const KernelW* W, int max_batch
         jl_dec_destroy(h);
         return r;
     };
-    if (cudaMemsetAsync(h->err, 0, 16, s) != cudaSuccess || cudaMemsetAsync(h->kc, 0, kvb, s) != cudaSuccess ||
-        cudaMemsetAsync(h->vc, 0, kvb, s) != cudaSuccess)
+    if (cudaMemsetAsync(h->err, 0, 16, s) != cudaSuccess || (kvb && cudaMemsetAsync(h->kc, 0, kvb, s) != cudaSuccess) ||
+        (kvb && cudaMemsetAsync(h->vc, 0, kvb, s) != cudaSuccess))
         return fail(JL_ERR_CUDA);
     if ((rc = put(h->embed, W->embed, V * d * 2, od, s)) || (rc = put(h->norm1, W->norm1, L * d * 2, od, s)) ||
         (rc = put(h->norm2, W->norm2, L * d * 2, od, s)) || (rc = put(h->fnorm, W->final_norm, d * 2, od, s)) ||
@@ -1421,9 +1464,15 @@ extern "C" int jl_dec_moe(jl_dec* h, jl_moe** moe) {
 }
 
 extern "C" int jl_dec_kv(jl_dec* h, float** k, float** v) {
-    if (!h || !k || !v) return JL_ERR_INVALID;
+    if (!h || !k || !v || h->kv4.base) return JL_ERR_INVALID;
     *k = h->kc;
     *v = h->vc;
+    return JL_OK;
+}
+
+extern "C" int jl_dec_kv4(jl_dec* h, jl_kv4* out) {
+    if (!h || !out || !h->kv4.base) return JL_ERR_INVALID;
+    *out = h->kv4;
     return JL_OK;
 }
 
@@ -1478,6 +1527,18 @@ static int dec_step(jl_dec* h, const int* slots, const int* positions, const flo
     aa.qk_type = h->qk_type, aa.eps = h->eps, aa.err = h->err, aa.qr = h->qr;
     aa.sqn = attn_sqn(h->qk_type, h->H, h->KH, h->hd);
     aa.nslots = h->slots;
+    const bool kv4 = h->kv4.base != nullptr;
+    aa.kv4.base = nullptr;
+    jl_kv4_attn_args ka = {};
+    if (kv4) {
+        rc = jl_kv4_view(&h->kv4, 0, &aa.kv4);
+        if (rc) return rc;
+        // one row per sequence, or prefill: the B rows of one sequence, which sees what the last row does
+        const int last = prefill ? B - 1 : 0;
+        ka.q = h->qr, ka.dtype = JL_F32, ka.q_stride = h->qn, ka.slots = slots + last, ka.lens = positions + last;
+        ka.len_add = 1, ka.longest = h->maxT, ka.B = prefill ? 1 : B, ka.T = prefill ? B : 1, ka.H = h->H;
+        ka.scale = 1.0f / sqrtf_fast_host((float)h->hd), ka.out = h->att, ka.ws = h->kv4_ws, ka.err = h->err;
+    }
     // column-major copies of the matvec inputs for the register-tiled kernel (B >= kMmMinB)
     float* tT = B >= kMmMinB ? h->tT : nullptr;
     aa.attT = B >= kMmMinB ? h->attT : nullptr;
@@ -1495,7 +1556,7 @@ static int dec_step(jl_dec* h, const int* slots, const int* positions, const flo
     const int gsz = h->H / h->KH, maxT4 = (h->maxT + 3) / 4 * 4;
     // the register-tiled kernels at batches of 16 and more, for contexts whose
     // score rows fit the value kernel's shared memory (longer ones take k_attn_pv)
-    const bool attn_t = B >= 16 && attn_tiled_ok(h->hd, gsz) &&
+    const bool attn_t = !kv4 && B >= 16 && attn_tiled_ok(h->hd, gsz) &&
                         (size_t)pv_t_layout(gsz, h->maxT, h->hd).total * sizeof(float) <= 200 * 1024;
     auto pick_slices = [&](int units, int target) {
         int ds = 1;
@@ -1520,7 +1581,7 @@ static int dec_step(jl_dec* h, const int* slots, const int* positions, const flo
     const int dw = h->hd / dslices;
     const int pv_whole = pv_whole_bytes(hpb, dslices) <= 100 * 1024;
     const size_t pv_smem = pv_whole ? pv_whole_bytes(hpb, dslices) : pv_bytes(hpb, dslices);
-    if (qk_smem > 200 * 1024 || pv_smem > 200 * 1024) return JL_ERR_INVALID;
+    if (!kv4 && (qk_smem > 200 * 1024 || pv_smem > 200 * 1024)) return JL_ERR_INVALID;
     for (int l = 0; l < h->L; l++) {
         // norm1 (adding the previous layer's MoE output to the residual)
         rc = launch(k_rms, dim3(B), dim3(kNormThreads), nsm, s, h->h, (const float*)(l ? h->h2 : nullptr),
@@ -1536,17 +1597,25 @@ static int dec_step(jl_dec* h, const int* slots, const int* positions, const flo
             aa.qnw = h->qk_type ? h->qnw + l * qs : nullptr;
             aa.knw = h->qk_type ? h->knw + l * ks : nullptr;
             aa.from_cache = prefill;
-            if (prefill && !attn_t)
-                rc = launch(k_kv_append, dim3(h->KH, B), dim3(kAttnThreads), (size_t)(128 + aa.sqn) * sizeof(float),
-                            s, aa);
-            if (!rc && attn_t)
-                rc = h->hd == 64 ? launch_attn_t<64>(aa, h->scores, B, sms, s)
-                                 : launch_attn_t<128>(aa, h->scores, B, sms, s);
-            else if (!rc) rc = launch(k_attn_qk, dim3(h->KH, B, splits), dim3(kQkThreads), qk_smem, s, aa, h->scores, tp);
-            if (!rc && !attn_t) {
-                auto kern = pv_items <= 1 ? k_attn_pv<1> : pv_items <= 2 ? k_attn_pv<2> : k_attn_pv<4>;
-                rc = launch(kern, dim3(h->H / hpb, B, dslices), dim3(kPvThreads), pv_smem, s, aa,
-                            (const float*)h->scores, hpb, dw, pv_whole);
+            if (kv4) {
+                ka.outT = aa.attT, ka.outT_ld = h->Bp;
+                rc = launch(k_qk_prep, dim3(h->KH, B), dim3(kAttnThreads),
+                            qk_prep_smem(h->qk_type, h->H, h->KH, h->hd), s, aa);
+                if (!rc) rc = jl_launch_kv4_attn(aa.kv4, l, ka, s);
+            } else {
+                if (prefill && !attn_t)
+                    rc = launch(k_kv_append, dim3(h->KH, B), dim3(kAttnThreads), (size_t)(128 + aa.sqn) * sizeof(float),
+                                s, aa);
+                if (!rc && attn_t)
+                    rc = h->hd == 64 ? launch_attn_t<64>(aa, h->scores, B, sms, s)
+                                     : launch_attn_t<128>(aa, h->scores, B, sms, s);
+                else if (!rc)
+                    rc = launch(k_attn_qk, dim3(h->KH, B, splits), dim3(kQkThreads), qk_smem, s, aa, h->scores, tp);
+                if (!rc && !attn_t) {
+                    auto kern = pv_items <= 1 ? k_attn_pv<1> : pv_items <= 2 ? k_attn_pv<2> : k_attn_pv<4>;
+                    rc = launch(kern, dim3(h->H / hpb, B, dslices), dim3(kPvThreads), pv_smem, s, aa,
+                                (const float*)h->scores, hpb, dw, pv_whole);
+                }
             }
         }
         if (!rc)

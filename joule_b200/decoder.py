@@ -19,7 +19,7 @@ import ctypes
 import numpy as np
 import torch
 
-from joule_b200.native import KernelCfg, KernelW, check, get_dll
+from joule_b200.native import DEC_KV4, KernelCfg, KernelW, Kv4, check, get_dll
 
 __all__ = ["Decoder", "qwen3_cfg"]
 
@@ -53,16 +53,31 @@ def rope_tables(maxT: int, hd: int, theta: float) -> tuple[np.ndarray, np.ndarra
     return cos, sin
 
 
-class Decoder:
-    """One model's decode step on the current CUDA device."""
+class _Buffer:
+    """Device memory of the library as __cuda_array_interface__ (no copy)."""
 
-    def __init__(self, cfg: KernelCfg, W: KernelW, max_batch: int, slots: int, src_on_device: bool):
+    def __init__(self, ptr: int, shape: tuple, owner):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": "|u1", "data": (ptr, False), "version": 2}
+
+
+class Decoder:
+    """One model's decode step on the current CUDA device.
+
+    kv4: keep the sequences' keys and values in 4 bits (joule_b200.kv4) instead
+    of fp32, for head dims 64 and 128: a 7.5th of the memory, contexts bound by
+    maxT alone, and logits of the cached values instead of the reference's bits.
+    """
+
+    def __init__(self, cfg: KernelCfg, W: KernelW, max_batch: int, slots: int, src_on_device: bool,
+                 kv4: bool = False):
         self._L = get_dll()
         self.cfg = cfg
         self.max_batch = max_batch
         h = ctypes.c_void_p()
-        check(self._L.jl_dec_create(ctypes.byref(cfg), ctypes.byref(W), max_batch, slots,
-                                    1 if src_on_device else 0, ctypes.byref(h)), "jl_dec_create")
+        check(self._L.jl_dec_create_ex(ctypes.byref(cfg), ctypes.byref(W), max_batch, slots,
+                                       1 if src_on_device else 0, DEC_KV4 if kv4 else 0, ctypes.byref(h)),
+              "jl_dec_create_ex")
         self.h = h
         moe = ctypes.c_void_p()
         check(self._L.jl_dec_moe(h, ctypes.byref(moe)), "jl_dec_moe")
@@ -70,7 +85,7 @@ class Decoder:
 
     @classmethod
     def random(cls, cfg: KernelCfg, max_batch: int, slots: int, seed: int = 3,
-               theta: float = 1e6) -> "Decoder":
+               theta: float = 1e6, kv4: bool = False) -> "Decoder":
         """Seeded random-init weights drawn on the device: bf16 projections,
         embedding and router rows N(0, 0.02), norm weights 1.0, fp32 lm_head
         N(0, 0.02), Q4 experts quantised from N(0, 0.02) by the library."""
@@ -96,7 +111,7 @@ class Decoder:
         W = KernelW()
         for n, v in t.items():
             setattr(W, n, v.data_ptr())
-        self = cls(cfg, W, max_batch, slots, True)
+        self = cls(cfg, W, max_batch, slots, True, kv4)
         del t
         E, m = cfg.E, cfg.intermediate
         for l in range(L):
@@ -125,6 +140,14 @@ class Decoder:
     def set_moe_path(self, path: int) -> None:
         check(self._L.jl_moe_set_path(self.moe, path), "jl_moe_set_path")
 
+    def kv4_cache(self) -> torch.Tensor:
+        """The 4-bit cache of a decoder created with kv4=True as the uint8 tensor
+        that joule_b200.kv4 takes (the decoder's own memory, not a copy)."""
+        c = Kv4()
+        check(self._L.jl_dec_kv4(self.h, ctypes.byref(c)), "jl_dec_kv4")
+        shape = (c.slots, c.L, c.n_kv, -(-c.maxT // 64), 68 * c.hd)
+        return torch.as_tensor(_Buffer(c.base, shape, self), device="cuda")
+
     # -- the step -----------------------------------------------------------
     def embed(self, tokens: torch.Tensor, x: torch.Tensor, stream=None) -> torch.Tensor:
         """x[b] = embedding row tokens[b] (fp32)."""
@@ -141,6 +164,14 @@ class Decoder:
         check(self._L.jl_dec_step(self.h, slots.data_ptr(), positions.data_ptr(), x.data_ptr(), B,
                                   None if logits is None else logits.data_ptr(),
                                   None if tok is None else tok.data_ptr(), _stream(stream)), "jl_dec_step")
+
+    def prefill(self, slot: int, tokens: torch.Tensor, pos0: int = 0, tok: torch.Tensor | None = None,
+                logits: torch.Tensor | None = None, stream=None) -> None:
+        """A prompt's tokens (int32 device [T]) into KV slot `slot` at positions
+        pos0 on, max_batch positions per pass; logits [V] and tok [1] of the last."""
+        check(self._L.jl_dec_prefill(self.h, slot, tokens.data_ptr(), tokens.numel(), pos0,
+                                     None if logits is None else logits.data_ptr(),
+                                     None if tok is None else tok.data_ptr(), _stream(stream)), "jl_dec_prefill")
 
     def check(self, stream=None) -> None:
         check(self._L.jl_dec_check(self.h, _stream(stream)), "jl_dec_check")

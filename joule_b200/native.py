@@ -25,6 +25,7 @@ ERRORS = {
 }
 PATH_AUTO, PATH_EXACT, PATH_TC, PATH_GEMV = 0, 1, 2, 3
 CREATE_ROUTER_ONLY = 1
+DEC_KV4 = 1
 F32, F16, BF16 = 0, 1, 2
 
 
@@ -112,6 +113,8 @@ SIGNATURES = {
     "q4_gemm_f32": ([_P, _P, _I, _P, _P, _I, _I, _I], None),
     "jl_compat_status": ([], _I),
     "jl_dec_create": ([ctypes.POINTER(KernelCfg), ctypes.POINTER(KernelW), _I, _I, _I, ctypes.POINTER(_P)], _I),
+    "jl_dec_create_ex": ([ctypes.POINTER(KernelCfg), ctypes.POINTER(KernelW), _I, _I, _I, _I, ctypes.POINTER(_P)],
+                         _I),
     "jl_dec_destroy": ([_P], _I),
     "jl_dec_moe": ([_P, ctypes.POINTER(_P)], _I),
     "jl_dec_kv": ([_P, ctypes.POINTER(_P), ctypes.POINTER(_P)], _I),
@@ -135,6 +138,7 @@ SIGNATURES = {
     "jl_kv4_attn_ws": ([ctypes.POINTER(Kv4), _I, _I, _I], _LL),
     "jl_kv4_attn": ([ctypes.POINTER(Kv4), _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _LL,
                      _P, _P], _I),
+    "jl_dec_kv4": ([_P, ctypes.POINTER(Kv4)], _I),
     "jl_version": ([], ctypes.c_char_p),
     "jl_last_cuda_error": ([], ctypes.c_char_p),
 }

@@ -79,3 +79,61 @@ def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, scale: float) -> tupl
             p = np.exp(s - s.max())
             out[i, h] = p @ vv[:m] / p.sum()
     return out, absdot, top
+
+
+def decode_step(model, x: np.ndarray, positions, cached):
+    """The decode step of oracle/joule_oracle.c (jo_decode_step) with attention in
+    64 bits over given cached values: cached(l, b) -> (k, v) [positions[b] + 1, n_kv,
+    hd], this step's own row the last of them. Norms, RoPE and the MoE layers are the
+    restatement's, the projections in 64 bits, rounded to fp32 where the step keeps
+    fp32 rows. x [B, d] embedded inputs. Returns logits [B, V] (64 bits), the
+    rows that the step appends (k, v [L][B, n_kv, hd] fp32), and the largest |score|."""
+    import ctypes
+
+    from oracle import restate
+    lib, s, w = restate.lib(), model.shape, model.w
+    lib.jo_rms_norm.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float]
+    lib.jo_rope.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int]
+    lib.jo_sqrtf_fast.argtypes, lib.jo_sqrtf_fast.restype = [ctypes.c_float], ctypes.c_float
+    f32 = lambda bits: (np.asarray(bits, np.uint16).astype(np.uint32) << 16).view(np.float32)  # noqa: E731
+
+    def norm(rows, weight):
+        rows = np.ascontiguousarray(rows, np.float32)
+        out, weight = np.empty_like(rows), np.ascontiguousarray(weight)
+        for i in range(rows.shape[0]):
+            lib.jo_rms_norm(out[i].ctypes.data, rows[i].ctypes.data, weight.ctypes.data, rows.shape[1], s.eps)
+        return out
+
+    B, qn, kn = x.shape[0], s.H * s.hd, s.KH * s.hd
+    h = np.array(x, np.float32)
+    scale = 1.0 / float(np.float32(lib.jo_sqrtf_fast(float(s.hd))))
+    ks, vs, top = [], [], 0.0
+    for l in range(s.L):
+        t = norm(h, w["norm1"][l])
+        rows = []
+        for name, bias, n in (("wq", "bq", qn), ("wk", "bk", kn), ("wv", "bv", kn)):
+            r = t.astype(np.float64) @ f32(w[name][l]).astype(np.float64).T
+            rows.append((r + (w[bias][l] if s.bias_qkv else 0.0)).astype(np.float32))
+        q, k, v = rows
+        if s.qk_norm_type == 2:
+            q, k = norm(q, w["qn"][l]), norm(k, w["kn"][l])
+        elif s.qk_norm_type == 1:
+            q = norm(q.reshape(-1, s.hd), w["qn"][l]).reshape(B, qn)
+            k = norm(k.reshape(-1, s.hd), w["kn"][l]).reshape(B, kn)
+        q, k = np.ascontiguousarray(q), np.ascontiguousarray(k)
+        for b in range(B):
+            cs, sn = w["cos"][positions[b]], w["sin"][positions[b]]
+            for r, heads in ((q[b], s.H), (k[b], s.KH)):
+                for i in range(heads):
+                    lib.jo_rope(r.ctypes.data + 4 * i * s.hd, cs.ctypes.data, sn.ctypes.data, s.hd)
+        ks.append(k.reshape(B, s.KH, s.hd).copy())
+        vs.append(v.reshape(B, s.KH, s.hd).copy())
+        att = np.empty((B, qn))
+        for b in range(B):
+            kc, vc = cached(l, b)
+            o, _, m = attention(q[b].reshape(1, s.H, s.hd).astype(np.float64), kc, vc, scale)
+            att[b], top = o.reshape(qn), max(top, m)
+        h = (h + att @ f32(w["wo"][l]).astype(np.float64).T).astype(np.float32)
+        t = norm(h, w["norm2"][l])
+        h = (h + restate.moe_layer(model.layers[l], t)[0]).astype(np.float32)
+    return norm(h, w["final_norm"]).astype(np.float64) @ w["lm_head"].astype(np.float64).T, ks, vs, top

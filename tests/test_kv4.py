@@ -116,3 +116,19 @@ def test_front_end_refuses_without_a_device():
         with pytest.raises(ValueError):
             kv4.kv4_cache(**(dict(slots=1, L=1, n_kv=1, hd=64, maxT=1, device="cpu") | bad))
     assert kv4.kv4_cache(2, 3, 4, 128, 65, device="cpu").shape == (2, 3, 4, 2, 68 * 128)
+
+
+def test_decoder_flags_are_checked(dll):
+    """jl_dec_create_ex refuses flags it does not know and head dims that the
+    4-bit cache does not hold, before any device work."""
+    from joule_b200.native import DEC_KV4, KernelCfg, KernelW
+    W = KernelW()
+    for n in ("embed", "lm_head", "final_norm", "norm1", "norm2", "wq", "wk", "wv", "wo", "gate_w", "cos", "sin"):
+        setattr(W, n, 4096)
+    h = ctypes.c_void_p()
+    cfg = dict(L=1, d=256, n_heads=4, n_kv=2, hd=32, E=8, topk=2, V=64, maxT=16, intermediate=128)
+    make = lambda flags, **kw: dll.jl_dec_create_ex(ctypes.byref(KernelCfg(**(cfg | kw))), ctypes.byref(W), 2, 2, 0,  # noqa: E731
+                                                    flags, ctypes.byref(h))
+    assert make(DEC_KV4) == -1 and make(2, hd=64) == -1 and make(-1, hd=64) == -1
+    c = Kv4()
+    assert dll.jl_dec_kv4(None, ctypes.byref(c)) == -1
