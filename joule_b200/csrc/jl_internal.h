@@ -122,7 +122,8 @@ int jl_moe_layer_done(jl_moe* h, int l, cudaStream_t s);
 // callers from several host threads are serialised. key < 32.
 enum {
     kOnceExact = 0, kOnceRouter, kOnceRouterFast, kOnceDispatch, kOnceGemm, kOnceTc, kOnceGemv,
-    kOnceDecode, kOnceEp, kOnceBf16, kOnceMmBf16, kOnceMmF32, kOnceAttn, kOnceKv4
+    kOnceDecode, kOnceEp, kOnceBf16, kOnceMmBf16, kOnceMmF32, kOnceAttn, kOnceKv4,
+    kOnceKv4Prompt
 };
 int jl_device_once(int key, int (*setup)());
 
@@ -222,3 +223,5 @@ struct jl_kv4_attn_args {
 };
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H);
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);
+// The tcgen05 form for many query rows (jl_kv4_prompt.cu); no workspace.
+int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);

@@ -10,64 +10,16 @@
 // device from lens, so captured graphs follow growing sequences). A segment
 // that one warp covers is written by it; the parts of the others meet in
 // k_kv4_merge.
-#include <cuda_bf16.h>
-
 #include <algorithm>
 #include <climits>
 
 #include "jl_internal.h"
-#include "jl_kv4.cuh"
+#include "jl_kv4_dev.cuh"
 
 namespace jl {
 
-constexpr int kKvUnit = kKv4Rows;  // positions that a warp takes at a time: a cache block
 constexpr int kKvRing = 2;     // units in a warp's ring
 constexpr int kKvTile = 8;     // query rows of a tile
-// Weights times V's scales are kept at or below 2^kTop in fp16; a new reference
-// puts the largest at 2^(kTop - kHeadroom), so that the sums are not rescaled at
-// every new maximum (most units of a short run have one in some row).
-constexpr float kTop = 15.0f, kHeadroom = 4.0f;
-
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = to_f32(h[j]);
-}
-__device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void put8(__half* p, const float (&x)[8]) {
-    __half2 h[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
-}
-__device__ __forceinline__ void put8(__nv_bfloat16* p, const float (&x)[8]) {
-    __nv_bfloat162 h[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
-}
-__device__ __forceinline__ void put1(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put1(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void put1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -84,19 +36,6 @@ __device__ __forceinline__ void mma16816_0(float (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-__device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// A pair as fp16 pairs, hi the nearest and lo what hi misses: 22 bits down to
-// fp16's smallest steps of 2^-24 (callers scale what they split to 2^10 and more).
-__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __float22half2_rn(x);
-    const float2 f = __half22float2(h);
-    hi = h2bits(h);
-    lo = h2bits(__float22half2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y))));
-}
-
-__device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
-
 // The scales of positions r, r + 1 of a section: per group a pair over the two.
 template <int NG>
 __device__ __forceinline__ void scale_pairs(const uint8_t* section, int r, float2 (&sc)[NG]) {
@@ -111,39 +50,6 @@ __device__ __forceinline__ void scale_pairs(const uint8_t* section, int r, float
         sc[0] = __half22float2(*reinterpret_cast<const __half2*>(p));
     }
 }
-
-// n - 8 of the nibbles at bits 0-3 (even) or 4-7 (odd) of both halves, exactly,
-// as fp16: 1024 + n (1024 + 16 n) by its bits, then one packed sum (FMA). The
-// and-or is one instruction only when written as lop3 (measured: 256 fewer of
-// 1,590 instructions per block, on the pipe that is busiest).
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(m), "r"(o));
-    return y;
-}
-__device__ __forceinline__ uint32_t code_even(uint32_t x) {
-    x = and_or(x, 0x000F000Fu, 0x64006400u);
-    return h2bits(__hsub2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(1032.0f, 1032.0f)));
-}
-__device__ __forceinline__ uint32_t code_odd(uint32_t x) {
-    x = and_or(x, 0x00F000F0u, 0x64006400u);
-    return h2bits(__hfma2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f),
-                          __floats2half2_rn(-72.0f, -72.0f)));
-}
-
-// Units of sequence b (0 when its slot or length is outside the cache), and
-// what it counts in the cut: its units, or 1 when segments are not cut.
-struct kv4_seqs {
-    const int* slots;
-    const int* lens;
-    int len_add, longest, nslots, whole;
-    __device__ int len(int b) const {
-        const int n = __ldg(lens + b) + len_add, s = __ldg(slots + b);
-        return s >= 0 && s < nslots && n >= 0 && n <= longest ? n : -1;
-    }
-    __device__ int units(int b) const { return (max(0, len(b)) + kKvUnit - 1) / kKvUnit; }
-    __device__ int weight(int b) const { return whole ? len(b) > 0 : units(b); }
-};
 
 // The sum of weights over all sequences, and the sequence that holds unit u
 // when a sequence has S segments of its weight: b and the unit's offset in it
@@ -830,6 +736,7 @@ long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
 }
 
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+    if ((long long)a.T * (a.H / c.KH) >= 128) return jl_launch_kv4_prompt(c, l, a, s);
     const int rc = jl_device_once(kOnceKv4, [] {
         const int r = attn_attrs<64>();
         return r ? r : attn_attrs<128>();

@@ -1,0 +1,489 @@
+// Attention of a prompt's rows over the 4-bit KV cache on tcgen05 (layout:
+// jl_kv4.cuh; the form for few rows: jl_kv4_attn.cu).
+//
+// The query rows (token i, head h of the kv head's group; r = i * group + h) of
+// one (sequence, kv head) form tiles of 128, two of them per block. Per cache
+// block of 64 positions and tile: S = q K^T, softmax by the thread that owns the
+// row (= TMEM lane), O += P V, both products on the tensor cores with fp32 sums
+// in TMEM. Codes enter as n - 8, which fp16 holds exactly; q and the weights in
+// fp32 calls as hi and lo parts (22 bits), two instructions onto the same sums.
+// K's scales multiply the finished sums of a 64-value group (one accumulator per
+// group), V's the weights of a group, both in fp32. The exponents' reference
+// moves only when a weight times its scale would pass 2^15 (jl_kv4_dev.cuh), and
+// the sums are then rescaled in TMEM.
+//
+// Roles (14 warps): 0-3 and 4-7 softmax of tile 0 and 1, 8-11 unpack the cache
+// block into the two operands (K as [64 positions][values], V as [values][64
+// positions]) and copy the next one in, 12 and 13 issue the instructions of tile 0
+// and 1. The tiles take turns on the tensor cores: one's products run beside the
+// other's softmax. Every wait is bounded; a timeout sets the status bit and an
+// abort flag on which every role leaves its loop.
+//
+// Bound by the tensor cores in fp32 (two passes of each product) and by the
+// softmax's issue slots in 16 bits.
+#include <algorithm>
+#include <climits>
+
+#include "jl_internal.h"
+#include "jl_kv4_dev.cuh"
+#include "jl_umma.cuh"
+
+namespace jl {
+
+constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 14 * 32;
+constexpr int kPrCore = 144;  // bytes between V's core matrices (128 of data: stores without bank conflicts)
+
+struct pr_bars {
+    uint64_t raw_full[2], raw_empty[2], kv_full[2], kv_empty[2], q_full;
+    uint64_t s_full[2], p_full[2], pv_done[2], fin[2];
+    uint32_t tmem;
+    int abort;
+    float top[2][2];  // per buffer, per warp of positions: 2^top is above V's scales
+};
+
+template <int HD, bool LO>
+struct pr_smem {
+    static constexpr int NG = HD / 64, PARTS = LO ? 2 : 1;
+    static constexpr int QTILE = kPrTile * HD * 2, KTILE = kKv4Rows * HD * 2, VTILE = NG * 64 * kPrCore;
+    static constexpr int sc = 512;                       // fp32 scales [2 buffers][K g0, K g1, V g0, V g1][64]
+    static constexpr int q = sc + 2 * 4 * kKv4Rows * 4;  // [tile][part][chunk of 8 values][128 rows x 16 B]
+    static constexpr int k = q + 2 * PARTS * QTILE;      // [buffer][chunk][64 positions x 16 B]
+    static constexpr int v = k + 2 * KTILE;              // [buffer][group][8 positions' chunk][8 values' core]
+    static constexpr int raw = v + 2 * VTILE;
+    static constexpr int total = raw + 2 * kv4_block_bytes(HD);
+    static constexpr int SCOLS = NG * 64, TCOLS = 2 * SCOLS;  // TMEM columns of a tile: S (then P), O
+    static_assert(sizeof(pr_bars) <= 512 && total <= 227 * 1024, "shared memory");
+};
+
+// A wait of a whole warp, bounded; false when it ran out or another role gave up.
+__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
+    bool ok = mbar_try_wait(bar, parity);
+    const long long t0 = clock64();
+    for (int i = 1; !ok; i++) {
+        ok = mbar_try_wait(bar, parity);
+        if (!ok && (i & 63) == 0) {
+            if (*abort) break;
+            if (clock64() - t0 > kWaitLimitCycles) {
+                if (err) atomicOr(err, kErrTimeout);
+                *abort = 1;
+                break;
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+// The thread's q row, scaled to base-2 scores and by a power of two (its largest
+// value in [2^10, 2^11)), into the operand's hi and lo parts; returns the power's inverse.
+template <int HD, bool LO, typename T>
+__device__ __forceinline__ float pr_load_q(const T* q, float scale, uint8_t* dst) {
+    float mx = 0.0f;
+    for (int c = 0; c < HD / 8; c++) {
+        float x[8];
+        load8(q + 8 * c, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[j] * (scale * 1.4426950408889634f)));
+    }
+    int e = (int)(__float_as_uint(mx) >> 23);
+    e = min(max(e, 11), 253);
+    const float inv = __uint_as_float((uint32_t)(264 - e) << 23);
+    for (int c = 0; c < HD / 8; c++) {
+        float x[8];
+        load8(q + 8 * c, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = x[j] * (scale * 1.4426950408889634f) * inv;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) split2(make_float2(x[j], x[j + 4]), hi[j], lo[j]);  // the order of an unpacked word
+        *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (LO) *reinterpret_cast<uint4*>(dst + pr_smem<HD, LO>::QTILE + c * 2048) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    return __uint_as_float((uint32_t)(e - 10) << 23);
+}
+
+// Unpacks one cache block (128 threads, tid 0..127) into operand tiles and fp32
+// scales; positions from n on (never written) get scales of 0.
+template <int HD>
+__device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, float* top, int n, int tid) {
+    constexpr int NG = HD / 64, ROW = HD / 2;
+    const int lane = tid & 31, w = tid >> 5;
+    // K: lane (t, position of 8) takes words 2t, 2t + 1 of the groups
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int t = lane >> 3, o = w + 4 * i, r = 8 * o + (lane & 7);
+        uint32_t kw[2 * NG];
+        if (NG == 2) {
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + r * ROW + 16 * t);
+            kw[0] = x.x, kw[1] = x.y, kw[NG] = x.z, kw[2 * NG - 1] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(raw + r * ROW + 8 * t);
+            kw[0] = x.x, kw[1] = x.y;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t x = kw[u * NG + g], y = x >> 8;
+                *reinterpret_cast<uint4*>(kt + (g * 8 + 2 * t + u) * 1024 + o * 128 + (lane & 7) * 16) =
+                    make_uint4(code_even(x), code_odd(x), code_even(y), code_odd(y));
+            }
+    }
+    // V: thread (8 positions o, word u of group g) writes the 8 x 8 core matrix of its values
+    if (tid < 64 * NG) {
+        const int u = lane & 7, g = NG == 2 ? lane >> 3 & 1 : 0, o = NG == 2 ? 2 * w + (lane >> 4) : tid >> 3;
+        uint32_t x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = *reinterpret_cast<const uint32_t*>(raw + kv4_word_off(HD, 1, 8 * o + i, g, u));
+        uint8_t* core = vt + ((g * 8 + o) * 8 + u) * kPrCore;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            uint32_t p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = __byte_perm(x[2 * i], x[2 * i + 1], q ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                *reinterpret_cast<uint4*>(core + (4 * q + 2 * h) * 16) =
+                    make_uint4(code_even(p[0]), code_even(p[1]), code_even(p[2]), code_even(p[3]));
+                *reinterpret_cast<uint4*>(core + (4 * q + 2 * h + 1) * 16) =
+                    make_uint4(code_odd(p[0]), code_odd(p[1]), code_odd(p[2]), code_odd(p[3]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[i] >>= 8;
+            }
+        }
+    }
+    if (tid < kKv4Rows) {
+        const uint16_t* ks = reinterpret_cast<const uint16_t*>(raw + kv4_kscale(HD)) + tid * NG;
+        const uint16_t* vs = reinterpret_cast<const uint16_t*>(raw + kv4_vscale(HD)) + tid * NG;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const uint32_t b = tid < n ? vs[g] : 0;
+            sc[g * kKv4Rows + tid] = tid < n ? half_bits_to_f32(ks[g]) : 0.0f;
+            sc[(2 + g) * kKv4Rows + tid] = half_bits_to_f32((uint16_t)b);
+            bits = max(bits, b);
+        }
+        bits = __reduce_max_sync(0xffffffffu, bits);
+        if (lane == 0) top[w] = (float)((int)(bits >> 10) - 14);
+    }
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l, jl_kv4_attn_args a, int pairs) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr bool LO = sizeof(T) == 4;
+    using SM = pr_smem<HD, LO>;
+    constexpr int NG = SM::NG, PARTS = SM::PARTS, BLK = kv4_block_bytes(HD);
+    pr_bars& sh = *reinterpret_cast<pr_bars*>(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    griddep_wait();
+    griddep_launch_dependents();
+    // blocks in the order of falling work: the last rows of a prompt see the most
+    const int per = c.KH * a.B, pair = pairs - 1 - (int)blockIdx.x / per, kh = blockIdx.x % c.KH, b = blockIdx.x % per / c.KH;
+    const int gsz = a.H / c.KH, rows = a.T * gsz, row0 = pair * kPrPair;
+    const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, 0};
+    const int len = seqs.len(b);
+    if (len < 0 && threadIdx.x == 0 && pair == 0 && kh == 0 && a.err) atomicOr(a.err, kErrKvIndex);
+    auto sees = [&](int r) { return max(0, len - a.T + 1 + min(r, rows - 1) / gsz); };  // positions that row r sees
+    const int nb = (sees(row0 + kPrPair - 1) + kKv4Rows - 1) / kKv4Rows, tiles = rows - row0 > kPrTile ? 2 : 1;
+    // softmax threads: the row's place in q and out (rows past the last repeat it and are not written)
+    const int row = row0 + (int)threadIdx.x, rc = min(row, rows - 1), tok = rc / gsz, h = kh * gsz + rc % gsz;
+    const long long orow = (long long)b * a.T + tok;
+    auto write = [&](int d, const float (&x)[8]) {
+        put8(static_cast<T*>(a.out) + (orow * a.H + h) * HD + d, x);
+        if (a.outT)
+#pragma unroll
+            for (int j = 0; j < 8; j++) a.outT[(size_t)(h * HD + d + j) * a.outT_ld + orow] = x[j];
+    };
+    if (nb == 0) {  // nothing to see for any row
+        const float z[8] = {};
+        if (warp < 8 && row < rows)
+            for (int d = 0; d < HD; d += 8) write(d, z);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        sh.abort = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.raw_full[i], 1);
+            mbar_init(&sh.raw_empty[i], 4);
+            mbar_init(&sh.kv_full[i], 4);
+            mbar_init(&sh.kv_empty[i], tiles);
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.pv_done[i], 1);
+            mbar_init(&sh.fin[i], 1);
+        }
+        mbar_init(&sh.q_full, 4 * tiles);
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(2 * SM::TCOLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* abort = &sh.abort;
+
+    if (warp < 8) {
+        // ---------------- softmax: thread = row of tile t = TMEM lane
+        const int t = warp >> 2;
+        if (t < tiles) {
+            const int r = threadIdx.x & (kPrTile - 1);
+            const float f = pr_load_q<HD, LO, T>(
+                static_cast<const T*>(a.q) + orow * a.q_stride + h * HD, a.scale,
+                smem + SM::q + t * PARTS * SM::QTILE + (r >> 3) * 128 + (r & 7) * 16);
+            fence_proxy_async_smem();  // before the tensor cores read it
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_full);
+            const int n_row = sees(row), n_min = sees(row0 + t * kPrTile);
+            const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * SM::TCOLS, to = ts + SM::SCOLS;
+            float ref = -INFINITY;
+            float2 lsum = f2(0.0f);
+            int j = 0;
+            for (; j < nb; j++) {
+                const int s = j & 1, j0 = j * kKv4Rows;
+                // the scales (kv_full), then the scores
+                if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) || !pr_wait(&sh.s_full[t], j & 1, a.err, abort)) break;
+                tc_fence_after();
+                const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
+                float2 x[32];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    float a0[16], a1[16];
+                    if (NG == 2) tc_ld16x2(ts + 16 * q, ts + 64 + 16 * q, a0, a1);
+                    else tc_ld16(ts + 16 * q, a0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 k0 = *reinterpret_cast<const float4*>(sc + 16 * q + 4 * i);
+                        float2 u = __fmul2_rn(make_float2(a0[4 * i], a0[4 * i + 1]), make_float2(k0.x, k0.y));
+                        float2 v = __fmul2_rn(make_float2(a0[4 * i + 2], a0[4 * i + 3]), make_float2(k0.z, k0.w));
+                        if (NG == 2) {
+                            const float4 k1 = *reinterpret_cast<const float4*>(sc + kKv4Rows + 16 * q + 4 * i);
+                            u = __ffma2_rn(make_float2(a1[4 * i], a1[4 * i + 1]), make_float2(k1.x, k1.y), u);
+                            v = __ffma2_rn(make_float2(a1[4 * i + 2], a1[4 * i + 3]), make_float2(k1.z, k1.w), v);
+                        }
+                        x[8 * q + 2 * i] = u;
+                        x[8 * q + 2 * i + 1] = v;
+                    }
+                }
+                if (j0 + kKv4Rows > n_min) {
+                    const int n = n_row - j0;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        if (2 * i >= n) x[i].x = -INFINITY;
+                        if (2 * i + 1 >= n) x[i].y = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) mx = fmaxf(mx, fmaxf(x[i].x, x[i].y));
+                mx *= f;
+                const float top = fmaxf(sh.top[s][0], sh.top[s][1]);
+                const bool past = mx - ref > kTop - top;  // a weight past the limit, or the row's first
+                if (__any_sync(0xffffffffu, past)) {
+                    float al = 1.0f;
+                    if (past) {
+                        const float nref = mx + top - (kTop - kHeadroom);
+                        al = ex2(ref - nref);
+                        ref = nref;
+                    }
+                    lsum = __fmul2_rn(lsum, f2(al));
+                    if (j > 0) {  // the sums of earlier blocks are complete (S was issued after them)
+#pragma unroll 1
+                        for (int q = 0; q < NG * 4; q++) {
+                            float o[16];
+                            tc_ld16(to + 16 * q, o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] *= al;
+                            tc_st16(to + 16 * q, o);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                const float2 nr = f2(ref == -INFINITY ? 0.0f : -ref), ff = f2(f);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {  // 16 positions: weights, times V's scales of a group, hi and lo, into S's place
+                    float4 v0[4], v1[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        v0[i] = *reinterpret_cast<const float4*>(sc + 2 * kKv4Rows + 16 * q + 4 * i);
+                        if (NG == 2) v1[i] = *reinterpret_cast<const float4*>(sc + 3 * kKv4Rows + 16 * q + 4 * i);
+                    }
+                    uint32_t hi[NG][8], lo[NG][8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float2 p = __ffma2_rn(x[8 * q + i], ff, nr);
+                        p.x = ex2(p.x);
+                        p.y = ex2(p.y);
+                        lsum = __fadd2_rn(lsum, p);
+                        const float4 w0 = v0[i / 2], w1 = NG == 2 ? v1[i / 2] : w0;
+                        const float2 y0 = __fmul2_rn(p, i & 1 ? make_float2(w0.z, w0.w) : make_float2(w0.x, w0.y));
+                        if (LO) split2(y0, hi[0][i], lo[0][i]);
+                        else hi[0][i] = h2bits(__float22half2_rn(y0));
+                        if (NG == 2) {
+                            const float2 y1 = __fmul2_rn(p, i & 1 ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
+                            if (LO) split2(y1, hi[NG - 1][i], lo[NG - 1][i]);
+                            else hi[NG - 1][i] = h2bits(__float22half2_rn(y1));
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        tc_st8(ts + 64 * g + 8 * q, hi[g]);
+                        if (LO) tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
+                    }
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+            }
+            if (j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
+                tc_fence_after();
+                const float ls = lsum.x + lsum.y, inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+#pragma unroll 1
+                for (int q = 0; q < NG * 4; q++) {
+                    float o[16];
+                    tc_ld16(to + 16 * q, o);
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = ls == 0.0f ? 0.0f : o[i] * inv;
+                    if (row < rows) write(16 * q, y);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = ls == 0.0f ? 0.0f : o[8 + i] * inv;
+                    if (row < rows) write(16 * q + 8, y);
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------- unpack, and the copies of the cache's blocks
+        const int tid = threadIdx.x - 256, w = warp - 8;
+        const uint8_t* src = c.run(a.slots[b], l, kh);
+        uint8_t* raw = smem + SM::raw;
+        auto issue = [&](int j) {
+            mbar_expect_tx(&sh.raw_full[j & 1], BLK);
+            bulk_g2s(raw + (j & 1) * BLK, src + (size_t)j * BLK, BLK, &sh.raw_full[j & 1]);
+        };
+        int issued = 0, j = 0;
+        if (tid == 0)
+            while (issued < min(nb, 2)) issue(issued++);
+        __syncwarp();
+        for (; j < nb; j++) {
+            const int s = j & 1;
+            if (!pr_wait(&sh.raw_full[s], j >> 1 & 1, a.err, abort)) break;
+            if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, a.err, abort)) break;
+            pr_unpack<HD>(raw + s * BLK, smem + SM::k + s * SM::KTILE, smem + SM::v + s * SM::VTILE,
+                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], len - j * kKv4Rows, tid);
+            fence_proxy_async_smem();  // the operands to the tensor cores, the reads before the next copy
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh.kv_full[s]);
+                mbar_arrive(&sh.raw_empty[s]);
+            }
+            if (w == 0 && j + 2 < nb) {
+                if (!pr_wait(&sh.raw_empty[s], j >> 1 & 1, a.err, abort)) {
+                    j++;
+                    break;
+                }
+                if (tid == 0) issue(issued++);
+                __syncwarp();
+            }
+        }
+        if (tid == 0)
+            for (; j < issued; j++) mbar_wait_bounded(&sh.raw_full[j & 1], j >> 1 & 1, a.err);  // no copy left in flight
+    } else {
+        // ---------------- the instructions of tile t (a whole warp, one elected lane issues)
+        const int t = warp - 12;
+        if (t < tiles) {
+            const uint32_t idesc = umma_idesc_f16(64), ts = tmem + t * SM::TCOLS, to = ts + SM::SCOLS;
+            const uint64_t qd = umma_desc(smem + SM::q + t * PARTS * SM::QTILE, 2048, 128);
+            const uint64_t kd = umma_desc(smem + SM::k, 1024, 128);
+            const uint64_t vd = umma_desc(smem + SM::v, 8 * kPrCore, kPrCore);
+            bool ok = pr_wait(&sh.q_full, 0, a.err, abort);
+            for (int j = 0; ok && j < nb; j++) {
+                const int s = j & 1;
+                // S goes where P was: after the last block's second product
+                ok = pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) &&
+                     (j == 0 || pr_wait(&sh.pv_done[t], (j - 1) & 1, a.err, abort));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int g = 0; g < NG; g++)
+#pragma unroll
+                        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                tc_mma_ss(ts + 64 * g, qd + ((p * SM::QTILE + (g * 4 + k) * 4096) >> 4),
+                                          kd + ((s * SM::KTILE + (g * 4 + k) * 2048) >> 4), idesc, p + k > 0);
+                    tc_commit(&sh.s_full[t]);
+                }
+                __syncwarp();
+                ok = pr_wait(&sh.p_full[t], j & 1, a.err, abort);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int g = 0; g < NG; g++)
+#pragma unroll
+                        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                tc_mma_ts(to + 64 * g, ts + 64 * g + 32 * p + 8 * k,
+                                          vd + ((s * SM::VTILE + (g * 64 + k * 16) * kPrCore) >> 4), idesc, j + p + k > 0);
+                    tc_commit(&sh.pv_done[t]);
+                    tc_commit(&sh.kv_empty[s]);
+                }
+                __syncwarp();
+            }
+            if (elect_one()) tc_commit(&sh.fin[t]);  // no instruction left in flight
+            __syncwarp();
+            mbar_wait_bounded(&sh.fin[t], 0, a.err);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * SM::TCOLS));
+}
+
+}  // namespace jl
+
+namespace {
+
+template <int HD, typename T>
+int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+    using namespace jl;
+    const long long pairs = ((long long)a.T * (a.H / c.KH) + kPrPair - 1) / kPrPair, blocks = pairs * c.KH * a.B;
+    if (blocks > INT_MAX) return JL_ERR_INVALID;
+    return launch(k_kv4_prompt<HD, T>, dim3((unsigned)blocks), dim3(kPrThreads), (size_t)pr_smem<HD, sizeof(T) == 4>::total, s,
+                  c, l, a, (int)pairs);
+}
+
+template <int HD>
+int prompt_attrs() {
+    using namespace jl;
+    JL_CUDA(cudaFuncSetAttribute(k_kv4_prompt<HD, float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (pr_smem<HD, true>::total)));
+    JL_CUDA(cudaFuncSetAttribute(k_kv4_prompt<HD, __half>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (pr_smem<HD, false>::total)));
+    JL_CUDA(cudaFuncSetAttribute(k_kv4_prompt<HD, __nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (pr_smem<HD, false>::total)));
+    return JL_OK;
+}
+
+}  // namespace
+
+int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+    const int rc = jl_device_once(kOnceKv4Prompt, [] {
+        const int r = prompt_attrs<64>();
+        return r ? r : prompt_attrs<128>();
+    });
+    if (rc) return rc;
+    if (a.dtype == JL_F32) return c.hd == 64 ? launch_t<64, float>(c, l, a, s) : launch_t<128, float>(c, l, a, s);
+    if (a.dtype == JL_F16) return c.hd == 64 ? launch_t<64, __half>(c, l, a, s) : launch_t<128, __half>(c, l, a, s);
+    return c.hd == 64 ? launch_t<64, __nv_bfloat16>(c, l, a, s) : launch_t<128, __nv_bfloat16>(c, l, a, s);
+}
