@@ -12,11 +12,10 @@
 // moves only when a weight times its scale would pass 2^15 (jl_kv4_dev.cuh), and
 // the sums are then rescaled in TMEM.
 //
-// Roles (14 warps): 0-3 and 4-7 softmax of tile 0 and 1, 8-11 unpack the cache
-// block into the two operands (K as [64 positions][values], V as [values][64
-// positions]) and copy the next one in, 12 and 13 issue the instructions of tile 0
-// and 1. The tiles take turns on the tensor cores: one's products run beside the
-// other's softmax. Every wait is bounded; a timeout sets the status bit and an
+// Roles (12 warps, so that the softmax has 168 registers a thread): 0-3 and 4-7
+// softmax of tile 0 and 1, 8-10 unpack the cache block into the two operands (K as
+// [64 positions][values], V as [values][64 positions]) and copy the next one in, 11
+// issues the instructions. The tiles take turns on the tensor cores: one's products run beside the other's softmax. Every wait is bounded; a timeout sets the status bit and an
 // abort flag on which every role leaves its loop.
 //
 // Bound by the tensor cores in fp32 (two passes of each product) and by the
@@ -30,12 +29,12 @@
 
 namespace jl {
 
-constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 14 * 32;
+constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 12 * 32, kPrUnpack = 3;  // unpacking warps
 constexpr int kPrCore = 144;  // bytes between V's core matrices (128 of data: stores without bank conflicts)
 
 struct pr_bars {
     uint64_t raw_full[2], raw_empty[2], kv_full[2], kv_empty[2], q_full;
-    uint64_t s_full[2], p_full[2], pv_done[2], fin[2];
+    uint64_t s_full[2], p_full[2], pv_done[2], fin;
     uint32_t tmem;
     int abort;
     float top[2][2];  // per buffer, per warp of positions: 2^top is above V's scales
@@ -44,7 +43,8 @@ struct pr_bars {
 template <int HD, bool LO>
 struct pr_smem {
     static constexpr int NG = HD / 64, PARTS = LO ? 2 : 1;
-    static constexpr int QTILE = kPrTile * HD * 2, KTILE = kKv4Rows * HD * 2, VTILE = NG * 64 * kPrCore;
+    static constexpr int QCHUNK = kPrTile * 16 + 16;  // bytes of 8 values of all rows (16 more: stores spread over the banks)
+    static constexpr int QTILE = HD / 8 * QCHUNK, KTILE = kKv4Rows * HD * 2, VTILE = NG * 64 * kPrCore;
     static constexpr int sc = 512;                       // fp32 scales [2 buffers][K g0, K g1, V g0, V g1][64]
     static constexpr int q = sc + 2 * 4 * kKv4Rows * 4;  // [tile][part][chunk of 8 values][128 rows x 16 B]
     static constexpr int k = q + 2 * PARTS * QTILE;      // [buffer][chunk][64 positions x 16 B]
@@ -56,52 +56,94 @@ struct pr_smem {
 };
 
 // A wait of a whole warp, bounded; false when it ran out or another role gave up.
+// (mbarrier.test_wait in place of try_wait, polling without a suspension, was 6 %
+// slower: the polls take the softmax's issue slots.)
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
     bool ok = mbar_try_wait(bar, parity);
-    const long long t0 = clock64();
-    for (int i = 1; !ok; i++) {
-        ok = mbar_try_wait(bar, parity);
-        if (!ok && (i & 63) == 0) {
-            if (*abort) break;
-            if (clock64() - t0 > kWaitLimitCycles) {
-                if (err) atomicOr(err, kErrTimeout);
-                *abort = 1;
-                break;
+    if (!ok) {
+        const long long t0 = clock64();
+        for (int i = 1; !ok; i++) {
+            ok = mbar_try_wait(bar, parity);
+            if (!ok && (i & 63) == 0) {
+                if (*abort) break;
+                if (clock64() - t0 > kWaitLimitCycles) {
+                    if (err) atomicOr(err, kErrTimeout);
+                    *abort = 1;
+                    break;
+                }
             }
         }
     }
     return __all_sync(0xffffffffu, ok);
 }
 
-// The thread's q row, scaled to base-2 scores and by a power of two (its largest
-// value in [2^10, 2^11)), into the operand's hi and lo parts; returns the power's inverse.
-template <int HD, bool LO, typename T>
-__device__ __forceinline__ float pr_load_q(const T* q, float scale, uint8_t* dst) {
-    float mx = 0.0f;
-    for (int c = 0; c < HD / 8; c++) {
-        float x[8];
-        load8(q + 8 * c, x);
-#pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[j] * (scale * 1.4426950408889634f)));
-    }
-    int e = (int)(__float_as_uint(mx) >> 23);
-    e = min(max(e, 11), 253);
-    const float inv = __uint_as_float((uint32_t)(264 - e) << 23);
-    for (int c = 0; c < HD / 8; c++) {
-        float x[8];
-        load8(q + 8 * c, x);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = x[j] * (scale * 1.4426950408889634f) * inv;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) split2(make_float2(x[j], x[j + 4]), hi[j], lo[j]);  // the order of an unpacked word
-        *reinterpret_cast<uint4*>(dst + c * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (LO) *reinterpret_cast<uint4*>(dst + pr_smem<HD, LO>::QTILE + c * 2048) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    return __uint_as_float((uint32_t)(e - 10) << 23);
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const T* h = reinterpret_cast<const T*>(&w);
+    return make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
 }
 
-// Unpacks one cache block (128 threads, tid 0..127) into operand tiles and fp32
+// The warp's 32 q rows, scaled to base-2 scores and by a power of two each (the
+// largest value in [2^10, 2^11)), into the operand's hi and lo parts from row r0 on;
+// returns the inverse of the power of row `lane`. HD / 4 lanes read a row (a row per
+// thread touched 32 lines a load and took 13 us a block). src(i): row i.
+template <int HD, bool LO, typename T, typename F>
+__device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int r0) {
+    constexpr int LPR = HD / 4, RPW = 32 / LPR, ROWS = 8;  // rows of a lane in flight
+    using SM = pr_smem<HD, LO>;
+    const int lane = threadIdx.x & 31, w = lane % LPR;
+    float f = 0.0f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += ROWS * RPW) {
+        float4 x[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) x[i] = load4(src(i0 + i * RPW + lane / LPR) + 4 * w);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            const int row = i0 + i * RPW + lane / LPR;
+            const float k = scale * 1.4426950408889634f;
+            float4 y = make_float4(x[i].x * k, x[i].y * k, x[i].z * k, x[i].w * k);
+            float mx = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+#pragma unroll
+            for (int o = LPR / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            int e = (int)(__float_as_uint(mx) >> 23);
+            e = min(max(e, 11), 253);
+            const float inv = __uint_as_float((uint32_t)(264 - e) << 23), fr = __uint_as_float((uint32_t)(e - 10) << 23);
+#pragma unroll
+            for (int q = 0; q < RPW; q++) {
+                const float fq = __shfl_sync(0xffffffffu, fr, q * LPR);
+                if (lane == i0 + i * RPW + q) f = fq;
+            }
+            y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+            // values (0, 4), (1, 5) of a chunk in its even lane, (2, 6), (3, 7) in its odd one: an unpacked word's order
+            const bool odd = w & 1;
+            const float sa = __shfl_xor_sync(0xffffffffu, odd ? y.x : y.z, 1), sb = __shfl_xor_sync(0xffffffffu, odd ? y.y : y.w, 1);
+            uint2 hi, lo;
+            split2(odd ? make_float2(sa, y.z) : make_float2(y.x, sa), hi.x, lo.x);
+            split2(odd ? make_float2(sb, y.w) : make_float2(y.y, sb), hi.y, lo.y);
+            uint8_t* p = dst + w / 2 * SM::QCHUNK + (r0 + row) * 16 + (w & 1) * 8;
+            *reinterpret_cast<uint2*>(p) = hi;
+            if (LO) *reinterpret_cast<uint2*>(p + SM::QTILE) = lo;
+        }
+    }
+    return f;
+}
+
+// 16 bytes of values.
+__device__ __forceinline__ void store_piece(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, const float* x) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = x[j];
+    put8(p, y);
+}
+
+// Unpacks one cache block (kPrUnpack warps, tid from 0) into operand tiles and fp32
 // scales; positions from n on (never written) get scales of 0.
 template <int HD>
 __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, float* top, int n, int tid) {
@@ -109,8 +151,8 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
     const int lane = tid & 31, w = tid >> 5;
     // K: lane (t, position of 8) takes words 2t, 2t + 1 of the groups
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int t = lane >> 3, o = w + 4 * i, r = 8 * o + (lane & 7);
+    for (int o = w; o < 8; o += kPrUnpack) {
+        const int t = lane >> 3, r = 8 * o + (lane & 7);
         uint32_t kw[2 * NG];
         if (NG == 2) {
             const uint4 x = *reinterpret_cast<const uint4*>(raw + r * ROW + 16 * t);
@@ -129,8 +171,11 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
             }
     }
     // V: thread (8 positions o, word u of group g) writes the 8 x 8 core matrix of its values
-    if (tid < 64 * NG) {
-        const int u = lane & 7, g = NG == 2 ? lane >> 3 & 1 : 0, o = NG == 2 ? 2 * w + (lane >> 4) : tid >> 3;
+#pragma unroll
+    for (int i0 = 0; i0 < 64 * NG; i0 += 32 * kPrUnpack) {
+        const int task = i0 + tid;
+        if (task >= 64 * NG) break;
+        const int u = task & 7, g = NG == 2 ? task >> 3 & 1 : 0, o = task >> (NG == 2 ? 4 : 3);
         uint32_t x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -205,18 +250,18 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         sh.abort = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.raw_full[i], 1);
-            mbar_init(&sh.raw_empty[i], 4);
-            mbar_init(&sh.kv_full[i], 4);
+            mbar_init(&sh.raw_empty[i], kPrUnpack);
+            mbar_init(&sh.kv_full[i], kPrUnpack);
             mbar_init(&sh.kv_empty[i], tiles);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_full[i], 4);
             mbar_init(&sh.pv_done[i], 1);
-            mbar_init(&sh.fin[i], 1);
         }
         mbar_init(&sh.q_full, 4 * tiles);
+        mbar_init(&sh.fin, 1);
         mbar_fence_init();
     }
-    if (warp == 12) {
+    if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(2 * SM::TCOLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -231,10 +276,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         // ---------------- softmax: thread = row of tile t = TMEM lane
         const int t = warp >> 2;
         if (t < tiles) {
-            const int r = threadIdx.x & (kPrTile - 1);
+            uint8_t* qs = smem + SM::q + t * PARTS * SM::QTILE;
             const float f = pr_load_q<HD, LO, T>(
-                static_cast<const T*>(a.q) + orow * a.q_stride + h * HD, a.scale,
-                smem + SM::q + t * PARTS * SM::QTILE + (r >> 3) * 128 + (r & 7) * 16);
+                [&](int i) {
+                    const int r = min(row0 + warp * 32 + i, rows - 1);
+                    return static_cast<const T*>(a.q) + ((long long)b * a.T + r / gsz) * a.q_stride + (kh * gsz + r % gsz) * HD;
+                },
+                a.scale, qs, (warp & 3) * 32);
             fence_proxy_async_smem();  // before the tensor cores read it
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full);
@@ -343,21 +391,36 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             if (j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
                 tc_fence_after();
                 const float ls = lsum.x + lsum.y, inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
+                constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
+                T* st = reinterpret_cast<T*>(qs) + (warp & 3) * 32 * HD;
 #pragma unroll 1
                 for (int q = 0; q < NG * 4; q++) {
                     float o[16];
                     tc_ld16(to + 16 * q, o);
-                    float y[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = ls == 0.0f ? 0.0f : o[i] * inv;
-                    if (row < rows) write(16 * q, y);
+                    for (int i = 0; i < 16; i++) o[i] = ls == 0.0f ? 0.0f : o[i] * inv;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = ls == 0.0f ? 0.0f : o[8 + i] * inv;
-                    if (row < rows) write(16 * q + 8, y);
+                    for (int i = 0; i < 16; i += VPC) {
+                        const int p = (16 * q + i) / VPC;
+                        store_piece(st + (lane * CPR + (p ^ (lane & 7))) * VPC, o + i);
+                    }
+                    if (a.outT && row < rows)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) a.outT[(size_t)(h * HD + 16 * q + i) * a.outT_ld + orow] = o[i];
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * CPR; i += 32) {
+                    const int r = i / CPR, p = i % CPR, g = row0 + warp * 32 + r;
+                    if (g >= rows) break;
+                    const long long to_row = (long long)b * a.T + g / gsz;
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (to_row * a.H + kh * gsz + g % gsz) * HD + p * VPC) =
+                        *reinterpret_cast<const uint4*>(st + (r * CPR + (p ^ (r & 7))) * VPC);
                 }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 8 + kPrUnpack) {
         // ---------------- unpack, and the copies of the cache's blocks
         const int tid = threadIdx.x - 256, w = warp - 8;
         const uint8_t* src = c.run(a.slots[b], l, kh);
@@ -394,37 +457,43 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         if (tid == 0)
             for (; j < issued; j++) mbar_wait_bounded(&sh.raw_full[j & 1], j >> 1 & 1, a.err);  // no copy left in flight
     } else {
-        // ---------------- the instructions of tile t (a whole warp, one elected lane issues)
-        const int t = warp - 12;
-        if (t < tiles) {
-            const uint32_t idesc = umma_idesc_f16(64), ts = tmem + t * SM::TCOLS, to = ts + SM::SCOLS;
-            const uint64_t qd = umma_desc(smem + SM::q + t * PARTS * SM::QTILE, 2048, 128);
-            const uint64_t kd = umma_desc(smem + SM::k, 1024, 128);
-            const uint64_t vd = umma_desc(smem + SM::v, 8 * kPrCore, kPrCore);
-            bool ok = pr_wait(&sh.q_full, 0, a.err, abort);
-            for (int j = 0; ok && j < nb; j++) {
+        // ---------------- the instructions (a whole warp, one elected lane issues). The
+        // tiles take turns: a tile's values and its next scores go out together, and
+        // the other tile's softmax runs meanwhile. (With an issuer per tile both were in
+        // the same phase and nothing overlapped: 6,760 cycles for a block of both.)
+        const uint32_t idesc = umma_idesc_f16(64);
+        const uint64_t kd = umma_desc(smem + SM::k, 1024, 128);
+        const uint64_t vd = umma_desc(smem + SM::v, 8 * kPrCore, kPrCore);
+        auto scores = [&](int t, int j) {
+            if (!pr_wait(&sh.kv_full[j & 1], j >> 1 & 1, a.err, abort)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t qd = umma_desc(smem + SM::q + t * PARTS * SM::QTILE, SM::QCHUNK, 128);
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_ss(tmem + t * SM::TCOLS + 64 * g, qd + ((p * SM::QTILE + (g * 4 + k) * 2 * SM::QCHUNK) >> 4),
+                                      kd + (((j & 1) * SM::KTILE + (g * 4 + k) * 2048) >> 4), idesc, p + k > 0);
+                tc_commit(&sh.s_full[t]);
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = pr_wait(&sh.q_full, 0, a.err, abort);
+        for (int t = 0; ok && t < tiles; t++) ok = scores(t, 0);
+        for (int j = 0; ok && j < nb; j++)
+            for (int t = 0; ok && t < tiles; t++) {
                 const int s = j & 1;
-                // S goes where P was: after the last block's second product
-                ok = pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) &&
-                     (j == 0 || pr_wait(&sh.pv_done[t], (j - 1) & 1, a.err, abort));
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-#pragma unroll
-                    for (int g = 0; g < NG; g++)
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                tc_mma_ss(ts + 64 * g, qd + ((p * SM::QTILE + (g * 4 + k) * 4096) >> 4),
-                                          kd + ((s * SM::KTILE + (g * 4 + k) * 2048) >> 4), idesc, p + k > 0);
-                    tc_commit(&sh.s_full[t]);
+                if (!pr_wait(&sh.p_full[t], j & 1, a.err, abort)) {
+                    ok = false;
+                    break;
                 }
-                __syncwarp();
-                ok = pr_wait(&sh.p_full[t], j & 1, a.err, abort);
-                if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
+                    const uint32_t ts = tmem + t * SM::TCOLS, to = ts + SM::SCOLS;
 #pragma unroll
                     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -437,16 +506,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                     tc_commit(&sh.kv_empty[s]);
                 }
                 __syncwarp();
+                // the next scores go where these weights are: after the product that reads them
+                if (j + 1 < nb) ok = pr_wait(&sh.pv_done[t], j & 1, a.err, abort) && scores(t, j + 1);
             }
-            if (elect_one()) tc_commit(&sh.fin[t]);  // no instruction left in flight
-            __syncwarp();
-            mbar_wait_bounded(&sh.fin[t], 0, a.err);
-        }
+        if (elect_one()) tc_commit(&sh.fin);  // no instruction left in flight
+        __syncwarp();
+        mbar_wait_bounded(&sh.fin, 0, a.err);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12)
+    if (warp == 11)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * SM::TCOLS));
 }
 
