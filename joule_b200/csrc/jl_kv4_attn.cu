@@ -122,8 +122,7 @@ constexpr int kKvWarps = 12;  // warps per block, one block per SM (168 register
 template <int HD>
 struct kv4_smem {
     static constexpr int UNIT = kv4_block_bytes(HD);
-    static constexpr int bars = kKvWarps * kKvRing * UNIT;
-    static constexpr int stat = bars + kKvWarps * kKvRing * 8;     // reference, sum [warps][2][8] of the block's sum
+    static constexpr int stat = kKvWarps * kKvRing * UNIT;  // reference, sum [warps][2][8] of the block's sum
     static constexpr int total = stat + kKvWarps * 2 * kKvTile * 4;
     static_assert(kKvRing * UNIT >= kKvTile * HD * 4, "a warp's ring holds its sums");
 };
@@ -379,8 +378,9 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
 
 // Bound by HBM for long caches (the codes and scales are read once, 4.25 bits
 // per value) and by launch and load latency for short ones. Each warp has a ring
-// of two whole cache blocks, filled by one bulk copy each; no barrier between warps
-// but for the sum of a block that is inside one segment.
+// of two whole cache blocks, filled by 16-byte asynchronous copies (17 instructions a
+// block; a bulk copy held its issuing warp for hundreds of ns); no barrier between
+// warps but for the sum of a block that is inside one segment.
 template <int HD, typename T>
 __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -388,12 +388,6 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     constexpr int UNIT = SM::UNIT, NG = HD / 64, NW = kKvWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kKvRing * UNIT;
-    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SM::bars) + warp * kKvRing;
-    if (lane == 0) {
-        for (int i = 0; i < kKvRing; i++) mbar_init(bar + i, 1);
-        mbar_fence_init();
-    }
-    __syncwarp();
     griddep_wait();
     griddep_launch_dependents();
     const int gsz = a.H / c.KH, rows = a.T * gsz, S = R * c.KH;
@@ -458,17 +452,19 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     const uint32_t seg0 = u0 - pr.j;
     const bool joined = !whole && cut.nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nu;
     int issued = 0;
-    auto issue = [&]() {
-        if (lane == 0) {
-            const int k = issued % kKvRing;
-            mbar_expect_tx(bar + k, UNIT);
-            bulk_g2s(ring + k * UNIT, pr.p, UNIT, bar + k);
+    auto issue = [&]() {  // one group of copies per unit, an empty one past the last
+        if (issued < units) {
+            uint8_t* dst = ring + issued % kKvRing * UNIT + lane * 16;
+#pragma unroll
+            for (int i = 0; i < (UNIT / 16 + 31) / 32; i++)
+                if (UNIT % 512 == 0 || i * 512 + lane * 16 < UNIT) cp_async16(dst + i * 512, pr.p + i * 512 + lane * 16);
+            if (++issued < units) advance(pr);
         }
-        if (++issued < units) advance(pr);
+        cp_async_commit();
     };
     issue();  // all warps' first units before anyone's others
     kv4_state<HD> st;
-    int slot_k = 0, phase = 0, n_min = 0, n_max = 0;
+    int n_min = 0, n_max = 0;
     bool began = false;
     for (int i = 0; i < units; i++) {
         if (!began) {  // a new segment: its rows (those past the last repeat it and are not written)
@@ -482,16 +478,16 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             n_min = sees(0), n_max = sees(kKvTile - 1);
             began = true;
             if (i == 0) {
-                while (issued < min(units, kKvRing)) issue();
+#pragma unroll
+                for (int k = 1; k < kKvRing; k++) issue();
             }
         }
-        if (!mbar_wait_bounded(bar + slot_k, phase, a.err)) break;  // flagged; the block's sum still meets
-        const int j0 = co.j * kKvUnit;
-        if (j0 < n_max) kv4_block<HD, sizeof(T) == 4>(st, ring + slot_k * UNIT, j0, n_min, n_max);
-        fence_proxy_async_smem();
+        cp_async_wait<kKvRing - 1>();  // this unit's copies, by every lane
         __syncwarp();
-        if (issued < units) issue();
-        if (++slot_k == kKvRing) slot_k = 0, phase ^= 1;
+        const int j0 = co.j * kKvUnit;
+        if (j0 < n_max) kv4_block<HD, sizeof(T) == 4>(st, ring + i % kKvRing * UNIT, j0, n_min, n_max);
+        __syncwarp();
+        issue();
         const bool ends = co.j == co.nu - 1;
         if (ends || i == units - 1) {
             float lrow = st.l.x + st.l.y;
@@ -736,7 +732,13 @@ long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
 }
 
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
-    if ((long long)a.T * (a.H / c.KH) >= 128) return jl_launch_kv4_prompt(c, l, a, s);
+    // The tcgen05 kernel takes the time of 256 query rows per block and wave whatever
+    // the rows are, this file's a time by the rows; they meet at 76 rows per SM (fp32,
+    // 32/4 heads of 128 over 2,048: 64 tokens of 4 sequences, 8,192 rows: 79 us here
+    // against 99 there; 128 tokens, 16,384 rows: 147 against 99; 0.75 to 0.88 and 1.3 to
+    // 1.7 over head dims, types and lengths).
+    const long long rows = (long long)a.B * a.T * a.H, blocks = jl_kv4_prompt_blocks(c, a);
+    if (rows >= 76 * std::max<long long>(sm_count(), blocks)) return jl_launch_kv4_prompt(c, l, a, s);
     const int rc = jl_device_once(kOnceKv4, [] {
         const int r = attn_attrs<64>();
         return r ? r : attn_attrs<128>();

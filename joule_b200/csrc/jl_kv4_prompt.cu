@@ -527,7 +527,7 @@ namespace {
 template <int HD, typename T>
 int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
     using namespace jl;
-    const long long pairs = ((long long)a.T * (a.H / c.KH) + kPrPair - 1) / kPrPair, blocks = pairs * c.KH * a.B;
+    const long long blocks = jl_kv4_prompt_blocks(c, a), pairs = blocks / ((long long)c.KH * a.B);
     if (blocks > INT_MAX) return JL_ERR_INVALID;
     return launch(k_kv4_prompt<HD, T>, dim3((unsigned)blocks), dim3(kPrThreads), (size_t)pr_smem<HD, sizeof(T) == 4>::total, s,
                   c, l, a, (int)pairs);
@@ -546,6 +546,10 @@ int prompt_attrs() {
 }
 
 }  // namespace
+
+long long jl_kv4_prompt_blocks(const jl::kv4_dims& c, const jl_kv4_attn_args& a) {
+    return ((long long)a.T * (a.H / c.KH) + jl::kPrPair - 1) / jl::kPrPair * c.KH * a.B;
+}
 
 int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
     const int rc = jl_device_once(kOnceKv4Prompt, [] {
