@@ -319,14 +319,37 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
                 f[gr][i][2] = code_even(i ? y >> 8 : y), f[gr][i][3] = code_odd(i ? y >> 8 : y);
             }
         }
-#pragma unroll
-        for (int part = 0; part < (LO ? 2 : 1); part++)
+        if constexpr (!LO) {
 #pragma unroll
             for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                 for (int i = 0; i < 2; i++)
-                    mma16816(st.o[gr][2 * q + i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3],
-                             part ? bl[gr][0] : bh[gr][0], part ? bl[gr][1] : bh[gr][1]);
+                    mma16816(st.o[gr][2 * q + i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bh[gr][0], bh[gr][1]);
+        } else {
+            // The instruction's sums are cut off, not rounded: 16 positions start from zero and
+            // are added here, or a long run's outputs shrink (by 1.3e-6 of themselves after 18
+            // blocks, and on with the length).
+            float acc[NG][2][4];
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    mma16816_0(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bl[gr][0], bl[gr][1]);
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    mma16816(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bh[gr][0], bh[gr][1]);
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float (&o)[4] = st.o[gr][2 * q + i];
+                    const float2 x0 = __fadd2_rn(make_float2(o[0], o[1]), make_float2(acc[gr][i][0], acc[gr][i][1]));
+                    const float2 x1 = __fadd2_rn(make_float2(o[2], o[3]), make_float2(acc[gr][i][2], acc[gr][i][3]));
+                    o[0] = x0.x, o[1] = x0.y, o[2] = x1.x, o[3] = x1.y;
+                }
+        }
     }
 }
 

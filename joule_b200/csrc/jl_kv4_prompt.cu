@@ -30,6 +30,14 @@
 namespace jl {
 
 constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 12 * 32, kPrUnpack = 3;  // unpacking warps
+// The tensor cores' sums are cut off, not rounded: over n blocks they come out short by
+// about 1e-7 n of themselves. In fp32 calls the sums therefore move to the rows of `out`
+// every kPrFold blocks, which hold them until the end, and TMEM starts anew. 2,047 rows
+// of 32/4 heads of 128 over 4,100 positions: error 1.6e-6 and 309 us (never: 7.4e-6,
+// 264 us; every 12: 2.0e-6, every 16: 2.5e-6); over 23,000: 1.9e-6 (never: 4.7e-5).
+// 16-bit calls have half the instructions per block and no room in `out`: their sums
+// stay in TMEM and are short by half a step of fp16 after some 480,000 positions.
+constexpr int kPrFold = 8;
 constexpr int kPrCore = 144;  // bytes between V's core matrices (128 of data: stores without bank conflicts)
 
 struct pr_bars {
@@ -38,6 +46,31 @@ struct pr_bars {
     uint32_t tmem;
     int abort;
     float top[2][2];  // per buffer, per warp of positions: 2^top is above V's scales
+};
+
+struct pr_held {
+    float* out;
+    int H, gsz, row0, rows;  // out: the sequence's first token, the kv head's first head
+    float ref[kPrPair];      // of what a row's places hold
+    struct place {
+        float4* p;
+        int left, run, rest, gap;  // pieces left in the run; a run's; of a step past whole runs; between runs
+        long long step;
+        __device__ float4* next() {
+            float4* at = p;
+            p += step;
+            if ((left -= rest) <= 0) left += run, p += gap;
+            return at;
+        }
+    };
+    __device__ bool mine() const { return row0 + (int)threadIdx.x < rows; }
+    template <int HD>
+    __device__ place first() const {
+        const int r0 = row0 + (int)(threadIdx.x & ~31u), nv = min(32, rows - r0), run = gsz * (HD / 4), gap = (H - gsz) * (HD / 4);
+        const int at = r0 % gsz * (HD / 4) + (int)(threadIdx.x & 31), left = run - at % run;
+        float4* p = reinterpret_cast<float4*>(out + (long long)(r0 / gsz + at / run) * H * HD) + (run - left);
+        return place{p, left, run, nv % run, gap, nv + (long long)(nv / run) * gap};
+    }
 };
 
 template <int HD, bool LO>
@@ -50,7 +83,8 @@ struct pr_smem {
     static constexpr int k = q + 2 * PARTS * QTILE;      // [buffer][chunk][64 positions x 16 B]
     static constexpr int v = k + 2 * KTILE;              // [buffer][group][8 positions' chunk][8 values' core]
     static constexpr int raw = v + 2 * VTILE;
-    static constexpr int total = raw + 2 * kv4_block_bytes(HD);
+    static constexpr int held = raw + 2 * kv4_block_bytes(HD);
+    static constexpr int total = held + (LO ? (int)sizeof(pr_held) : 0);
     static constexpr int SCOLS = NG * 64, TCOLS = 2 * SCOLS;  // TMEM columns of a tile: S (then P), O
     static_assert(sizeof(pr_bars) <= 512 && total <= 227 * 1024, "shared memory");
 };
@@ -213,6 +247,64 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
     }
 }
 
+// Moves the finished sums in TMEM (HD columns from `to`) to `out`, onto what earlier
+// calls put there, rescaled to the reference `ref`. Places: pieces (4 values) of the
+// warp's rows in turn over the rows' own part of `out` (runs of the kv head's heads,
+// one run a token). A call of its own that finds its arguments in shared memory:
+// inlined it took the softmax's registers (chunk below: 326 us inlined, 309 so).
+template <int HD>
+__device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool holds) {
+    const float href = held->ref[threadIdx.x], al = ex2(href - (ref == -INFINITY ? 0.0f : ref));
+    const bool mine = held->mine();
+    held->ref[threadIdx.x] = ref;
+    pr_held::place st = held->first<HD>(), ld = st;
+#pragma unroll 1
+    for (int q = 0; q < HD; q += 32) {
+        float4 y[8];
+        if (holds && mine)
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = *ld.next();
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            float o[16];
+            __syncwarp();
+            tc_ld16(to + q + 16 * p, o);
+            if (mine)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float4 x = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    const float4 z = y[4 * p + i];
+                    if (holds) x = make_float4(fmaf(z.x, al, x.x), fmaf(z.y, al, x.y), fmaf(z.z, al, x.z), fmaf(z.w, al, x.w));
+                    *st.next() = x;
+                }
+        }
+    }
+}
+
+// At the end: what the places hold, back onto the last sums in TMEM.
+template <int HD>
+__device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
+    const float al = ex2(held->ref[threadIdx.x] - (ref == -INFINITY ? 0.0f : ref));
+    pr_held::place at = held->first<HD>();
+#pragma unroll 1
+    for (int q = 0; q < HD; q += 16) {
+        float4 y[4] = {};
+        if (held->mine())
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = *at.next();
+        float o[16];
+        __syncwarp();
+        tc_ld16(to + q, o);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            o[4 * i] = fmaf(y[i].x, al, o[4 * i]), o[4 * i + 1] = fmaf(y[i].y, al, o[4 * i + 1]);
+            o[4 * i + 2] = fmaf(y[i].z, al, o[4 * i + 2]), o[4 * i + 3] = fmaf(y[i].w, al, o[4 * i + 3]);
+        }
+        tc_st16(to + q, o);
+    }
+    tc_wait_st();
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l, jl_kv4_attn_args a, int pairs) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -246,8 +338,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             for (int d = 0; d < HD; d += 8) write(d, z);
         return;
     }
+    pr_held* held = reinterpret_cast<pr_held*>(smem + SM::held);  // fp32 calls
     if (threadIdx.x == 0) {
         sh.abort = 0;
+        if (LO) {
+            held->out = static_cast<float*>(a.out) + ((long long)b * a.T * a.H + kh * gsz) * HD;
+            held->H = a.H, held->gsz = gsz, held->row0 = row0, held->rows = rows;
+        }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.raw_full[i], 1);
             mbar_init(&sh.raw_empty[i], kPrUnpack);
@@ -270,6 +367,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    auto starts = [](int j) { return LO ? j % kPrFold == 0 : j == 0; };  // blocks at which TMEM's sums start anew
     volatile int* abort = &sh.abort;
 
     if (warp < 8) {
@@ -296,6 +394,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 // the scales (kv_full), then the scores
                 if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) || !pr_wait(&sh.s_full[t], j & 1, a.err, abort)) break;
                 tc_fence_after();
+                if (LO && j > 0 && starts(j)) {  // S was issued after the last block's values: the sums are complete
+                    pr_fold<HD>(to, ref, held, j > kPrFold);
+                }
                 const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
                 float2 x[32];
                 float mx = -INFINITY;
@@ -339,7 +440,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                         ref = nref;
                     }
                     lsum = __fmul2_rn(lsum, f2(al));
-                    if (j > 0) {  // the sums of earlier blocks are complete (S was issued after them)
+                    if (!starts(j)) {  // the sums of earlier blocks are complete (S was issued after them)
 #pragma unroll 1
                         for (int q = 0; q < NG * 4; q++) {
                             float o[16];
@@ -390,6 +491,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             }
             if (j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
                 tc_fence_after();
+                if (LO && nb > kPrFold) pr_unfold<HD>(to, ref, held);
                 const float ls = lsum.x + lsum.y, inv = ls == 0.0f ? 0.0f : 1.0f / ls;
                 // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
                 constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
@@ -409,7 +511,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
 #pragma unroll
                         for (int i = 0; i < 16; i++) a.outT[(size_t)(h * HD + 16 * q + i) * a.outT_ld + orow] = o[i];
                 }
-                __syncwarp();
+                __syncwarp();  // (and the warp has taken what `out` held)
 #pragma unroll 4
                 for (int i = lane; i < 32 * CPR; i += 32) {
                     const int r = i / CPR, p = i % CPR, g = row0 + warp * 32 + r;
@@ -493,6 +595,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 }
                 tc_fence_after();
                 if (elect_one()) {
+                    const bool fresh = starts(j);
                     const uint32_t ts = tmem + t * SM::TCOLS, to = ts + SM::SCOLS;
 #pragma unroll
                     for (int g = 0; g < NG; g++)
@@ -501,7 +604,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 tc_mma_ts(to + 64 * g, ts + 64 * g + 32 * p + 8 * k,
-                                          vd + ((s * SM::VTILE + (g * 64 + k * 16) * kPrCore) >> 4), idesc, j + p + k > 0);
+                                          vd + ((s * SM::VTILE + (g * 64 + k * 16) * kPrCore) >> 4), idesc,
+                                          p + k > 0 || !fresh);
                     tc_commit(&sh.pv_done[t]);
                     tc_commit(&sh.kv_empty[s]);
                 }

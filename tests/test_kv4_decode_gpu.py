@@ -130,6 +130,29 @@ def test_prompts_and_steps(name, kw):
     dec.close(), ref.close()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_prompt_in_one_chunk(hd):
+    """A prompt of 713 rows of 16 heads in one call: the last position's logits over
+    the values that the cache then holds, and the last cached rows."""
+    from oracle.decode import embed, make_model
+    s = _shape("qwen3s", H=16, KH=4, hd=hd, maxT=720)
+    model = make_model(s, seed=54)
+    n = 713
+    p = np.random.default_rng(hd).integers(0, s.V, n).astype(np.int32)
+    dec = _decoder(model, n, n)
+    logits = torch.empty(s.V, device="cuda")
+    dec.prefill(1, torch.from_numpy(p).cuda(), logits=logits)
+    dec.check()
+    rows = _cached(dec, 1, n)
+    want, ks, vs, top = okv4.decode_step(model, embed(model, p[-1:]), [n - 1], lambda l, b: rows[l])
+    for l in range(s.L):
+        _held_near(rows[l][0][-1], ks[l][0], _tol(s, top))
+        _held_near(rows[l][1][-1], vs[l][0], _tol(s, top))
+    err = np.linalg.norm(logits.double().cpu().numpy() - want[0]) / np.linalg.norm(want[0])
+    assert err <= _tol(s, top), err
+    dec.close()
+
+
 @pytest.mark.parametrize("B", [16, 33])
 def test_large_batches(B):
     """Batches whose matvecs read the attention's column-major copy; ragged positions over seeded caches."""

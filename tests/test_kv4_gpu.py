@@ -199,7 +199,7 @@ STEP = [  # B, H, kv, hd, lens
     (1, 1, 1, 64, [1]), (1, 32, 4, 128, [1]), (3, 8, 1, 128, [63, 64, 65]), (5, 6, 2, 64, [0, 1, 2, 200, 127]),
     (2, 7, 7, 128, [700, 3]), (4, 10, 2, 64, [129, 0, 640, 511]), (3, 16, 1, 128, [300, 5, 77]),
     (2, 22, 2, 64, [90, 1000]), (1, 16, 16, 128, [2500]), (7, 4, 4, 64, [0, 0, 0, 0, 0, 0, 0]),
-    (40, 8, 2, 128, [(37 * b) % 190 for b in range(40)]),
+    (40, 8, 2, 128, [(37 * b) % 190 for b in range(40)]), (170, 2, 1, 64, [(53 * b) % 301 for b in range(170)]),
 ]
 
 
@@ -246,7 +246,22 @@ def test_chunk(B, T, H, kv, hd, lens, t):
     _check(got, q.double().cpu().numpy(), ks, vs, hd ** -0.5, t)
 
 
-@pytest.mark.parametrize("T", [1, 24])
+MANY = [  # B, T, H, kv, hd, lens: 76 rows and more for each SM of 148 and each block of 256
+    (1, 710, 16, 4, 128, [1300]), (3, 260, 15, 3, 64, [1100, 259, 700]), (2, 40, 142, 2, 128, [600, 0]),
+    (70, 8, 24, 2, 64, [(37 * b) % 301 for b in range(70)]), (1, 2900, 4, 4, 128, [2900]), (1, 2, 6002, 2, 64, [1290]),
+    (1, 1, 11904, 1, 128, [577]), (2, 360, 16, 4, 64, [512, 513]),
+]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", MANY)
+def test_many_rows(B, T, H, kv, hd, lens, t):
+    """Calls whose rows fill the tensor cores' tiles: ends inside a tile, blocks of one
+    tile, sums of one block to 46, tokens whose heads pass a tile, empty sequences."""
+    test_chunk(B, T, H, kv, hd, lens, t)
+
+
+@pytest.mark.parametrize("T", [1, 24, 720])
 @pytest.mark.parametrize("scale,ksize,vsize", [(0.0, 1, 1), (-0.3, 1, 1), (1.0, 8, 1), (0.1, 1e-5, 1e-4), (0.05, 300, 3e4)])
 def test_scales_and_magnitudes(T, scale, ksize, vsize):
     """Uniform weights (scale 0), negative scales, one key taking all the weight
@@ -266,23 +281,24 @@ def test_scales_and_magnitudes(T, scale, ksize, vsize):
     _check(got, q.double().cpu().numpy(), ks, vs, scale, "f32")
 
 
-def test_rows_of_q_do_not_mix():
+@pytest.mark.parametrize("T,lens", [(3, [150, 70]), (704, [1500, 690])])
+def test_rows_of_q_do_not_mix(T, lens):
     """A NaN or an infinity in one head's q leaves every other head's output as it was."""
     from joule_b200 import kv4
     rng = np.random.default_rng(13)
-    B, T, H, kv, hd, lens = 2, 3, 8, 1, 128, [150, 70]
-    cache, ks, vs = _filled(rng, B, 1, kv, hd, 160, 0, lens, [0, 1])
+    B, H, kv, hd = 2, 8, 1, 128
+    cache, ks, vs = _filled(rng, B, 1, kv, hd, 1500, 0, lens, [0, 1])
     q = _to(rng.standard_normal((B, T, H, hd)), "f32")
     want = kv4.kv4_attention(cache, 0, q, _i32([0, 1]), _i32(lens))
-    q[0, 1, 3, 5], q[1, 2, 0, 0] = float("nan"), float("inf")
+    q[0, 1, 3, 5], q[1, T - 1, 0, 0] = float("nan"), float("inf")
     got = kv4.kv4_attention(cache, 0, q, _i32([0, 1]), _i32(lens))
     bad = torch.zeros(B, T, H, dtype=torch.bool, device="cuda")
-    bad[0, 1, 3] = bad[1, 2, 0] = True
+    bad[0, 1, 3] = bad[1, T - 1, 0] = True
     assert torch.equal(got[~bad], want[~bad])
-    assert torch.isnan(got[0, 1, 3]).all() and not torch.isfinite(got[1, 2, 0]).any()
+    assert torch.isnan(got[0, 1, 3]).all() and not torch.isfinite(got[1, T - 1, 0]).any()
 
 
-@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("T", [1, 20, 1000])
 def test_bad_slots_and_lengths_give_zeros_and_a_flag(T):
     from joule_b200 import kv4
     rng = np.random.default_rng(14)
@@ -299,7 +315,7 @@ def test_bad_slots_and_lengths_give_zeros_and_a_flag(T):
     assert status.item() == kv4.KV4_BAD_INDEX and (got[0] == 0).all() and (got[1] != 0).any()
 
 
-@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("T", [1, 40, 650])
 def test_two_sequences_of_one_slot_and_strided_q(T):
     """Entries of a batch may share a slot; q may be a slice of a fused projection or transposed."""
     from joule_b200 import kv4
