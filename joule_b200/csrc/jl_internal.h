@@ -223,7 +223,8 @@ struct jl_kv4_attn_args {
 };
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H);
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);
-// The tcgen05 form for many query rows (jl_kv4_prompt.cu), a block per 256 of them;
-// no workspace.
-long long jl_kv4_prompt_blocks(const jl::kv4_dims& c, const jl_kv4_attn_args& a);
-int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);
+// The tcgen05 form for many query rows (jl_kv4_prompt.cu): a block per unit of 256 rows
+// of one kv head and per split of its cache blocks; S > 1 splits need a workspace.
+long long jl_kv4_prompt_units(const jl::kv4_dims& c, int B, int T, int H);
+long long jl_kv4_prompt_ws_bytes(const jl::kv4_dims& c, long long units, int S);
+int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, int S, cudaStream_t s);

@@ -97,14 +97,16 @@ struct kv4_split {
 
 // The cut of U units over at most `blocks` blocks of NW warps: ctas blocks take
 // a share each and nw of a block's warps share that alike, in order (few units
-// spread over all blocks first). U >= 1.
+// spread over all blocks first; a block of fewer units than nw leaves warps idle).
+// U >= 1.
 struct kv4_cut {
     uint32_t ctas, nw;
     kv4_split by_block;
     __device__ kv4_cut(uint32_t U, uint32_t blocks, uint32_t NW)
-        : ctas(min(blocks, U)), nw(min(NW, U / min(blocks, U))), by_block(U, min(blocks, U)) {}
+        : ctas(min(blocks, U)), nw(min(NW, (U - 1) / min(blocks, U) + 1)), by_block(U, min(blocks, U)) {}
     __device__ uint32_t start(uint32_t c) const { return by_block.start(c); }
-    __device__ kv4_split by_warp(uint32_t c) const { return kv4_split(start(c + 1) - start(c), nw); }
+    __device__ uint32_t warps(uint32_t c) const { return min(nw, start(c + 1) - start(c)); }  // that have units
+    __device__ kv4_split by_warp(uint32_t c) const { return kv4_split(start(c + 1) - start(c), warps(c)); }
     __device__ uint32_t warp_of(uint32_t u) const {  // nw * block + warp
         const uint32_t c = by_block.of(u);
         return c * nw + by_warp(c).of(u - start(c));
@@ -430,7 +432,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     const uint32_t U = warp_total(seqs, a.B) * S;
     if (U == 0) return;
     const kv4_cut cut(U, gridDim.x, NW);
-    if (warp >= cut.nw || blockIdx.x >= cut.ctas) return;
+    if (blockIdx.x >= cut.ctas) return;
+    const int used = cut.warps(blockIdx.x);
+    if (warp >= used) return;
     const int wid = blockIdx.x * cut.nw + warp;
     const kv4_split mine = cut.by_warp(blockIdx.x);
     const uint32_t c0 = cut.start(blockIdx.x), c1 = cut.start(blockIdx.x + 1), u0 = c0 + mine.start(warp);
@@ -563,18 +567,18 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         if (i + 1 < units) advance(co);
     }
     if (!joined) return;
-    // all cut.nw warps of the block come here: the warps' sums, in their order
-    asm volatile("bar.sync 1, %0;" ::"r"(cut.nw * 32) : "memory");
+    // all used warps of the block come here: the warps' sums, in their order
+    asm volatile("bar.sync 1, %0;" ::"r"(used * 32) : "memory");
     const float* ml = reinterpret_cast<const float*>(smem + SM::stat);
     float* part = static_cast<float*>(a.ws) +
                   ((size_t)blockIdx.x * cut.nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
-    for (int x = threadIdx.x; x < kKvTile * HD / 4; x += cut.nw * 32) {
+    for (int x = threadIdx.x; x < kKvTile * HD / 4; x += used * 32) {
         const int r = x / (HD / 4);
         float m = -INFINITY, lsum = 0.0f;
-        for (int w = 0; w < (int)cut.nw; w++) m = fmaxf(m, ml[w * 2 * kKvTile + r]);
+        for (int w = 0; w < used; w++) m = fmaxf(m, ml[w * 2 * kKvTile + r]);
         const float mu = m == -INFINITY ? 0.0f : m;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int w = 0; w < (int)cut.nw; w++) {
+        for (int w = 0; w < used; w++) {
             const float f = ex2(ml[w * 2 * kKvTile + r] - mu);
             const float4 v = reinterpret_cast<const float4*>(smem + w * kKvRing * UNIT)[x];
             lsum = fmaf(ml[w * 2 * kKvTile + kKvTile + r], f, lsum);
@@ -622,8 +626,9 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
     int b0 = w0 / nw, b1 = w1 / nw + 1;  // joined blocks [b0, b1)
     if (cut.start(b0) < first) b0++;
     if (cut.start(b1) > last) b1--;
-    if (nw == 1 || b1 <= b0) b0 = b1 = w1 / nw + 1;
-    const int head = min(w1 + 1, b0 * nw) - w0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
+    if (nw == 1) b0 = b1 = w1 + 1;  // (a unit per block)
+    else if (b1 <= b0) b0 = b1 = max(w0 / nw + 1, w1 / nw);
+    const int c0 = w0 / nw, head = nw == 1 ? w1 + 1 - w0 : b0 > c0 ? min(w1 + 1, c0 * nw + (int)cut.warps(c0)) - w0 : 0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
     const int g = blockIdx.y * RB + warp % RB, lanes = 8 / RB, pl = warp / RB;
     const float* ws = static_cast<const float*>(a.ws) + g * HD;
     // warp w0 began the segment: its part 1
@@ -745,13 +750,23 @@ int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStrea
     return launch_t<HD, __nv_bfloat16>(c, l, a, s);
 }
 
+// Splits of each unit of a call in the tcgen05 form: as many as fill the SMs, of at
+// least kMinSplit cache blocks each. Calls of at most 256 positions have no workspace.
+constexpr int kMinSplit = 2;
+int splits_of(long long units, int longest, int sms) {
+    if (longest <= 256 || units >= sms) return 1;
+    return std::max(1, (int)std::min<long long>(sms / units, (longest + jl::kKv4Rows - 1) / jl::kKv4Rows / kMinSplit));
+}
+
 }  // namespace
 
-// Two parts for each warp that has blocks.
+// Two parts for each warp that has blocks, or the splits of the tcgen05 form.
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
     const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kKvWarps;
-    const long long n = segs >= warps ? warps : std::min(warps, segs * c.nb);
-    return n * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float);
+    const long long n = segs >= warps ? warps : std::min(warps, 2 * segs * c.nb);  // blocks x warps of a cut: below units + blocks
+    const long long units = jl_kv4_prompt_units(c, B, T, H);
+    return std::max(n * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float),
+                    jl_kv4_prompt_ws_bytes(c, units, splits_of(units, c.nb * jl::kKv4Rows, kMaxSms)));
 }
 
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
@@ -760,8 +775,12 @@ int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, 
     // 32/4 heads of 128 over 2,048: 64 tokens of 4 sequences, 8,192 rows: 79 us here
     // against 99 there; 128 tokens, 16,384 rows: 147 against 99; 0.75 to 0.88 and 1.3 to
     // 1.7 over head dims, types and lengths).
-    const long long rows = (long long)a.B * a.T * a.H, blocks = jl_kv4_prompt_blocks(c, a);
-    if (rows >= 76 * std::max<long long>(sm_count(), blocks)) return jl_launch_kv4_prompt(c, l, a, s);
+    const int sms = std::min(sm_count(), kMaxSms);
+    if (sms < 1) return JL_ERR_CUDA;
+    const long long rows = (long long)a.B * a.T * a.H, units = jl_kv4_prompt_units(c, a.B, a.T, a.H);
+    const int S = splits_of(units, a.longest, sms);
+    if (rows >= 76 * units && rows * ((a.longest + jl::kKv4Rows - 1) / jl::kKv4Rows) >= 1 << 15)
+        return jl_launch_kv4_prompt(c, l, a, S, s);
     const int rc = jl_device_once(kOnceKv4, [] {
         const int r = attn_attrs<64>();
         return r ? r : attn_attrs<128>();

@@ -73,6 +73,15 @@ struct pr_held {
     }
 };
 
+// A split's sums in the workspace: [32 rows' group][pieces of a row][32 rows][4 values],
+// then (reference, sum of weights) of each row.
+template <int HD>
+struct pr_part {
+    static constexpr int floats = kPrPair * HD + 2 * kPrPair;
+    __device__ static float* of(void* ws, size_t i) { return static_cast<float*>(ws) + i * floats; }
+    __device__ static float2* stats(float* part) { return reinterpret_cast<float2*>(part + kPrPair * HD); }
+};
+
 template <int HD, bool LO>
 struct pr_smem {
     static constexpr int NG = HD / 64, PARTS = LO ? 2 : 1;
@@ -84,7 +93,7 @@ struct pr_smem {
     static constexpr int v = k + 2 * KTILE;              // [buffer][group][8 positions' chunk][8 values' core]
     static constexpr int raw = v + 2 * VTILE;
     static constexpr int held = raw + 2 * kv4_block_bytes(HD);
-    static constexpr int total = held + (LO ? (int)sizeof(pr_held) : 0);
+    static constexpr int total = held + (int)sizeof(pr_held);
     static constexpr int SCOLS = NG * 64, TCOLS = 2 * SCOLS;  // TMEM columns of a tile: S (then P), O
     static_assert(sizeof(pr_bars) <= 512 && total <= 227 * 1024, "shared memory");
 };
@@ -175,6 +184,17 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
 #pragma unroll
     for (int j = 0; j < 8; j++) y[j] = x[j];
     put8(p, y);
+}
+
+// Four values.
+__device__ __forceinline__ void put4(float* p, const float* x) { store_piece(p, x); }
+__device__ __forceinline__ void put4(__half* p, const float* x) {
+    const __half2 u = __floats2half2_rn(x[0], x[1]), v = __floats2half2_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+}
+__device__ __forceinline__ void put4(__nv_bfloat16* p, const float* x) {
+    const __nv_bfloat162 u = __floats2bfloat162_rn(x[0], x[1]), v = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
 }
 
 // Unpacks one cache block (kPrUnpack warps, tid from 0) into operand tiles and fp32
@@ -306,7 +326,7 @@ __device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l, jl_kv4_attn_args a, int pairs) {
+__global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l, jl_kv4_attn_args a, int pairs, int S) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr bool LO = sizeof(T) == 4;
     using SM = pr_smem<HD, LO>;
@@ -314,15 +334,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     pr_bars& sh = *reinterpret_cast<pr_bars*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     griddep_wait();
-    griddep_launch_dependents();
     // blocks in the order of falling work: the last rows of a prompt see the most
-    const int per = c.KH * a.B, pair = pairs - 1 - (int)blockIdx.x / per, kh = blockIdx.x % c.KH, b = blockIdx.x % per / c.KH;
+    const int per = c.KH * a.B, unit = blockIdx.x / S, split = blockIdx.x % S;
+    const int pair = pairs - 1 - unit / per, kh = unit % c.KH, b = unit % per / c.KH;
     const int gsz = a.H / c.KH, rows = a.T * gsz, row0 = pair * kPrPair;
     const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, 0};
     const int len = seqs.len(b);
-    if (len < 0 && threadIdx.x == 0 && pair == 0 && kh == 0 && a.err) atomicOr(a.err, kErrKvIndex);
+    if (len < 0 && threadIdx.x == 0 && pair == 0 && kh == 0 && split == 0 && a.err) atomicOr(a.err, kErrKvIndex);
     auto sees = [&](int r) { return max(0, len - a.T + 1 + min(r, rows - 1) / gsz); };  // positions that row r sees
-    const int nb = (sees(row0 + kPrPair - 1) + kKv4Rows - 1) / kKv4Rows, tiles = rows - row0 > kPrTile ? 2 : 1;
+    const int all = (sees(row0 + kPrPair - 1) + kKv4Rows - 1) / kKv4Rows;  // the pair's cache blocks, this split's: [jb, jb + nb)
+    const int jb = (int)((long long)all * split / S), nb = (int)((long long)all * (split + 1) / S) - jb, off = jb * kKv4Rows;
+    const int tiles = rows - row0 > kPrTile ? 2 : 1;
     // softmax threads: the row's place in q and out (rows past the last repeat it and are not written)
     const int row = row0 + (int)threadIdx.x, rc = min(row, rows - 1), tok = rc / gsz, h = kh * gsz + rc % gsz;
     const long long orow = (long long)b * a.T + tok;
@@ -332,16 +354,22 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
 #pragma unroll
             for (int j = 0; j < 8; j++) a.outT[(size_t)(h * HD + d + j) * a.outT_ld + orow] = x[j];
     };
+    if (nb == 0 && S > 1) {
+        if (warp < 8) pr_part<HD>::stats(pr_part<HD>::of(a.ws, blockIdx.x))[threadIdx.x] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
     if (nb == 0) {  // nothing to see for any row
         const float z[8] = {};
         if (warp < 8 && row < rows)
             for (int d = 0; d < HD; d += 8) write(d, z);
         return;
     }
-    pr_held* held = reinterpret_cast<pr_held*>(smem + SM::held);  // fp32 calls
+    pr_held* held = reinterpret_cast<pr_held*>(smem + SM::held);
     if (threadIdx.x == 0) {
         sh.abort = 0;
-        if (LO) {
+        if (S > 1) {
+            held->out = pr_part<HD>::of(a.ws, blockIdx.x), held->H = held->gsz = 1, held->row0 = 0, held->rows = kPrPair;
+        } else if (LO) {
             held->out = static_cast<float*>(a.out) + ((long long)b * a.T * a.H + kh * gsz) * HD;
             held->H = a.H, held->gsz = gsz, held->row0 = row0, held->rows = rows;
         }
@@ -384,7 +412,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             fence_proxy_async_smem();  // before the tensor cores read it
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full);
-            const int n_row = sees(row), n_min = sees(row0 + t * kPrTile);
+            const int n_row = sees(row) - off, n_min = sees(row0 + t * kPrTile) - off;
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * SM::TCOLS, to = ts + SM::SCOLS;
             float ref = -INFINITY;
             float2 lsum = f2(0.0f);
@@ -491,8 +519,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             }
             if (j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
                 tc_fence_after();
+                const float ls = lsum.x + lsum.y;
+                griddep_launch_dependents();  // not before: the next kernel's blocks, the merge's, would poll beside this one's
+                if (S > 1) {
+                    pr_fold<HD>(to, ref, held, LO && nb > kPrFold);
+                    pr_part<HD>::stats(held->out)[threadIdx.x] = make_float2(ref, ls);
+                } else {
                 if (LO && nb > kPrFold) pr_unfold<HD>(to, ref, held);
-                const float ls = lsum.x + lsum.y, inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
                 // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
                 constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
                 T* st = reinterpret_cast<T*>(qs) + (warp & 3) * 32 * HD;
@@ -520,12 +554,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (to_row * a.H + kh * gsz + g % gsz) * HD + p * VPC) =
                         *reinterpret_cast<const uint4*>(st + (r * CPR + (p ^ (r & 7))) * VPC);
                 }
+                }
             }
         }
     } else if (warp < 8 + kPrUnpack) {
         // ---------------- unpack, and the copies of the cache's blocks
         const int tid = threadIdx.x - 256, w = warp - 8;
-        const uint8_t* src = c.run(a.slots[b], l, kh);
+        const uint8_t* src = c.run(a.slots[b], l, kh) + (size_t)jb * BLK;
         uint8_t* raw = smem + SM::raw;
         auto issue = [&](int j) {
             mbar_expect_tx(&sh.raw_full[j & 1], BLK);
@@ -540,7 +575,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             if (!pr_wait(&sh.raw_full[s], j >> 1 & 1, a.err, abort)) break;
             if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, a.err, abort)) break;
             pr_unpack<HD>(raw + s * BLK, smem + SM::k + s * SM::KTILE, smem + SM::v + s * SM::VTILE,
-                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], len - j * kKv4Rows, tid);
+                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], len - off - j * kKv4Rows, tid);
             fence_proxy_async_smem();  // the operands to the tensor cores, the reads before the next copy
             __syncwarp();
             if (lane == 0) {
@@ -624,17 +659,81 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * SM::TCOLS));
 }
 
+// Adds the splits of 32 rows up: warp w takes splits w, w + 8, ..., lane = row, 32
+// values of each (blockIdx.y).
+template <int HD, typename T>
+__global__ void __launch_bounds__(256) k_kv4_prompt_merge(kv4_dims c, jl_kv4_attn_args a, int pairs, int S) {
+    __shared__ float4 sums[8][8][32];
+    __shared__ float2 stats[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = c.KH * a.B, unit = blockIdx.x / 8, grp = blockIdx.x % 8;
+    const int pair = pairs - 1 - unit / per, kh = unit % c.KH, b = unit % per / c.KH;
+    const int gsz = a.H / c.KH, rows = a.T * gsz, row = pair * kPrPair + grp * 32 + lane;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (row - lane >= rows) return;
+    float m = -INFINITY, ls = 0.0f;
+    float4 x[8] = {};
+    for (int s = warp; s < S; s += 8) {
+        float* p = pr_part<HD>::of(a.ws, (size_t)unit * S + s);
+        const float4* y = reinterpret_cast<const float4*>(p) + (grp * (HD / 4) + blockIdx.y * 8) * 32 + lane;
+        const float2 st = pr_part<HD>::stats(p)[grp * 32 + lane];
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = y[i * 32];
+        if (st.y == 0.0f) continue;  // (a split of no blocks wrote no sums)
+        const float nm = fmaxf(m, st.x), al = ex2(m - nm), f = ex2(st.x - nm);
+        m = nm;
+        ls = fmaf(ls, al, st.y * f);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = make_float4(fmaf(x[i].x, al, v[i].x * f), fmaf(x[i].y, al, v[i].y * f), fmaf(x[i].z, al, v[i].z * f),
+                               fmaf(x[i].w, al, v[i].w * f));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) sums[warp][i][lane] = x[i];
+    stats[warp][lane] = make_float2(m, ls);
+    __syncthreads();
+    // warp w: piece w of the 32 values
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 8; w++) m = fmaxf(m, stats[w][lane].x);
+    m = m == -INFINITY ? 0.0f : m;
+    ls = 0.0f;
+    float o[4] = {};
+#pragma unroll
+    for (int w = 0; w < 8; w++) {
+        const float2 st = stats[w][lane];
+        const float f = ex2(st.x - m);
+        const float4 v = sums[w][warp][lane];
+        ls = fmaf(st.y, f, ls);
+        o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+    }
+    if (row >= rows) return;
+    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+    const int h = kh * gsz + row % gsz, d = blockIdx.y * 32 + warp * 4;
+    const long long orow = (long long)b * a.T + row / gsz;
+    T* to = static_cast<T*>(a.out) + (orow * a.H + h) * HD + d;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] *= inv;
+    put4(to, o);
+    if (a.outT)
+#pragma unroll
+        for (int i = 0; i < 4; i++) a.outT[(size_t)(h * HD + d + i) * a.outT_ld + orow] = o[i];
+}
+
 }  // namespace jl
 
 namespace {
 
 template <int HD, typename T>
-int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, int S, cudaStream_t s) {
     using namespace jl;
-    const long long blocks = jl_kv4_prompt_blocks(c, a), pairs = blocks / ((long long)c.KH * a.B);
-    if (blocks > INT_MAX) return JL_ERR_INVALID;
-    return launch(k_kv4_prompt<HD, T>, dim3((unsigned)blocks), dim3(kPrThreads), (size_t)pr_smem<HD, sizeof(T) == 4>::total, s,
-                  c, l, a, (int)pairs);
+    const long long units = jl_kv4_prompt_units(c, a.B, a.T, a.H), pairs = units / ((long long)c.KH * a.B);
+    if (units > INT_MAX / 8) return JL_ERR_INVALID;
+    const int rc = launch(k_kv4_prompt<HD, T>, dim3((unsigned)units * S), dim3(kPrThreads),
+                          (size_t)pr_smem<HD, sizeof(T) == 4>::total, s, c, l, a, (int)pairs, S);
+    if (rc || S == 1) return rc;
+    return launch(k_kv4_prompt_merge<HD, T>, dim3((unsigned)units * 8, HD / 32), dim3(256), 0, s, c, a, (int)pairs, S);
 }
 
 template <int HD>
@@ -651,17 +750,21 @@ int prompt_attrs() {
 
 }  // namespace
 
-long long jl_kv4_prompt_blocks(const jl::kv4_dims& c, const jl_kv4_attn_args& a) {
-    return ((long long)a.T * (a.H / c.KH) + jl::kPrPair - 1) / jl::kPrPair * c.KH * a.B;
+long long jl_kv4_prompt_units(const jl::kv4_dims& c, int B, int T, int H) {
+    return ((long long)T * (H / c.KH) + jl::kPrPair - 1) / jl::kPrPair * c.KH * B;
 }
 
-int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+long long jl_kv4_prompt_ws_bytes(const jl::kv4_dims& c, long long units, int S) {
+    return S > 1 ? units * S * (c.hd == 64 ? jl::pr_part<64>::floats : jl::pr_part<128>::floats) * (long long)sizeof(float) : 0;
+}
+
+int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, int S, cudaStream_t s) {
     const int rc = jl_device_once(kOnceKv4Prompt, [] {
         const int r = prompt_attrs<64>();
         return r ? r : prompt_attrs<128>();
     });
     if (rc) return rc;
-    if (a.dtype == JL_F32) return c.hd == 64 ? launch_t<64, float>(c, l, a, s) : launch_t<128, float>(c, l, a, s);
-    if (a.dtype == JL_F16) return c.hd == 64 ? launch_t<64, __half>(c, l, a, s) : launch_t<128, __half>(c, l, a, s);
-    return c.hd == 64 ? launch_t<64, __nv_bfloat16>(c, l, a, s) : launch_t<128, __nv_bfloat16>(c, l, a, s);
+    if (a.dtype == JL_F32) return c.hd == 64 ? launch_t<64, float>(c, l, a, S, s) : launch_t<128, float>(c, l, a, S, s);
+    if (a.dtype == JL_F16) return c.hd == 64 ? launch_t<64, __half>(c, l, a, S, s) : launch_t<128, __half>(c, l, a, S, s);
+    return c.hd == 64 ? launch_t<64, __nv_bfloat16>(c, l, a, S, s) : launch_t<128, __nv_bfloat16>(c, l, a, S, s);
 }
