@@ -592,10 +592,14 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     }
 }
 
-// Adds up the parts of segments that several warps shared: block = RB rows of
-// one segment, 8 / RB warps per row, each adding every (8 / RB)-th part.
-template <int HD, typename T>
-__global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int ctas, int RB) {
+// Adds up the parts of segments that several warps shared: block = RB rows of a run
+// of segments, 8 / RB warps per row, each adding every (8 / RB)-th part.
+// RUN: `per` segments a block, where a block each (2 us of latency, four to an SM)
+// took longer than the sums: 256 sequences of 16/16 heads over 512, 105 us against 97.
+// 
+template <int HD, typename T, bool RUN>
+__global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int ctas, int RB,
+                                                   int per) {
     constexpr int V = HD / 32, NW = kKvWarps, PF = kv4_part_floats(HD);  // V values per lane
     __shared__ float sums[8][HD], stat[8][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -603,7 +607,8 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
     const kv4_seqs seqs = {a.slots, a.lens, a.len_add, a.longest, c.slots, 0};
     // The attention's blocks have all passed their own wait when this kernel
     // starts, so lens and slots are there before this kernel's wait.
-    const int b = blockIdx.x / S, s = blockIdx.x % S, nu = seqs.units(b);
+    const int i0 = RUN ? blockIdx.x * per : blockIdx.x, i1 = RUN ? min(i0 + per, a.B * S) : i0 + 1;
+    int b = i0 / S, s = i0 % S, nu = seqs.units(b);
     uint32_t before = 0, U = 0;
     for (int i = lane; i < a.B; i += 32) {
         const int n = seqs.units(i);
@@ -616,88 +621,99 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const kv4_cut cut(max(1u, U * S), ctas, NW);
-    const uint32_t first = before * S + s * nu, last = first + nu;
-    const int w0 = nu ? cut.warp_of(first) : 0, w1 = nu ? cut.warp_of(last - 1) : 0, nw = cut.nw;
-    griddep_wait();
-    griddep_launch_dependents();
-    if (w0 == w1) return;  // nothing to add, or one warp had it all
-    // Parts: one per warp of the first and last block where these reach out of
-    // the segment, one per block in between.
-    int b0 = w0 / nw, b1 = w1 / nw + 1;  // joined blocks [b0, b1)
-    if (cut.start(b0) < first) b0++;
-    if (cut.start(b1) > last) b1--;
-    if (nw == 1) b0 = b1 = w1 + 1;  // (a unit per block)
-    else if (b1 <= b0) b0 = b1 = max(w0 / nw + 1, w1 / nw);
-    const int c0 = w0 / nw, head = nw == 1 ? w1 + 1 - w0 : b0 > c0 ? min(w1 + 1, c0 * nw + (int)cut.warps(c0)) - w0 : 0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
-    const int g = blockIdx.y * RB + warp % RB, lanes = 8 / RB, pl = warp / RB;
-    const float* ws = static_cast<const float*>(a.ws) + g * HD;
-    // warp w0 began the segment: its part 1
-    auto part = [&](int i) {
-        const int w = i < head ? w0 + i : i < head + b1 - b0 ? (b0 + i - head) * nw : b1 * nw + i - head - (b1 - b0);
-        return ws + ((size_t)w * 2 + (w == w0)) * PF;
-    };
-    const int so = kKvTile * HD + g - g * HD;  // m from the row's values; l is kKvTile further
-    float m = -INFINITY, lsum = 0.0f, x[V] = {};
-    for (int i0 = pl; i0 < n; i0 += 4 * lanes) {
-        float v[4][V], pm[4], pl4[4], mx = m;
+    auto merge = [&]() {
+        const uint32_t first = before * S + s * nu, last = first + nu;
+        const int w0 = nu ? cut.warp_of(first) : 0, w1 = nu ? cut.warp_of(last - 1) : 0, nw = cut.nw;
+        griddep_wait();  // (the cut before it)
+        griddep_launch_dependents();
+        if (w0 == w1) return;  // nothing to add, or one warp had it all
+        // Parts: one per warp of the first and last block where these reach out of
+        // the segment, one per block in between.
+        int b0 = w0 / nw, b1 = w1 / nw + 1;  // joined blocks [b0, b1)
+        if (cut.start(b0) < first) b0++;
+        if (cut.start(b1) > last) b1--;
+        if (nw == 1) b0 = b1 = w1 + 1;  // (a unit per block)
+        else if (b1 <= b0) b0 = b1 = max(w0 / nw + 1, w1 / nw);
+        const int c0 = w0 / nw, head = nw == 1 ? w1 + 1 - w0 : b0 > c0 ? min(w1 + 1, c0 * nw + (int)cut.warps(c0)) - w0 : 0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
+        const int g = blockIdx.y * RB + warp % RB, lanes = 8 / RB, pl = warp / RB;
+        const float* ws = static_cast<const float*>(a.ws) + g * HD;
+        // warp w0 began the segment: its part 1
+        auto part = [&](int i) {
+            const int w = i < head ? w0 + i : i < head + b1 - b0 ? (b0 + i - head) * nw : b1 * nw + i - head - (b1 - b0);
+            return ws + ((size_t)w * 2 + (w == w0)) * PF;
+        };
+        const int so = kKvTile * HD + g - g * HD;  // m from the row's values; l is kKvTile further
+        float m = -INFINITY, lsum = 0.0f, x[V] = {};
+        for (int i0 = pl; i0 < n; i0 += 4 * lanes) {
+            float v[4][V], pm[4], pl4[4], mx = m;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int i = i0 + k * lanes;
-            pm[k] = -INFINITY, pl4[k] = 0.0f;
+            for (int k = 0; k < 4; k++) {
+                const int i = i0 + k * lanes;
+                pm[k] = -INFINITY, pl4[k] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < V; e++) v[k][e] = 0.0f;
-            if (i < n) {
-                const float* p = part(i);
-                pm[k] = p[so];
-                pl4[k] = p[so + kKvTile];
+                for (int e = 0; e < V; e++) v[k][e] = 0.0f;
+                if (i < n) {
+                    const float* p = part(i);
+                    pm[k] = p[so];
+                    pl4[k] = p[so + kKvTile];
 #pragma unroll
-                for (int e = 0; e < V; e++) v[k][e] = p[lane + 32 * e];
+                    for (int e = 0; e < V; e++) v[k][e] = p[lane + 32 * e];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) mx = fmaxf(mx, pm[k]);
+            const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
+            lsum *= al;
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] *= al;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = ex2(pm[k] - mu);
+                lsum = fmaf(pl4[k], f, lsum);
+#pragma unroll
+                for (int e = 0; e < V; e++) x[e] = fmaf(v[k][e], f, x[e]);
+            }
+            m = mx;
+        }
+        if (lanes > 1) {
+#pragma unroll
+            for (int e = 0; e < V; e++) sums[warp][lane + 32 * e] = x[e];
+            if (lane == 0) stat[warp][0] = m, stat[warp][1] = lsum;
+            __syncthreads();
+            if (pl) return;
+            float mx = m;
+            for (int w = 1; w < lanes; w++) mx = fmaxf(mx, stat[warp + w * RB][0]);
+            const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
+            lsum *= al;
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] *= al;
+            for (int w = 1; w < lanes; w++) {
+                const float f = ex2(stat[warp + w * RB][0] - mu);
+                lsum = fmaf(stat[warp + w * RB][1], f, lsum);
+#pragma unroll
+                for (int e = 0; e < V; e++) x[e] = fmaf(sums[warp + w * RB][lane + 32 * e], f, x[e]);
             }
         }
+        const int row = s % R * kKvTile + g;
+        if (row >= rows) return;
+        const int h = s / R * gsz + row % gsz;
+        const long long orow = (long long)b * a.T + row / gsz;
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
 #pragma unroll
-        for (int k = 0; k < 4; k++) mx = fmaxf(mx, pm[k]);
-        const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
-        lsum *= al;
-#pragma unroll
-        for (int e = 0; e < V; e++) x[e] *= al;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float f = ex2(pm[k] - mu);
-            lsum = fmaf(pl4[k], f, lsum);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[e] = fmaf(v[k][e], f, x[e]);
+        for (int e = 0; e < V; e++) {
+            const int d = lane + 32 * e;
+            put1(static_cast<T*>(a.out) + (orow * a.H + h) * HD + d, x[e] * inv);
+            if (a.outT) a.outT[(size_t)(h * HD + d) * a.outT_ld + orow] = x[e] * inv;
         }
-        m = mx;
-    }
-    if (lanes > 1) {
-#pragma unroll
-        for (int e = 0; e < V; e++) sums[warp][lane + 32 * e] = x[e];
-        if (lane == 0) stat[warp][0] = m, stat[warp][1] = lsum;
-        __syncthreads();
-        if (pl) return;
-        float mx = m;
-        for (int w = 1; w < lanes; w++) mx = fmaxf(mx, stat[warp + w * RB][0]);
-        const float mu = mx == -INFINITY ? 0.0f : mx, al = ex2(m - mu);
-        lsum *= al;
-#pragma unroll
-        for (int e = 0; e < V; e++) x[e] *= al;
-        for (int w = 1; w < lanes; w++) {
-            const float f = ex2(stat[warp + w * RB][0] - mu);
-            lsum = fmaf(stat[warp + w * RB][1], f, lsum);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[e] = fmaf(sums[warp + w * RB][lane + 32 * e], f, x[e]);
+    };
+    merge();
+    for (int i = i0 + 1; RUN && i < i1; i++) {  // (RB = 8: no barrier inside)
+        if (++s == S) {
+            s = 0;
+            before += nu;
+            nu = seqs.units(++b);
         }
-    }
-    const int row = s % R * kKvTile + g;
-    if (row >= rows) return;
-    const int h = s / R * gsz + row % gsz;
-    const long long orow = (long long)b * a.T + row / gsz;
-    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-        const int d = lane + 32 * e;
-        put1(static_cast<T*>(a.out) + (orow * a.H + h) * HD + d, x[e] * inv);
-        if (a.outT) a.outT[(size_t)(h * HD + d) * a.outT_ld + orow] = x[e] * inv;
+        merge();
     }
 }
 
@@ -740,7 +756,10 @@ int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream
                           whole);
     if (rc || whole) return rc;
     const int RB = segs >= sms ? 8 : segs * 4 >= sms ? 2 : 1;
-    return launch(k_kv4_merge<HD, T>, dim3((unsigned)segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB);
+    const int per = (int)((segs - 1) / (4 * sms) + 1);
+    if (per == 1)
+        return launch(k_kv4_merge<HD, T, false>, dim3((unsigned)segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB, 1);
+    return launch(k_kv4_merge<HD, T, true>, dim3((unsigned)((segs - 1) / per + 1)), dim3(256), 0, s, c, a, R, sms, 8, per);
 }
 
 template <int HD>
