@@ -553,7 +553,9 @@ int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* positions, 
  * that sees nothing is 0. T = 1 is a decode step, T > 1 a piece of a prompt.
  * `longest` is a bound that the caller knows of the lens (0: maxT); a length
  * outside [0, longest] or a slot outside the cache gives zeros and the status
- * bit. ws: jl_kv4_attn_ws(c, B, T, H) bytes of device memory, 16-byte aligned,
+ * bit (and a wait inside the call that ran out sets bit 1, with out undefined).
+ * out does not overlap q's rows or what lies between them, nor the other buffers.
+ * ws: jl_kv4_attn_ws(c, B, T, H) bytes of device memory, 16-byte aligned,
  * used by this call alone until it has run (calls that can run at the same
  * time, captured graphs among them, need one each); none where longest is 1 to
  * 256. B = 0 does nothing. The result does not depend on what else runs: no

@@ -272,6 +272,10 @@ extern "C" int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, lon
     if (!q || !slots || !lens || !out || !aligned16(q) || !aligned16(out) || q_stride % unit ||
         ((long long)B * T > 1 && q_stride < row))
         return JL_ERR_INVALID;
+    // out takes intermediate sums in some forms, and rows of q are read more than once
+    const long long n = (long long)B * T, esize = dtype == JL_F32 ? 4 : 2;
+    const char *q0 = static_cast<const char*>(q), *o0 = static_cast<const char*>(out);
+    if (q0 < o0 + n * row * esize && o0 < q0 + ((n > 1 ? (n - 1) * q_stride : 0) + row) * esize) return JL_ERR_INVALID;
     const long long need = longest && longest <= 256 ? 0 : jl_kv4_attn_ws_bytes(d, B, T, H);
     if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need)) return JL_ERR_INVALID;
     jl_kv4_attn_args a;

@@ -748,7 +748,7 @@ int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream
     const int sms = std::min(sm_count(), kMaxSms), R = row_tiles(c, a.T, a.H);
     if (sms < 1) return JL_ERR_CUDA;
     const long long segs = (long long)a.B * R * c.KH;
-    if (segs > INT_MAX || segs * c.nb > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
+    if (segs > INT_MAX || segs * ((a.longest + kKv4Rows - 1) / kKv4Rows) > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
     // Segments of at most 256 positions are not cut (and need no workspace): a warp
     // takes that many sooner than a second kernel starts.
     const int whole = a.longest <= 256;

@@ -171,7 +171,8 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     them. H is a multiple of the cache's n_kv. scale: 1 / sqrt(hd) by default.
     longest: a bound of the lens that the caller knows (by default the cache's
     length); a longer entry counts as outside the cache. Rows that see nothing
-    are zero. Returns out, of q's shape and type."""
+    are zero. Returns out, of q's shape and type; one that is given does not
+    overlap q (JouleError)."""
     c, dev = _view(cache, l)
     shape = q.shape
     hd, H = c.hd, shape[-2] if len(shape) >= 3 else 0

@@ -72,7 +72,7 @@ def test_bad_caches_are_refused(dll, kw, l):
     r = ctypes.byref(c)
     assert dll.jl_kv4_append(r, l, 4096, 4096, 0, 256, 256, 4096, 4096, 1, None, None) == -1
     assert dll.jl_kv4_read(r, l, 4096, 4096, 1, 4096, 4096, 0, None, None) == -1
-    assert dll.jl_kv4_attn(r, l, 4096, 0, 512, 4096, 4096, 0, 1, 1, 4, 1.0, 4096, 4096, 1 << 40, None, None) == -1
+    assert dll.jl_kv4_attn(r, l, 4096, 0, 512, 4096, 4096, 0, 1, 1, 4, 1.0, 1 << 20, 4096, 1 << 40, None, None) == -1
 
 
 def test_bad_arguments_are_refused(dll):
@@ -87,12 +87,13 @@ def test_bad_arguments_are_refused(dll):
     assert rd(n=0) == 0
     assert all(x == -1 for x in (rd(n=-1), rd(t=3), rd(s=None), rd(p=None), rd(k=None), rd(v=4100)))
 
-    def at(q=4096, t=0, qs=512, s=4096, n=4096, longest=0, B=2, T=1, H=4, scale=1.0, out=4096, ws=4096, wb=1 << 40):
+    def at(q=4096, t=0, qs=512, s=4096, n=4096, longest=0, B=2, T=1, H=4, scale=1.0, out=1 << 20, ws=4096, wb=1 << 40):
         return dll.jl_kv4_attn(r, 0, q, t, qs, s, n, longest, B, T, H, scale, out, ws, wb, None, None)
     assert at(B=0) == 0
     assert all(x == -1 for x in (at(q=None), at(q=4100), at(t=3), at(qs=511), at(qs=256), at(s=None), at(n=None),
                                  at(longest=-1), at(longest=129), at(B=-1), at(T=0), at(H=3), at(H=0),
-                                 at(scale=float("nan")), at(scale=float("inf")), at(out=None), at(out=4104),
+                                 at(scale=float("nan")), at(scale=float("inf")), at(out=None), at(out=(1 << 20) + 8),
+                                 at(out=4096), at(out=4096 + 2 * 512 * 4 - 16), at(qs=1 << 20, out=1 << 20),
                                  at(B=2**20, T=2**20)))
     assert dll.jl_kv4_attn_ws(r, 2, 1, 3) == -1 and dll.jl_kv4_attn_ws(r, 2, 0, 4) == -1
     need = dll.jl_kv4_attn_ws(r, 2, 1, 4)

@@ -427,6 +427,8 @@ def test_front_end_refusals():
     from joule_b200.native import JouleError
     with pytest.raises(JouleError):
         kv4.kv4_attention(cache, 0, q, i, i, scale=float("nan"))
+    with pytest.raises(JouleError):
+        kv4.kv4_attention(cache, 0, q, i, i, out=q)
     # empty batches do nothing
     e = _i32([])
     kv4.kv4_append(cache, 0, x[:0], x[:0], e, e)
