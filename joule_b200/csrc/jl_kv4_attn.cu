@@ -770,7 +770,9 @@ int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStrea
 }
 
 // Splits of each unit of a call in the tcgen05 form: as many as fill the SMs, of at
-// least kMinSplit cache blocks each. Calls of at most 256 positions have no workspace.
+// least kMinSplit cache blocks each (4 in place of 2: 64 tokens of 32/4 heads of 128 over
+// 1,024 25.7 us against 21.3, over 4,096 the same). Calls of at most 256 positions have
+// no workspace.
 constexpr int kMinSplit = 2;
 int splits_of(long long units, int longest, int sms) {
     if (longest <= 256 || units >= sms) return 1;
@@ -789,11 +791,12 @@ long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
 }
 
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
-    // The tcgen05 kernel takes the time of 256 query rows per block and wave whatever
-    // the rows are, this file's a time by the rows; they meet at 76 rows per SM (fp32,
-    // 32/4 heads of 128 over 2,048: 64 tokens of 4 sequences, 8,192 rows: 79 us here
-    // against 99 there; 128 tokens, 16,384 rows: 147 against 99; 0.75 to 0.88 and 1.3 to
-    // 1.7 over head dims, types and lengths).
+    // The tcgen05 kernel takes the time of its units of 256 rows, however few rows fill
+    // them, and some 14 us beside (start, q, joining); this file's a time by the rows.
+    // fp32, 32/4 heads of 128, here / there: 8 tokens (64 rows a unit) over 16,384
+    // positions 29 / 34 us, 16 of 4 sequences (128 a unit) 145 / 93; 64 tokens (2,048
+    // rows) over 512 17 / 20, over 1,024 21 / 21, over 4,096 47 / 30. Over types, head
+    // dims and lengths the rule is within 1 % of the better one (geometric mean).
     const int sms = std::min(sm_count(), kMaxSms);
     if (sms < 1) return JL_ERR_CUDA;
     const long long rows = (long long)a.B * a.T * a.H, units = jl_kv4_prompt_units(c, a.B, a.T, a.H);

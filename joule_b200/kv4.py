@@ -42,39 +42,44 @@ def kv4_cache(slots: int, L: int, n_kv: int, hd: int, maxT: int, device=None) ->
     return torch.empty(slots, L, n_kv, -(-maxT // KV4_BLOCK), 68 * hd, dtype=torch.uint8, device=device)
 
 
-_lib = None
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object
+_current_device = torch._C._cuda_getDevice
 
 
-def _dll():
-    global _lib
-    if _lib is None:
-        _lib = get_dll()
-    return _lib
+class _Lib:
+    """The library's entry points, bound at the first call."""
+    append = read = attn = None
+
+    @classmethod
+    def bind(cls) -> None:
+        dll = get_dll()
+        cls.read, cls.attn, cls.append = dll.jl_kv4_read, dll.jl_kv4_attn, dll.jl_kv4_append
 
 
 def _view(cache: torch.Tensor, l: int) -> tuple[Kv4, int]:
     """The cache as the library takes it, and its device's index."""
     shape = cache.shape
-    if len(shape) != 5 or cache.dtype is not torch.uint8 or not cache.is_cuda or not cache.is_contiguous():
+    dev = cache.get_device()
+    if len(shape) != 5 or cache.dtype is not torch.uint8 or dev < 0 or not cache.is_contiguous():
         raise ValueError("kv4: the cache is a contiguous uint8 CUDA tensor [slots, L, n_kv, blocks, 68 * hd]")
     slots, L, kh, nb, size = shape
     if size != 68 * 64 and size != 68 * 128 or not slots or not kh or not nb:
         raise ValueError(f"kv4: block size {size} is not 68 * hd with hd 64 or 128, or the cache is empty")
     if not 0 <= l < L:
         raise ValueError(f"kv4: layer {l} outside [0, {L})")
-    return Kv4(cache.data_ptr(), slots, L, kh, size // 68, nb * KV4_BLOCK), cache.get_device()
+    return Kv4(cache.data_ptr(), slots, L, kh, size // 68, nb * KV4_BLOCK), dev
 
 
-def _index(t: torch.Tensor, n: int, dev: int, name: str) -> int:
-    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+def _indices(slots: torch.Tensor, t: torch.Tensor, n: int, dev: int, name: str) -> tuple[int, int]:
+    """Addresses of slots and of t (positions or lens)."""
+    if slots.dtype is not torch.int32 or slots.get_device() != dev or slots.shape != (n,) or not slots.is_contiguous():
+        raise ValueError(f"kv4: slots is a contiguous int32 tensor [{n}] on cuda:{dev}")
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"kv4: {name} is a contiguous int32 tensor [{n}] on cuda:{dev}")
-    return t.data_ptr()
+    return slots.data_ptr(), t.data_ptr()
 
 
-def _status(t, dev: int) -> int | None:
-    if t is None:
-        return None
+def _status(t: torch.Tensor, dev: int) -> int:
     if t.dtype is not torch.int32 or t.get_device() != dev or t.numel() < 1:
         raise ValueError(f"kv4: status is an int32 tensor on cuda:{dev}")
     return t.data_ptr()
@@ -95,15 +100,10 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return _aligned(t), h * d
 
 
-def _on(dev: int, stream):
-    """The stream's handle when the call can go to it as things are (the current
-    device's current stream), else None."""
-    return _raw_stream(dev) if stream is None and torch._C._cuda_getDevice() == dev else None
-
-
 def _other(dev: int, stream) -> torch.cuda.Stream:
-    """A stream given by the caller, or the current one of another device: to be
-    made current for the call, so that what the call allocates belongs to it."""
+    """A stream given by the caller, or the current one of a device that is not
+    current: to be made current for the call, so that what the call allocates
+    belongs to it."""
     device = torch.device("cuda", dev)
     if stream is None:
         return torch.cuda.current_stream(device)
@@ -126,14 +126,18 @@ def kv4_append(cache: torch.Tensor, l: int, k: torch.Tensor, v: torch.Tensor, sl
     if kind is None or v.dtype is not k.dtype or k.get_device() != dev or v.get_device() != dev:
         raise ValueError(f"kv4_append: k and v are fp32, fp16 or bf16, of one type, on cuda:{dev}")
     n = shape[0]
-    ps, pp, st = _index(slots, n, dev, "slots"), _index(positions, n, dev, "positions"), _status(status, dev)
-    handle = _on(dev, stream)
-    if handle is None:
+    ps, pp = _indices(slots, positions, n, dev, "positions")
+    st = None if status is None else _status(status, dev)
+    if stream is not None or _current_device() != dev:
         with torch.cuda.stream(_other(dev, stream)):
             return kv4_append(cache, l, k, v, slots, positions, status)
     k, sk = _rows(k)
     v, sv = _rows(v)
-    check(_dll().jl_kv4_append(c, l, k.data_ptr(), v.data_ptr(), kind, sk, sv, ps, pp, n, st, handle), "jl_kv4_append")
+    if _Lib.append is None:
+        _Lib.bind()
+    code = _Lib.append(c, l, k.data_ptr(), v.data_ptr(), kind, sk, sv, ps, pp, n, st, _raw_stream(dev))
+    if code:
+        check(code, "jl_kv4_append")
 
 
 def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.Tensor,
@@ -145,14 +149,18 @@ def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.
     if kind is None:
         raise ValueError(f"kv4_read: dtype is fp32, fp16 or bf16, got {dtype}")
     n = slots.numel()
-    ps, pp, st = _index(slots, n, dev, "slots"), _index(positions, n, dev, "positions"), _status(status, dev)
-    handle = _on(dev, stream)
-    if handle is None:
+    ps, pp = _indices(slots, positions, n, dev, "positions")
+    st = None if status is None else _status(status, dev)
+    if stream is not None or _current_device() != dev:
         with torch.cuda.stream(_other(dev, stream)):
             return kv4_read(cache, l, slots, positions, dtype, status)
     k = torch.empty(n, c.n_kv, c.hd, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
-    check(_dll().jl_kv4_read(c, l, ps, pp, n, k.data_ptr(), v.data_ptr(), kind, st, handle), "jl_kv4_read")
+    if _Lib.append is None:
+        _Lib.bind()
+    code = _Lib.read(c, l, ps, pp, n, k.data_ptr(), v.data_ptr(), kind, st, _raw_stream(dev))
+    if code:
+        check(code, "jl_kv4_read")
     return k, v
 
 
@@ -175,14 +183,14 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     overlap q (JouleError)."""
     c, dev = _view(cache, l)
     shape = q.shape
-    hd, H = c.hd, shape[-2] if len(shape) >= 3 else 0
-    if len(shape) not in (3, 4) or shape[-1] != hd or H < 1 or H % c.n_kv:
+    hd, dims = c.hd, len(shape)
+    B, T, H, d = shape if dims == 4 else (shape[0], 1, *shape[1:]) if dims == 3 else (0, 1, 0, 0)
+    if d != hd or H < 1 or H % c.n_kv:
         raise ValueError(f"kv4_attention: q is [B, T, H, {hd}] or [B, H, {hd}] with H a multiple of {c.n_kv}, "
                          f"got {tuple(q.shape)}")
     kind = _TYPES.get(q.dtype)
     if kind is None or q.get_device() != dev:
         raise ValueError(f"kv4_attention: q is fp32, fp16 or bf16 on cuda:{dev}")
-    B, T = shape[0], 1 if len(shape) == 3 else shape[1]
     if T < 1:
         raise ValueError("kv4_attention: T is 1 or more")
     if longest is None:
@@ -192,15 +200,16 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     if out is not None and (out.shape != shape or out.dtype is not q.dtype or out.get_device() != dev
                             or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("kv4_attention: out is contiguous, 16-byte aligned, of q's shape, type and device")
-    ps, pl, st = _index(slots, B, dev, "slots"), _index(lens, B, dev, "lens"), _status(status, dev)
-    handle = _on(dev, stream)
-    if handle is None:
+    ps, pl = _indices(slots, lens, B, dev, "lens")
+    st = None if status is None else _status(status, dev)
+    if stream is not None or _current_device() != dev:
         with torch.cuda.stream(_other(dev, stream)):
             return kv4_attention(cache, l, q, slots, lens, scale, longest or None, out, status)
-    row = H * hd
-    if q.is_contiguous() and q.data_ptr() % 16 == 0:
-        rows = q
-    elif len(shape) == 3:
+    row, rows, pq = H * hd, q, q.data_ptr()
+    if q.is_contiguous() and pq % 16 == 0:
+        if out is None:
+            out = torch.empty_like(q)
+    elif dims == 3:
         rows, row = _rows(q)
     else:  # one stride between all rows, or a copy
         s = q.stride()
@@ -208,11 +217,16 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
             rows, row = _rows(q.as_strided((B * T, H, hd), (s[1] if T > 1 else s[0], s[2], s[3])))
         else:
             rows = _aligned(q)
+    if rows is not q:
+        pq = rows.data_ptr()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     n = 0 if 0 < longest <= 256 else _ws_bytes(c.slots, c.L, c.n_kv, hd, c.maxT, B, T, H)
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
-    check(_dll().jl_kv4_attn(c, l, rows.data_ptr(), kind, row, ps, pl, longest, B, T, H,
-                             1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(),
-                             ws.data_ptr() if n else None, n, st, handle), "jl_kv4_attn")
+    if _Lib.append is None:
+        _Lib.bind()
+    code = _Lib.attn(c, l, pq, kind, row, ps, pl, longest, B, T, H, 1.0 / math.sqrt(hd) if scale is None else scale,
+                     out.data_ptr(), ws.data_ptr() if n else None, n, st, _raw_stream(dev))
+    if code:
+        check(code, "jl_kv4_attn")
     return out
