@@ -555,12 +555,12 @@ int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* positions, 
  * outside [0, longest] or a slot outside the cache gives zeros and the status
  * bit (and a wait inside the call that ran out sets bit 1, with out undefined).
  * out does not overlap q's rows or what lies between them, nor the other buffers.
- * ws: jl_kv4_attn_ws(c, B, T, H) bytes of device memory, 16-byte aligned,
- * used by this call alone until it has run (calls that can run at the same
- * time, captured graphs among them, need one each); none where longest is 1 to
- * 256. B = 0 does nothing. The result does not depend on what else runs: no
+ * ws: jl_kv4_attn_ws(c, B, T, H, longest) bytes of device memory (asked on the
+ * call's device; 0: none, as where longest is 1 to 256), 16-byte aligned, used
+ * by this call alone until it has run (calls that can run at the same time,
+ * captured graphs among them, need one each). B = 0 does nothing. The result does not depend on what else runs: no
  * atomics on it, one order of sums. */
-long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H);
+long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H, int longest);
 int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, long long q_stride,
                 const int* slots, const int* lens, int longest, int B, int T, int H,
                 float scale, void* out, void* ws, long long ws_bytes, int* dev_status,

@@ -1350,7 +1350,7 @@ extern "C" int jl_dec_create_ex(const KernelCfg* c, const KernelW* W, int max_ba
         kv4_dims d4;
         d4.slots = slots, d4.L = h->L, d4.KH = h->KH, d4.hd = h->hd, d4.maxT = h->maxT;
         d4.nb = (h->maxT + kKv4Rows - 1) / kKv4Rows;
-        h->kv4_ws_bytes = std::max(jl_kv4_attn_ws_bytes(d4, max_batch, 1, h->H), jl_kv4_attn_ws_bytes(d4, 1, max_batch, h->H));
+        h->kv4_ws_bytes = jl_kv4_attn_ws_most(d4);
     }
     h->stage_bytes = std::max({V * d * sizeof(float), (size_t)h->nqkv * d * 2, d * (size_t)h->qn * 2});
     struct alloc { void** p; size_t n; } al[] = {

@@ -221,7 +221,9 @@ struct jl_kv4_attn_args {
     float scale;
     int dtype, len_add, longest, B, T, H, outT_ld;
 };
-long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H);
+// The workspace of one call on the current device, and the most that any call on c needs.
+long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H, int longest);
+long long jl_kv4_attn_ws_most(const jl::kv4_dims& c);
 int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s);
 // The tcgen05 form for many query rows (jl_kv4_prompt.cu): a block per unit of 256 rows
 // of one kv head and per split of its cache blocks; S > 1 splits need a workspace.

@@ -251,10 +251,12 @@ extern "C" int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* 
     return (wide ? launch_read<128, __nv_bfloat16> : launch_read<64, __nv_bfloat16>)(d, l, slots, positions, N, k, v, dev_status, s);
 }
 
-extern "C" long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H) {
+extern "C" long long jl_kv4_attn_ws(const jl_kv4* c, int B, int T, int H, int longest) {
     jl::kv4_dims d;
-    if (jl_kv4_view(c, 0, &d) || B < 0 || T < 1 || H < 1 || H % d.KH) return -1;
-    return jl_kv4_attn_ws_bytes(d, B, T, H);
+    if (jl_kv4_view(c, 0, &d) || B < 0 || T < 1 || H < 1 || H % d.KH || (long long)B * T > INT_MAX / H || longest < 0 ||
+        longest > d.maxT)
+        return -1;
+    return B ? jl_kv4_attn_ws_bytes(d, B, T, H, longest ? longest : d.maxT) : 0;
 }
 
 extern "C" int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, long long q_stride, const int* slots,
@@ -276,7 +278,7 @@ extern "C" int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, lon
     const long long n = (long long)B * T, esize = dtype == JL_F32 ? 4 : 2;
     const char *q0 = static_cast<const char*>(q), *o0 = static_cast<const char*>(out);
     if (q0 < o0 + n * row * esize && o0 < q0 + ((n > 1 ? (n - 1) * q_stride : 0) + row) * esize) return JL_ERR_INVALID;
-    const long long need = longest && longest <= 256 ? 0 : jl_kv4_attn_ws_bytes(d, B, T, H);
+    const long long need = jl_kv4_attn_ws_bytes(d, B, T, H, longest ? longest : d.maxT);
     if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need)) return JL_ERR_INVALID;
     jl_kv4_attn_args a;
     a.q = q, a.dtype = dtype, a.q_stride = q_stride, a.slots = slots, a.lens = lens, a.len_add = 0;

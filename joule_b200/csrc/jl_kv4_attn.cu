@@ -12,6 +12,7 @@
 // k_kv4_merge.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "jl_internal.h"
 #include "jl_kv4_dev.cuh"
@@ -406,7 +407,8 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
 // of two whole cache blocks, filled by 16-byte asynchronous copies (17 instructions a
 // block; a bulk copy held its issuing warp for hundreds of ns); no barrier between
 // warps but for the sum of a block that is inside one segment.
-template <int HD, typename T>
+// BLOCK: a segment per block, whose warps share it and join here; no cut, no second kernel.
+template <int HD, typename T, bool BLOCK>
 __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
     extern __shared__ __align__(128) uint8_t smem[];
     using SM = kv4_smem<HD>;
@@ -429,29 +431,37 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             for (long long i = lane; i < 8 * n8; i += 32)
                 a.outT[(size_t)(i % (a.H * HD)) * a.outT_ld + r0 + i / (a.H * HD)] = 0.0f;
     }
-    const uint32_t U = warp_total(seqs, a.B) * S;
-    if (U == 0) return;
-    const kv4_cut cut(U, gridDim.x, NW);
-    if (blockIdx.x >= cut.ctas) return;
-    const int used = cut.warps(blockIdx.x);
-    if (warp >= used) return;
-    const int wid = blockIdx.x * cut.nw + warp;
-    const kv4_split mine = cut.by_warp(blockIdx.x);
-    const uint32_t c0 = cut.start(blockIdx.x), c1 = cut.start(blockIdx.x + 1), u0 = c0 + mine.start(warp);
-    int units = mine.start(warp + 1) - mine.start(warp);  // units of this warp's run
-    int b;
-    uint32_t off;
-    warp_find(seqs, a.B, S, u0, b, off);
     struct cursor {
         int b, s, j, nu;  // sequence, segment, unit of nu
         const uint8_t* p;  // the unit
     } pr;
-    pr.b = b;
-    pr.nu = seqs.units(b);
-    pr.s = (int)(whole ? off : off / pr.nu);
-    pr.j = (int)(whole ? 0 : off % pr.nu);
-    if (whole) {  // so many segments, each with its sequence's units
-        int segs = units, bb = b, ss = pr.s;
+    int used, nw = 1, units;  // warps of the block that have units, of any block; units of this warp's run
+    uint32_t c0, c1, u0;       // the block's units, the warp's first
+    if constexpr (BLOCK) {
+        pr.b = blockIdx.x / S, pr.s = blockIdx.x % S, pr.nu = seqs.units(pr.b);
+        used = min(NW, pr.nu), c0 = 0, c1 = pr.nu;
+        const kv4_split mine(max(1, pr.nu), max(1, used));
+        pr.j = u0 = warp < used ? mine.start(warp) : 0;
+        units = warp < used ? mine.start(warp + 1) - u0 : 0;  // (all warps join the sums)
+    } else {
+        const uint32_t U = warp_total(seqs, a.B) * S;
+        if (U == 0) return;
+        const kv4_cut cut(U, gridDim.x, NW);
+        if (blockIdx.x >= cut.ctas) return;
+        used = cut.warps(blockIdx.x);
+        if (warp >= used) return;
+        nw = cut.nw;
+        const kv4_split mine = cut.by_warp(blockIdx.x);
+        c0 = cut.start(blockIdx.x), c1 = cut.start(blockIdx.x + 1), u0 = c0 + mine.start(warp);
+        units = mine.start(warp + 1) - mine.start(warp);
+        uint32_t off;
+        warp_find(seqs, a.B, S, u0, pr.b, off);
+        pr.nu = seqs.units(pr.b);
+        pr.s = (int)(whole ? off : off / pr.nu);
+        pr.j = (int)(whole ? 0 : off % pr.nu);
+    }
+    if (!BLOCK && whole) {  // so many segments, each with its sequence's units
+        int segs = units, bb = pr.b, ss = pr.s;
         for (units = 0; segs; segs--) {
             units += seqs.units(bb);
             if (++ss == S && segs > 1) {
@@ -461,7 +471,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             }
         }
     }
-    pr.p = c.run(a.slots[b], l, pr.s / R) + (size_t)pr.j * UNIT;
+    pr.p = c.run(a.slots[pr.b], l, pr.s / R) + (size_t)pr.j * UNIT;
     auto advance = [&](cursor& x) {  // not past the last unit
         x.p += UNIT;
         if (++x.j == x.nu) {
@@ -477,7 +487,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     cursor co = pr;
     // the block's run is inside one segment: its warps' sums meet here
     const uint32_t seg0 = u0 - pr.j;
-    const bool joined = !whole && cut.nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nu;
+    const bool joined = BLOCK ? used > 1 : !whole && nw > 1 && c0 >= seg0 && c1 <= seg0 + pr.nu;
     int issued = 0;
     auto issue = [&]() {  // one group of copies per unit, an empty one past the last
         if (issued < units) {
@@ -545,7 +555,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
                 }
             } else {
                 float* part = joined ? reinterpret_cast<float*>(ring)
-                                     : static_cast<float*>(a.ws) + ((size_t)wid * 2 + from_start) * kv4_part_floats(HD);
+                                     : static_cast<float*>(a.ws) + ((size_t)(blockIdx.x * nw + warp) * 2 + from_start) * kv4_part_floats(HD);
                 float* ml = joined ? reinterpret_cast<float*>(smem + SM::stat) + warp * 2 * kKvTile : part + kKvTile * HD;
 #pragma unroll
                 for (int cc = 0; cc < 2; cc++) {
@@ -567,12 +577,13 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         if (i + 1 < units) advance(co);
     }
     if (!joined) return;
-    // all used warps of the block come here: the warps' sums, in their order
-    asm volatile("bar.sync 1, %0;" ::"r"(used * 32) : "memory");
+    // the warps' sums, in their order
+    const int joining = (BLOCK ? NW : used) * 32;
+    asm volatile("bar.sync 1, %0;" ::"r"(joining) : "memory");
     const float* ml = reinterpret_cast<const float*>(smem + SM::stat);
     float* part = static_cast<float*>(a.ws) +
-                  ((size_t)blockIdx.x * cut.nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
-    for (int x = threadIdx.x; x < kKvTile * HD / 4; x += used * 32) {
+                  ((size_t)blockIdx.x * nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
+    for (int x = threadIdx.x; x < kKvTile * HD / 4; x += joining) {
         const int r = x / (HD / 4);
         float m = -INFINITY, lsum = 0.0f;
         for (int w = 0; w < used; w++) m = fmaxf(m, ml[w * 2 * kKvTile + r]);
@@ -583,6 +594,17 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             const float4 v = reinterpret_cast<const float4*>(smem + w * kKvRing * UNIT)[x];
             lsum = fmaf(ml[w * 2 * kKvTile + kKvTile + r], f, lsum);
             o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+        }
+        if constexpr (BLOCK) {
+            const int row = blockIdx.x % S % R * kKvTile + r, h = blockIdx.x % S / R * gsz + row % gsz, d = x % (HD / 4) * 4;
+            if (row >= rows) continue;
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum, y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+            const long long orow = (long long)(blockIdx.x / S) * a.T + row / gsz;
+            put4(static_cast<T*>(a.out) + (orow * a.H + h) * HD + d, y);
+            if (a.outT)
+#pragma unroll
+                for (int j = 0; j < 4; j++) a.outT[(size_t)(h * HD + d + j) * a.outT_ld + orow] = y[j];
+            continue;
         }
         reinterpret_cast<float4*>(part)[x] = o;
         if (x % (HD / 4) == 0) {
@@ -730,44 +752,13 @@ int sm_count() {
 
 int row_tiles(const jl::kv4_dims& c, int T, int H) { return (T * (H / c.KH) + jl::kKvTile - 1) / jl::kKvTile; }
 
-constexpr int kMaxSms = 256;  // the workspace is sized without asking the device
-
-template <int HD>
-int attn_attrs() {
-    using namespace jl;
-    JL_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<HD>::total));
-    JL_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, __half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<HD>::total));
-    JL_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, __nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kv4_smem<HD>::total));
-    return JL_OK;
-}
-
-template <int HD, typename T>
-int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
-    using namespace jl;
-    const int sms = std::min(sm_count(), kMaxSms), R = row_tiles(c, a.T, a.H);
-    if (sms < 1) return JL_ERR_CUDA;
-    const long long segs = (long long)a.B * R * c.KH;
-    if (segs > INT_MAX || segs * ((a.longest + kKv4Rows - 1) / kKv4Rows) > INT_MAX) return JL_ERR_INVALID;  // the cut counts in 32 bits
-    // Segments of at most 256 positions are not cut (and need no workspace): a warp
-    // takes that many sooner than a second kernel starts.
-    const int whole = a.longest <= 256;
-    const int rc = launch(k_kv4_attn<HD, T>, dim3(sms), dim3(kKvWarps * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
-                          whole);
-    if (rc || whole) return rc;
-    const int RB = segs >= sms ? 8 : segs * 4 >= sms ? 2 : 1;
-    const int per = (int)((segs - 1) / (4 * sms) + 1);
-    if (per == 1)
-        return launch(k_kv4_merge<HD, T, false>, dim3((unsigned)segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB, 1);
-    return launch(k_kv4_merge<HD, T, true>, dim3((unsigned)((segs - 1) / per + 1)), dim3(256), 0, s, c, a, R, sms, 8, per);
-}
-
-template <int HD>
-int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
-    if (a.dtype == JL_F32) return launch_t<HD, float>(c, l, a, s);
-    if (a.dtype == JL_F16) return launch_t<HD, __half>(c, l, a, s);
-    return launch_t<HD, __nv_bfloat16>(c, l, a, s);
-}
+// How a call is run: kernel, splits of a unit (tcgen05 form), workspace.
+enum class kv4_form { whole, block, cut, prompt, none };
+struct kv4_plan {
+    kv4_form form;
+    int S;
+    long long ws;
+};
 
 // Splits of each unit of a call in the tcgen05 form: as many as fill the SMs, of at
 // least kMinSplit cache blocks each (4 in place of 2: 64 tokens of 32/4 heads of 128 over
@@ -779,34 +770,101 @@ int splits_of(long long units, int longest, int sms) {
     return std::max(1, (int)std::min<long long>(sms / units, (longest + jl::kKv4Rows - 1) / jl::kKv4Rows / kMinSplit));
 }
 
-}  // namespace
-
-// Two parts for each warp that has blocks, or the splits of the tcgen05 form.
-long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H) {
-    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH, warps = (long long)kMaxSms * jl::kKvWarps;
-    const long long n = segs >= warps ? warps : std::min(warps, 2 * segs * c.nb);  // blocks x warps of a cut: below units + blocks
-    const long long units = jl_kv4_prompt_units(c, B, T, H);
-    return std::max(n * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float),
-                    jl_kv4_prompt_ws_bytes(c, units, splits_of(units, c.nb * jl::kKv4Rows, kMaxSms)));
-}
-
-int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+kv4_plan plan(const jl::kv4_dims& c, int B, int T, int H, int longest, int sms) {
+    using namespace jl;
+    const long long nb = (longest + kKv4Rows - 1) / kKv4Rows, rows = (long long)B * T * H, units = jl_kv4_prompt_units(c, B, T, H);
     // The tcgen05 kernel takes the time of its units of 256 rows, however few rows fill
     // them, and some 14 us beside (start, q, joining); this file's a time by the rows.
     // fp32, 32/4 heads of 128, here / there: 8 tokens (64 rows a unit) over 16,384
     // positions 29 / 34 us, 16 of 4 sequences (128 a unit) 145 / 93; 64 tokens (2,048
     // rows) over 512 17 / 20, over 1,024 21 / 21, over 4,096 47 / 30. Over types, head
     // dims and lengths the rule is within 1 % of the better one (geometric mean).
-    const int sms = std::min(sm_count(), kMaxSms);
+    if (rows >= 76 * units && rows * nb >= 1 << 15) {
+        const int S = splits_of(units, longest, sms);
+        return {kv4_form::prompt, S, jl_kv4_prompt_ws_bytes(c, units, S)};
+    }
+    const long long segs = (long long)B * row_tiles(c, T, H) * c.KH;
+    if (segs > INT_MAX || segs * nb > INT_MAX) return {kv4_form::none, 0, 0};  // the cut counts in 32 bits
+    // Three ways to share the segments' blocks out, with what they take in fp32 at head
+    // dim 128, in units of 0.35 us (a block alone takes a warp 2 us, with all warps busy 4):
+    // a warp per segment, a thread block per segment, or all blocks cut evenly and a second
+    // kernel that adds up. 32/4 heads, 1 / 32 / 64 / 256 sequences, us: over 128 positions
+    // 7.8 / 8.6 / 9.1 / 12.9 by warps, 6.2 / 6.8 / 12.4 / 42 by blocks, over 512 8.4 / 12.6 /
+    // 17.5 / 35 cut, 6.8 / 7.4 / 13.7 / 46 by blocks, over 2,048 9.2 / 20.5 / 30 / 86 and
+    // 15 / 16 / 30 / 110. Lengths are taken as even up to 3/4 of the longest for the cut,
+    // whose work follows them; a block of head dim 64 takes half.
+    const double per_sm = (double)segs / sms, work = c.hd == 64 ? 0.5 * nb : nb, u = per_sm * work;
+    const double whole = 10 + work * (6 + std::min(per_sm, 12.0) / 2) * std::max(1.0, std::ceil(per_sm / kKvWarps));
+    const double block = (double)((segs - 1) / sms + 1) * (12 + work), cut = 24 + std::min(9.0, 6 * u) + 0.75 * u;
+    if (longest <= 256) return {whole < block ? kv4_form::whole : kv4_form::block, 1, 0};
+    if (block < cut) return {kv4_form::block, 1, 0};
+    // two parts for each warp that has blocks (blocks x warps of a cut: below its units + blocks)
+    const long long warps = std::min<long long>((long long)sms * kKvWarps, 2 * segs * nb);
+    return {kv4_form::cut, 1, warps * 2 * kv4_part_floats(c.hd) * (long long)sizeof(float)};
+}
+
+template <int HD, typename T>
+int attn_attrs_t() {
+    using namespace jl;
+    JL_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<HD>::total));
+    JL_CUDA(cudaFuncSetAttribute(k_kv4_attn<HD, T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<HD>::total));
+    return JL_OK;
+}
+
+template <int HD>
+int attn_attrs() {
+    int rc = attn_attrs_t<HD, float>();
+    if (!rc) rc = attn_attrs_t<HD, __half>();
+    if (!rc) rc = attn_attrs_t<HD, __nv_bfloat16>();
+    return rc;
+}
+
+template <int HD, typename T>
+int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, kv4_form form, int sms, cudaStream_t s) {
+    using namespace jl;
+    const int R = row_tiles(c, a.T, a.H);
+    const unsigned segs = (unsigned)((long long)a.B * R * c.KH);
+    const dim3 threads(kKvWarps * 32);
+    const size_t smem = kv4_smem<HD>::total;
+    if (form == kv4_form::block) return launch(k_kv4_attn<HD, T, true>, dim3(segs), threads, smem, s, c, l, a, R, 0);
+    const int rc = launch(k_kv4_attn<HD, T, false>, dim3(sms), threads, smem, s, c, l, a, R, (int)(form == kv4_form::whole));
+    if (rc || form == kv4_form::whole) return rc;
+    const int RB = segs >= (unsigned)sms ? 8 : segs * 4 >= (unsigned)sms ? 2 : 1, per = (int)((segs - 1) / (4 * sms) + 1);
+    if (per == 1) return launch(k_kv4_merge<HD, T, false>, dim3(segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB, 1);
+    return launch(k_kv4_merge<HD, T, true>, dim3((segs - 1) / per + 1), dim3(256), 0, s, c, a, R, sms, 8, per);
+}
+
+template <int HD>
+int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, kv4_form form, int sms, cudaStream_t s) {
+    if (a.dtype == JL_F32) return launch_t<HD, float>(c, l, a, form, sms, s);
+    if (a.dtype == JL_F16) return launch_t<HD, __half>(c, l, a, form, sms, s);
+    return launch_t<HD, __nv_bfloat16>(c, l, a, form, sms, s);
+}
+
+}  // namespace
+
+// (Without a device: a B200's 148 SMs.)
+long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H, int longest) {
+    const int sms = sm_count();
+    return plan(c, B, T, H, longest, sms > 0 ? sms : 148).ws;
+}
+
+long long jl_kv4_attn_ws_most(const jl::kv4_dims& c) {
+    const long long sms = sm_count();
+    return std::max(sms * jl::kKvWarps * 2 * jl::kv4_part_floats(c.hd) * (long long)sizeof(float),
+                    jl_kv4_prompt_ws_bytes(c, 1, (int)sms));
+}
+
+int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, cudaStream_t s) {
+    const int sms = sm_count();
     if (sms < 1) return JL_ERR_CUDA;
-    const long long rows = (long long)a.B * a.T * a.H, units = jl_kv4_prompt_units(c, a.B, a.T, a.H);
-    const int S = splits_of(units, a.longest, sms);
-    if (rows >= 76 * units && rows * ((a.longest + jl::kKv4Rows - 1) / jl::kKv4Rows) >= 1 << 15)
-        return jl_launch_kv4_prompt(c, l, a, S, s);
+    const kv4_plan p = plan(c, a.B, a.T, a.H, a.longest, sms);
+    if (p.form == kv4_form::none) return JL_ERR_INVALID;
+    if (p.form == kv4_form::prompt) return jl_launch_kv4_prompt(c, l, a, p.S, s);
     const int rc = jl_device_once(kOnceKv4, [] {
         const int r = attn_attrs<64>();
         return r ? r : attn_attrs<128>();
     });
     if (rc) return rc;
-    return c.hd == 64 ? launch_hd<64>(c, l, a, s) : launch_hd<128>(c, l, a, s);
+    return c.hd == 64 ? launch_hd<64>(c, l, a, p.form, sms, s) : launch_hd<128>(c, l, a, p.form, sms, s);
 }

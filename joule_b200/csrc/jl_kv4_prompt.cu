@@ -194,17 +194,6 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
     put8(p, y);
 }
 
-// Four values.
-__device__ __forceinline__ void put4(float* p, const float* x) { store_piece(p, x); }
-__device__ __forceinline__ void put4(__half* p, const float* x) {
-    const __half2 u = __floats2half2_rn(x[0], x[1]), v = __floats2half2_rn(x[2], x[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
-}
-__device__ __forceinline__ void put4(__nv_bfloat16* p, const float* x) {
-    const __nv_bfloat162 u = __floats2bfloat162_rn(x[0], x[1]), v = __floats2bfloat162_rn(x[2], x[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
-}
-
 // Unpacks one cache block (kPrUnpack warps, tid from 0) into operand tiles and fp32
 // scales; positions from n on (never written) get scales of 0.
 template <int HD>

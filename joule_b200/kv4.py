@@ -165,9 +165,9 @@ def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.
 
 
 @functools.lru_cache(maxsize=4096)
-def _ws_bytes(slots: int, L: int, n_kv: int, hd: int, maxT: int, B: int, T: int, H: int) -> int:
-    """jl_kv4_attn_ws for these sizes."""
-    return max(0, get_dll().jl_kv4_attn_ws(Kv4(16, slots, L, n_kv, hd, maxT), B, T, H))
+def _ws_bytes(dev: int, slots: int, L: int, n_kv: int, hd: int, maxT: int, B: int, T: int, H: int, longest: int) -> int:
+    """jl_kv4_attn_ws for these sizes on device `dev`, the current one."""
+    return max(0, get_dll().jl_kv4_attn_ws(Kv4(16, slots, L, n_kv, hd, maxT), B, T, H, longest))
 
 
 def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Tensor, lens: torch.Tensor,
@@ -221,7 +221,7 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
         pq = rows.data_ptr()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    n = 0 if 0 < longest <= 256 else _ws_bytes(c.slots, c.L, c.n_kv, hd, c.maxT, B, T, H)
+    n = 0 if 0 < longest <= 256 else _ws_bytes(dev, c.slots, c.L, c.n_kv, hd, c.maxT, B, T, H, longest)
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
     if _Lib.append is None:
         _Lib.bind()

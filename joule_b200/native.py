@@ -135,7 +135,7 @@ SIGNATURES = {
     "jl_kv4_bytes": ([ctypes.POINTER(Kv4)], _LL),
     "jl_kv4_append": ([ctypes.POINTER(Kv4), _I, _P, _P, _I, _LL, _LL, _P, _P, _I, _P, _P], _I),
     "jl_kv4_read": ([ctypes.POINTER(Kv4), _I, _P, _P, _I, _P, _P, _I, _P, _P], _I),
-    "jl_kv4_attn_ws": ([ctypes.POINTER(Kv4), _I, _I, _I], _LL),
+    "jl_kv4_attn_ws": ([ctypes.POINTER(Kv4), _I, _I, _I, _I], _LL),
     "jl_kv4_attn": ([ctypes.POINTER(Kv4), _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _LL,
                      _P, _P], _I),
     "jl_dec_kv4": ([_P, ctypes.POINTER(Kv4)], _I),

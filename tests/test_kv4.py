@@ -95,11 +95,22 @@ def test_bad_arguments_are_refused(dll):
                                  at(scale=float("nan")), at(scale=float("inf")), at(out=None), at(out=(1 << 20) + 8),
                                  at(out=4096), at(out=4096 + 2 * 512 * 4 - 16), at(qs=1 << 20, out=1 << 20),
                                  at(B=2**20, T=2**20)))
-    assert dll.jl_kv4_attn_ws(r, 2, 1, 3) == -1 and dll.jl_kv4_attn_ws(r, 2, 0, 4) == -1
-    need = dll.jl_kv4_attn_ws(r, 2, 1, 4)
-    assert need >= 0
-    if need:
-        assert at(ws=None) == -1 and at(wb=need - 1) == -1 and at(ws=4100) == -1
+    ws = dll.jl_kv4_attn_ws
+    assert all(x == -1 for x in (ws(r, 2, 1, 3, 0), ws(r, 2, 0, 4, 0), ws(r, -1, 1, 4, 0), ws(r, 2, 1, 4, -1),
+                                 ws(r, 2, 1, 4, 129), ws(r, 2**20, 2**20, 4, 0)))
+    assert ws(r, 0, 1, 4, 0) == 0 and ws(r, 2, 1, 4, 0) == 0
+
+
+@pytest.mark.parametrize("B,T,longest", [(64, 1, 0), (2, 1, 9000), (1, 64, 3000)])
+def test_calls_without_their_workspace_are_refused(dll, B, T, longest):
+    """Steps that are cut over all warps, and chunks whose cache is split."""
+    c = _c(slots=64, maxT=10000)
+    r = ctypes.byref(c)
+    need = dll.jl_kv4_attn_ws(r, B, T, 16, longest)
+    assert need > 0 and dll.jl_kv4_attn_ws(r, B, T, 16, 256) == 0
+    at = lambda ws, wb: dll.jl_kv4_attn(r, 0, 4096, 0, 2048, 4096, 4096, longest, B, T, 16, 1.0, 1 << 30, ws, wb, None,  # noqa: E731
+                                        None)
+    assert at(None, need) == -1 and at(4096, need - 1) == -1 and at(4100, need) == -1
 
 
 def test_front_end_refuses_without_a_device():

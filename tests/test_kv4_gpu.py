@@ -203,6 +203,13 @@ STEP = [  # B, H, kv, hd, lens
 ]
 
 
+# more (sequence, kv head) pairs than SMs, with short, middle and long caches: a warp for each, all
+# blocks cut over all warps, runs of pairs in the adding up; and one long sequence
+STEP += [(200, 8, 8, 64, [(31 * b) % 251 for b in range(200)]), (40, 16, 4, 128, [(211 * b) % 1501 for b in range(40)]),
+         (40, 15, 5, 64, [(211 * b) % 1501 for b in range(40)]), (80, 16, 8, 64, [(53 * b) % 701 for b in range(80)]),
+         (75, 8, 8, 128, [(53 * b) % 1701 for b in range(75)]), (1, 16, 2, 128, [3000])]
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("B,H,kv,hd,lens", STEP)
 def test_step(B, H, kv, hd, lens, t):
@@ -227,6 +234,7 @@ CHUNK = [  # B, T, H, kv, hd, lens
     (1, 2, 4, 2, 64, [2]), (1, 5, 8, 1, 128, [5]), (2, 3, 5, 5, 64, [100, 2]), (1, 64, 8, 1, 128, [64]),
     (3, 17, 6, 2, 128, [300, 17, 0]), (1, 33, 10, 2, 64, [700]), (2, 130, 4, 2, 128, [190, 131]),
     (1, 200, 3, 1, 64, [200]), (4, 16, 16, 1, 128, [64, 65, 500, 1]), (1, 257, 2, 1, 128, [900]),
+    (5, 7, 40, 4, 128, [2000, 6, 1999, 0, 700]),
 ]
 
 
