@@ -777,9 +777,9 @@ kv4_plan plan(const jl::kv4_dims& c, int B, int T, int H, int longest, int sms) 
     // them, and some 14 us beside (start, q, joining); this file's a time by the rows.
     // fp32, 32/4 heads of 128, here / there: 8 tokens (64 rows a unit) over 16,384
     // positions 29 / 34 us, 16 of 4 sequences (128 a unit) 145 / 93; 64 tokens (2,048
-    // rows) over 512 17 / 20, over 1,024 21 / 21, over 4,096 47 / 30. Over types, head
-    // dims and lengths the rule is within 1 % of the better one (geometric mean).
-    if (rows >= 76 * units && rows * nb >= 1 << 15) {
+    // rows) over 512 14 / 20, over 1,024 21 / 21, over 4,096 47 / 30. Over types, head
+    // dims and lengths the rule is within 0.5 % of the better one (geometric mean).
+    if (rows >= 76 * units && rows * nb >= 310ll * sms) {
         const int S = splits_of(units, longest, sms);
         return {kv4_form::prompt, S, jl_kv4_prompt_ws_bytes(c, units, S)};
     }
