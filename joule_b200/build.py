@@ -5,7 +5,8 @@
 
 Each .cu under csrc/ compiles to an object in parallel; the objects link into
 one shared library with a static CUDA runtime. No torch headers are used:
-the library's ABI is plain C (include/joule_moe.h).
+the library's ABI is plain C (include/joule_moe.h). csrc/kv4_call.c, which
+needs Python's headers alone, becomes joule_b200/_kv4_call.so.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,6 +23,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libjoule_moe.so"
+CALL = PKG / "_kv4_call.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I", str(ROOT / "include"), "-I", str(CSRC)]
@@ -48,6 +51,21 @@ def _compile(src: Path, force: bool, extra: list[str]) -> Path:
     return obj
 
 
+def _call_module(force: bool) -> None:
+    src = CSRC / "kv4_call.c"
+    deps = [src, ROOT / "include" / "joule_moe.h"]
+    if not force and CALL.exists() and CALL.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
+        return
+    cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")
+    if not cc:
+        raise RuntimeError("no C compiler")
+    cmd = [cc, "-O2", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"], "-I", str(ROOT / "include"), str(src),
+           "-o", str(CALL), "-lm"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cc} failed for {src.name}:\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
@@ -59,6 +77,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    _call_module(force)
     return LIB
 
 

@@ -17,7 +17,7 @@ length outside it skips the row (append) or reads as zeros, and sets bit 8 of
 """
 from __future__ import annotations
 
-import functools
+import ctypes
 import math
 
 import torch
@@ -46,14 +46,22 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle 
 _current_device = torch._C._cuda_getDevice
 
 
-class _Lib:
-    """The library's entry points, bound at the first call."""
-    append = read = attn = None
+_call = None  # the compiled form of regular calls (csrc/kv4_call.c), bound at the first one
+_dll = None
 
-    @classmethod
-    def bind(cls) -> None:
-        dll = get_dll()
-        cls.read, cls.attn, cls.append = dll.jl_kv4_read, dll.jl_kv4_attn, dll.jl_kv4_append
+
+def _bind() -> None:
+    global _call, _dll
+    dll = get_dll()
+    try:
+        from joule_b200 import _kv4_call
+    except ImportError as e:
+        raise FileNotFoundError("joule_b200/_kv4_call.so is missing: run `python -m joule_b200.build`") from e
+    entries = [ctypes.cast(f, ctypes.c_void_p).value
+               for f in (dll.jl_kv4_append, dll.jl_kv4_read, dll.jl_kv4_attn, dll.jl_kv4_attn_ws)]
+    _kv4_call.bind(torch.uint8, torch.int32, torch.float32, torch.float16, torch.bfloat16, torch.empty, torch.empty_like,
+                   _current_device, _raw_stream, *entries)
+    _dll, _call = dll, _kv4_call
 
 
 def _view(cache: torch.Tensor, l: int) -> tuple[Kv4, int]:
@@ -118,6 +126,12 @@ def kv4_append(cache: torch.Tensor, l: int, k: torch.Tensor, v: torch.Tensor, sl
                positions: torch.Tensor, status: torch.Tensor | None = None, stream=None) -> None:
     """Quantise k, v [N, n_kv, hd] (fp32, fp16 or bf16; rows of any stride)
     into positions[n] of slot slots[n] (int32 [N], distinct pairs) of layer l."""
+    if _call is None:
+        _bind()
+    if status is None and stream is None:
+        code = _call.append(cache, l, k, v, slots, positions)
+        if code is not None:
+            return check(code, "jl_kv4_append") if code else None
     c, dev = _view(cache, l)
     shape = k.shape
     if shape != v.shape or len(shape) != 3 or shape[1] != c.n_kv or shape[2] != c.hd:
@@ -133,17 +147,22 @@ def kv4_append(cache: torch.Tensor, l: int, k: torch.Tensor, v: torch.Tensor, sl
             return kv4_append(cache, l, k, v, slots, positions, status)
     k, sk = _rows(k)
     v, sv = _rows(v)
-    if _Lib.append is None:
-        _Lib.bind()
-    code = _Lib.append(c, l, k.data_ptr(), v.data_ptr(), kind, sk, sv, ps, pp, n, st, _raw_stream(dev))
-    if code:
-        check(code, "jl_kv4_append")
+    check(_dll.jl_kv4_append(c, l, k.data_ptr(), v.data_ptr(), kind, sk, sv, ps, pp, n, st, _raw_stream(dev)), "jl_kv4_append")
 
 
 def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.Tensor,
              dtype: torch.dtype = torch.float32, status: torch.Tensor | None = None,
              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values [N, n_kv, hd] of (slots[n], positions[n])."""
+    if _call is None:
+        _bind()
+    if status is None and stream is None:
+        done = _call.read(cache, l, slots, positions, dtype)
+        if done is not None:
+            code, k, v = done
+            if code:
+                check(code, "jl_kv4_read")
+            return k, v
     c, dev = _view(cache, l)
     kind = _TYPES.get(dtype)
     if kind is None:
@@ -156,18 +175,8 @@ def kv4_read(cache: torch.Tensor, l: int, slots: torch.Tensor, positions: torch.
             return kv4_read(cache, l, slots, positions, dtype, status)
     k = torch.empty(n, c.n_kv, c.hd, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
-    if _Lib.append is None:
-        _Lib.bind()
-    code = _Lib.read(c, l, ps, pp, n, k.data_ptr(), v.data_ptr(), kind, st, _raw_stream(dev))
-    if code:
-        check(code, "jl_kv4_read")
+    check(_dll.jl_kv4_read(c, l, ps, pp, n, k.data_ptr(), v.data_ptr(), kind, st, _raw_stream(dev)), "jl_kv4_read")
     return k, v
-
-
-@functools.lru_cache(maxsize=4096)
-def _ws_bytes(dev: int, slots: int, L: int, n_kv: int, hd: int, maxT: int, B: int, T: int, H: int, longest: int) -> int:
-    """jl_kv4_attn_ws for these sizes on device `dev`, the current one."""
-    return max(0, get_dll().jl_kv4_attn_ws(Kv4(16, slots, L, n_kv, hd, maxT), B, T, H, longest))
 
 
 def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Tensor, lens: torch.Tensor,
@@ -181,6 +190,15 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     length); a longer entry counts as outside the cache. Rows that see nothing
     are zero. Returns out, of q's shape and type; one that is given does not
     overlap q (JouleError)."""
+    if _call is None:
+        _bind()
+    if out is None and status is None and stream is None:
+        done = _call.attention(cache, l, q, slots, lens, scale, longest)
+        if done is not None:
+            code, out = done
+            if code:
+                check(code, "jl_kv4_attn")
+            return out
     c, dev = _view(cache, l)
     shape = q.shape
     hd, dims = c.hd, len(shape)
@@ -221,12 +239,8 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
         pq = rows.data_ptr()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    n = 0 if 0 < longest <= 256 else _ws_bytes(dev, c.slots, c.L, c.n_kv, hd, c.maxT, B, T, H, longest)
+    n = max(0, _dll.jl_kv4_attn_ws(c, B, T, H, longest))
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
-    if _Lib.append is None:
-        _Lib.bind()
-    code = _Lib.attn(c, l, pq, kind, row, ps, pl, longest, B, T, H, 1.0 / math.sqrt(hd) if scale is None else scale,
-                     out.data_ptr(), ws.data_ptr() if n else None, n, st, _raw_stream(dev))
-    if code:
-        check(code, "jl_kv4_attn")
+    check(_dll.jl_kv4_attn(c, l, pq, kind, row, ps, pl, longest, B, T, H, 1.0 / math.sqrt(hd) if scale is None else scale,
+                           out.data_ptr(), ws.data_ptr() if n else None, n, st, _raw_stream(dev)), "jl_kv4_attn")
     return out

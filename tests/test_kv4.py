@@ -144,3 +144,20 @@ def test_decoder_flags_are_checked(dll):
     assert make(DEC_KV4) == -1 and make(2, hd=64) == -1 and make(-1, hd=64) == -1
     c = Kv4()
     assert dll.jl_dec_kv4(None, ctypes.byref(c)) == -1
+
+
+def test_the_compiled_calls_pass_on_what_is_not_regular():
+    """joule_b200._kv4_call answers None, and leaves no error set, to arguments
+    that the Python function must copy, refuse or raise on."""
+    kv4._bind()
+    call = kv4._call
+    cache = torch.zeros(2, 1, 2, 1, 68 * 64, dtype=torch.uint8)
+    i, x, q = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, 64), torch.zeros(2, 4, 64)
+    for bad in (cache, None, 3, "x", torch.zeros(1, 1, 1, 1, 1, 1)):
+        assert call.append(bad, 0, x, x, i, i) is None
+        assert call.read(bad, 0, i, i, torch.float32) is None
+        assert call.attention(bad, 0, q, i, i, None, None) is None
+    assert call.append() is None and call.read(cache) is None and call.attention(cache, 0) is None
+    assert call.read(cache, 0, i, i, torch.float64) is None
+    with pytest.raises(TypeError):
+        call.bind(1)

@@ -412,6 +412,38 @@ def test_a_step_captured_and_replayed():
             _check(outs[w][i][:, None], q[w, i][:, None].astype(np.float64), ks, vs, hd ** -0.5, "f32")
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_compiled_and_interpreted_calls_agree(t):
+    """A call with a status word goes through the Python function, one without
+    through its compiled form, when the tensors are regular; misaligned and strided
+    ones are copied either way. References to the arguments are as before."""
+    import sys
+    from joule_b200 import kv4
+    rng = np.random.default_rng(23)
+    B, H, kv, hd = 3, 6, 2, 64
+    caches = [kv4.kv4_cache(B, 2, kv, hd, 700).zero_() for _ in range(2)]
+    n = 900
+    k, v = (_to(rng.standard_normal((n, kv, hd)), t) for _ in range(2))
+    at = rng.permutation(B * 700)[:n]
+    slots, pos, status = _i32(at // 700), _i32(at % 700), _i32([0])
+    lens, ls = _i32([700, 1, 0]), _i32([2, 0, 1])
+    q = _to(rng.standard_normal((B, 4, H, hd)), t)
+    args = [caches[0], k, v, slots, pos, q, lens, ls]
+    before = [sys.getrefcount(a) for a in args]
+    kv4.kv4_append(caches[0], 1, k, v, slots, pos)
+    kv4.kv4_append(caches[1], 1, k, v, slots, pos, status=status)
+    assert torch.equal(caches[0], caches[1])
+    for dt in DT.values():
+        a, b = kv4.kv4_read(caches[0], 1, slots, pos, dtype=dt), kv4.kv4_read(caches[0], 1, slots, pos, dtype=dt, status=status)
+        assert all(x.dtype is dt and torch.equal(x, y) for x, y in zip(a, b))
+    for x in (q, q[:, 0], q.transpose(1, 2).contiguous().transpose(1, 2), torch.cat([q.flatten()[:1], q.flatten()])[1:].view(q.shape)):
+        for kw in (dict(), dict(scale=0.3), dict(longest=700), dict(longest=699)):
+            a, b = kv4.kv4_attention(caches[0], 1, x, ls, lens, **kw), kv4.kv4_attention(caches[0], 1, x, ls, lens, status=status, **kw)
+            assert a.shape == x.shape and a.dtype is x.dtype and a.is_contiguous() and torch.equal(a, b)
+    del x, a, b
+    assert [sys.getrefcount(a) for a in args] == before
+
+
 def test_front_end_refusals():
     from joule_b200 import kv4
     cache = kv4.kv4_cache(2, 1, 2, 64, 64)
