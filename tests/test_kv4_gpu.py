@@ -151,6 +151,23 @@ def test_values_a_record_cannot_hold():
     assert np.array_equal(gv.double().cpu().numpy(), okv4.held(-x))
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_values_around_the_largest_scale(t):
+    """Groups whose largest value passes 7 * 65504 by a little, by 16 steps, by far:
+    every value is the nearest of -8 .. 7 steps, none wraps."""
+    from joule_b200 import kv4
+    rng = np.random.default_rng(29)
+    n = 300
+    x = rng.standard_normal((n, 2, 64)) * 10 ** rng.uniform(4, 14, (n, 2, 1))
+    x = _to(x, t).float().cpu().numpy()
+    cache = kv4.kv4_cache(1, 1, 2, 64, n)
+    at = (_i32([0] * n), _i32(range(n)))
+    kv4.kv4_append(cache, 0, _to(x, t), _to(-x, t), *at)
+    gk, gv = kv4.kv4_read(cache, 0, *at)
+    assert np.array_equal(gk.double().cpu().numpy(), okv4.held(x))
+    assert np.array_equal(gv.double().cpu().numpy(), okv4.held(-x))
+
+
 def test_append_takes_strided_rows_and_other_orders():
     """Rows inside a fused projection, every second row, a transposed tensor, an odd offset."""
     from joule_b200 import kv4
