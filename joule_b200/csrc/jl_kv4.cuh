@@ -84,7 +84,7 @@ __device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, 
     const __half sh = __float2half_rn(fminf(__fdiv_rn(fmaxf(amax, 1e-12f), 7.0f), 65504.0f));
     const float s = __half2float(sh), inv = __frcp_rn(s), bound = 0.4999f * s;
     uint32_t w = 0;
-    bool sure = s < 65504.0f;  // (a value past the largest scale)
+    bool sure = s >= 0x1p-21f && s < 65504.0f;  // (others can leave values past 7.5 steps)
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float q = fmaf(v[j], inv, 12582920.0f);

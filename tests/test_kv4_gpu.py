@@ -152,13 +152,15 @@ def test_values_a_record_cannot_hold():
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
-def test_values_around_the_largest_scale(t):
-    """Groups whose largest value passes 7 * 65504 by a little, by 16 steps, by far:
-    every value is the nearest of -8 .. 7 steps, none wraps."""
+@pytest.mark.parametrize("low,high", [(4, 14), (-9, -4), (-7.5, -6)])
+def test_values_around_the_largest_and_smallest_scales(low, high, t):
+    """Groups whose largest value passes 7 * 65504 by a little, by 16 steps, by far,
+    and groups whose scale is a few of fp16's smallest steps, rounded by up to half
+    one: every value is the nearest of -8 .. 7 steps, none wraps."""
     from joule_b200 import kv4
     rng = np.random.default_rng(29)
     n = 300
-    x = rng.standard_normal((n, 2, 64)) * 10 ** rng.uniform(4, 14, (n, 2, 1))
+    x = rng.standard_normal((n, 2, 64)) * 10 ** rng.uniform(low, high, (n, 2, 1))
     x = _to(x, t).float().cpu().numpy()
     cache = kv4.kv4_cache(1, 1, 2, 64, n)
     at = (_i32([0] * n), _i32(range(n)))
