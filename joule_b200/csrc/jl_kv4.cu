@@ -13,42 +13,58 @@ namespace jl {
 
 constexpr int kKvThreads = 256;
 
-// Eight values as fp32. STREAM: first to leave L2 (a long call's rows, read once).
+// Eight values as they lie, and as fp32 (apart: a conversion among the loads would
+// wait for each before the next is issued). STREAM: first to leave L2 (a long call's
+// rows, read once).
+template <typename T>
+struct kv4_eight {
+    uint4 w;
+};
+template <>
+struct kv4_eight<float> {
+    float4 x, y;
+};
 template <bool STREAM, typename V>
 __device__ __forceinline__ V load_from(const void* p) {
     return STREAM ? __ldcs(static_cast<const V*>(p)) : *static_cast<const V*>(p);
 }
 template <bool STREAM>
-__device__ __forceinline__ void load8(const float* p, float4& x, float4& y) {
-    x = load_from<STREAM, float4>(p);
-    y = load_from<STREAM, float4>(p + 4);
+__device__ __forceinline__ void load8(const float* p, kv4_eight<float>& v) {
+    v.x = load_from<STREAM, float4>(p);
+    v.y = load_from<STREAM, float4>(p + 4);
 }
-template <bool STREAM>
-__device__ __forceinline__ void load8(const __half* p, float4& x, float4& y) {
-    const uint4 w = load_from<STREAM, uint4>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&w.z));
-    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&w.w));
+template <bool STREAM, typename T>
+__device__ __forceinline__ void load8(const T* p, kv4_eight<T>& v) {
+    v.w = load_from<STREAM, uint4>(p);
+}
+__device__ __forceinline__ void to_fp32(const kv4_eight<float>& v, float4& x, float4& y) { x = v.x, y = v.y; }
+__device__ __forceinline__ void to_fp32(const kv4_eight<__half>& v, float4& x, float4& y) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v.w.y));
+    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v.w.z));
+    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&v.w.w));
     x = make_float4(a.x, a.y, b.x, b.y);
     y = make_float4(c.x, c.y, d.x, d.y);
 }
-template <bool STREAM>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float4& x, float4& y) {
-    const uint4 w = load_from<STREAM, uint4>(p);
-    x = make_float4(bf16_to_f32(w.x & 0xFFFFu), bf16_to_f32(w.x >> 16), bf16_to_f32(w.y & 0xFFFFu), bf16_to_f32(w.y >> 16));
-    y = make_float4(bf16_to_f32(w.z & 0xFFFFu), bf16_to_f32(w.z >> 16), bf16_to_f32(w.w & 0xFFFFu), bf16_to_f32(w.w >> 16));
+__device__ __forceinline__ void to_fp32(const kv4_eight<__nv_bfloat16>& v, float4& x, float4& y) {
+    auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
+    auto hi = [](uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); };
+    x = make_float4(lo(v.w.x), hi(v.w.x), lo(v.w.y), hi(v.w.y));
+    y = make_float4(lo(v.w.z), hi(v.w.z), lo(v.w.w), hi(v.w.w));
 }
 
-// Append and read back: block (row chunk, K or V of a head), a row's head by
-// HD / values-per-lane lanes, STEPS rows of a lane in flight. (An index of one
+// Append and read back: block (row chunk, K or V of a head; a chunk's heads next to one
+// another, or rows of many heads are fetched in pieces: append 29 -> 26 us), a row's
+// head by HD / values-per-lane lanes, several rows of a lane in flight. (An index of one
 // flat item per lane took three times the instructions and bound both kernels by
-// issue: 8,179 rows x 16 heads 65 + 47 us under ncu.)
-constexpr int kKvSteps = 4;
+// issue: 8,179 rows x 16 heads 65 + 47 us under ncu.) Rows in flight in long calls:
+// append 4 (8: 35 us against 26, by registers), read 8 (4: 27 us against 24).
+constexpr int kKvAppendRows = 4, kKvReadRows = 8;
 
 // Append: a lane has one code word (8 values); the 8 lanes of a group reduce its
-// maximum by shuffles and store its record. Bound by HBM (each value read once, an
-// eighth of its fp32 size written).
+// maximum by shuffles and store its record. 8,179 rows of 16 heads of 128: fp32 26 us
+// (23 at the copy rate), bound by HBM and issue alike; bf16 27 us, by issue (some 180
+// instructions for 8 values of each lane).
 template <int HD, typename T, int STEPS>
 __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, const T* __restrict__ k,
                                                            const T* __restrict__ v, long long ks, long long vs,
@@ -57,30 +73,29 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, co
     constexpr int LPR = HD / 8, ROWS = kKvThreads / LPR;  // lanes per row, rows per step
     griddep_wait();
     griddep_launch_dependents();
-    const int is_v = blockIdx.y & 1, h = blockIdx.y >> 1, w = threadIdx.x % LPR, g = w / 8, u = w % 8;
+    const int hv = blockIdx.x % (2 * c.KH), chunk = blockIdx.x / (2 * c.KH);
+    const int is_v = hv & 1, h = hv >> 1, w = threadIdx.x % LPR, g = w / 8, u = w % 8;
     const long long stride = is_v ? vs : ks;
-    const int n0 = blockIdx.x * ROWS * STEPS + threadIdx.x / LPR;
-    const T* src = (is_v ? v : k) + n0 * stride + h * HD + 8 * w;
-    float4 x[STEPS], y[STEPS];
+    const int n0 = chunk * ROWS * STEPS + threadIdx.x / LPR;
+    const T* src = (is_v ? v : k) + h * HD + 8 * w;
+    kv4_eight<T> raw[STEPS];
     int slot[STEPS], pos[STEPS];
 #pragma unroll
-    for (int j = 0; j < STEPS; j++) {
-        const int n = n0 + j * ROWS;
-        slot[j] = -1;
-        x[j] = y[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (n < N) {
-            slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
-            load8<(STEPS > 1)>(src + j * ROWS * stride, x[j], y[j]);
-        }
+    for (int j = 0; j < STEPS; j++) {  // (rows past the last: the last, not stored)
+        const int n = min(n0 + j * ROWS, N - 1);
+        slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
+        load8<(STEPS > 1)>(src + n * stride, raw[j]);
     }
     uint8_t* base = c.run(0, l, h);
     const size_t per_slot = (size_t)c.L * c.KH * c.nb * kv4_block_bytes(HD);
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
-        const bool ok = (unsigned)slot[j] < (unsigned)c.slots && (unsigned)pos[j] < (unsigned)c.maxT;
-        if (!ok && n0 + j * ROWS < N && blockIdx.y == 0 && w == 0 && err) atomicOr(err, kErrKvIndex);
-        uint8_t* blk = base + slot[j] * per_slot + (size_t)(pos[j] / kKv4Rows) * kv4_block_bytes(HD);
-        kv4_store_group(blk, HD, is_v, pos[j] % kKv4Rows, g, u, x[j], y[j], ok);
+        const bool in = n0 + j * ROWS < N, ok = in && (unsigned)slot[j] < (unsigned)c.slots && (unsigned)pos[j] < (unsigned)c.maxT;
+        if (in && !ok && hv == 0 && w == 0 && err) atomicOr(err, kErrKvIndex);
+        uint8_t* blk = base + (unsigned)slot[j] * per_slot + (size_t)((unsigned)pos[j] / kKv4Rows) * kv4_block_bytes(HD);
+        float4 x, y;
+        to_fp32(raw[j], x, y);
+        kv4_store_group(blk, HD, is_v, pos[j] % kKv4Rows, g, u, x, y, ok);
     }
 }
 
@@ -112,7 +127,8 @@ __device__ __forceinline__ void store_values(__nv_bfloat16* p, const float (&x)[
 
 // Read back: a lane writes 16 bytes (half a code word's values in fp32, a word's in
 // 16 bits); (n - 8) * s is exact in fp32 (4 by 11 bits), rounded once to a 16-bit
-// type. A row outside the cache reads as zeros. Bound by HBM (the values written).
+// type. A row outside the cache reads as zeros. Bound by HBM (the values written):
+// 8,179 rows of 16 heads of 128 in fp32 24 us, 23 at the copy rate.
 template <int HD, typename T, int STEPS>
 __global__ void __launch_bounds__(kKvThreads) k_kv4_read(kv4_dims c, int l, T* __restrict__ k, T* __restrict__ v,
                                                          const int* __restrict__ slots,
@@ -120,38 +136,44 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_read(kv4_dims c, int l, T* _
     constexpr int VPT = 16 / sizeof(T), LPR = HD / VPT, ROWS = kKvThreads / LPR;
     griddep_wait();
     griddep_launch_dependents();
-    const int is_v = blockIdx.y & 1, h = blockIdx.y >> 1, e = threadIdx.x % LPR * VPT, g = e / 64, u = e % 64 / 8;
-    const int n0 = blockIdx.x * ROWS * STEPS + threadIdx.x / LPR;
+    const int hv = blockIdx.x % (2 * c.KH), chunk = blockIdx.x / (2 * c.KH);
+    const int is_v = hv & 1, h = hv >> 1, e = threadIdx.x % LPR * VPT, g = e / 64, u = e % 64 / 8;
+    const int n0 = chunk * ROWS * STEPS + threadIdx.x / LPR;
     const uint8_t* base = c.run(0, l, h);
     const size_t per_slot = (size_t)c.L * c.KH * c.nb * kv4_block_bytes(HD);
     uint32_t word[STEPS];
-    float s[STEPS];
+    uint16_t scale[STEPS];
+    int slot[STEPS], pos[STEPS];
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {  // (rows past the last: the last, not stored)
+        const int n = min(n0 + j * ROWS, N - 1);
+        slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
+    }
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
-        const int n = n0 + j * ROWS;
-        word[j] = 0, s[j] = 0.0f;
-        if (n >= N) continue;
-        const int slot = __ldg(slots + n), pos = __ldg(positions + n);
-        if ((unsigned)slot < (unsigned)c.slots && (unsigned)pos < (unsigned)c.maxT) {
-            const uint8_t* blk = base + slot * per_slot + (size_t)(pos / kKv4Rows) * kv4_block_bytes(HD);
-            const int row = pos % kKv4Rows;
-            word[j] = *reinterpret_cast<const uint32_t*>(blk + kv4_word_off(HD, is_v, row, g, u));
-            s[j] = half_bits_to_f32(*reinterpret_cast<const uint16_t*>(blk + kv4_scale_off(HD, is_v, row, g)));
-        } else if (blockIdx.y == 0 && e == 0 && err) {
-            atomicOr(err, kErrKvIndex);
+        const bool ok = (unsigned)slot[j] < (unsigned)c.slots && (unsigned)pos[j] < (unsigned)c.maxT;
+        if (!ok) {
+            if (hv == 0 && e == 0 && err) atomicOr(err, kErrKvIndex);
+            slot[j] = 0, pos[j] = -1;  // some record, read as zeros
         }
+        const unsigned at = max(pos[j], 0);
+        const uint8_t* blk = base + (unsigned)slot[j] * per_slot + (size_t)(at / kKv4Rows) * kv4_block_bytes(HD);
+        word[j] = *reinterpret_cast<const uint32_t*>(blk + kv4_word_off(HD, is_v, at % kKv4Rows, g, u));
+        scale[j] = *reinterpret_cast<const uint16_t*>(blk + kv4_scale_off(HD, is_v, at % kKv4Rows, g));
     }
     T* dst = (is_v ? v : k) + ((size_t)n0 * c.KH + h) * HD + e;
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
         if (n0 + j * ROWS >= N) break;
+        const float s = pos[j] < 0 ? 0.0f : half_bits_to_f32(scale[j]);
+        if (pos[j] < 0) word[j] = 0x88888888u;
         // nibble q of a half word left in place in 2^23's mantissa: 2^23 + 16^q n, then n - 8 by an exact FMA
         float x[VPT];
 #pragma unroll
         for (int q = 0; q < VPT; q++) {
             const uint32_t half = VPT == 4 ? word[j] >> (e % 8 * 4) : q < 4 ? word[j] : word[j] >> 16;
             const float unit = q % 4 == 0 ? 1.0f : q % 4 == 1 ? 0.0625f : q % 4 == 2 ? 0.00390625f : 0.000244140625f;
-            x[q] = __fmul_rn(fmaf(__uint_as_float((half & (15u << (4 * (q % 4)))) | 0x4B000000u), unit, -8388608.0f * unit - 8.0f), s[j]);
+            x[q] = __fmul_rn(fmaf(__uint_as_float((half & (15u << (4 * (q % 4)))) | 0x4B000000u), unit, -8388608.0f * unit - 8.0f), s);
         }
         store_values<(STEPS > 1)>(dst + (size_t)j * ROWS * c.KH * HD, x);
     }
@@ -189,13 +211,15 @@ namespace {
 
 // Several rows of a lane in flight for calls that fill the device with blocks all
 // the same, one row for short ones.
-template <int HD, typename T, int VPT, typename K1, typename K4, typename... Args>
-int launch_rows(K1 one, K4 many, int KH, int N, cudaStream_t s, Args... args) {
+template <int HD, typename T, int VPT, int STEPS, typename K1, typename K, typename... Args>
+int launch_rows(K1 one, K many, int KH, int N, cudaStream_t s, Args... args) {
     using namespace jl;
     const int rows = kKvThreads / (HD / VPT);
     const bool big = (long long)N * KH >= (long long)rows * 1024;
-    const int per = big ? rows * kKvSteps : rows;
-    const dim3 grid((N + per - 1) / per, 2 * KH);
+    const int per = big ? rows * STEPS : rows;
+    const long long blocks = ((long long)N + per - 1) / per * 2 * KH;
+    if (blocks > INT_MAX) return JL_ERR_INVALID;
+    const dim3 grid((unsigned)blocks);
     return big ? launch(many, grid, dim3(kKvThreads), 0, s, args...) : launch(one, grid, dim3(kKvThreads), 0, s, args...);
 }
 
@@ -203,7 +227,7 @@ template <int HD, typename T>
 int launch_append(const jl::kv4_dims& c, int l, const void* k, const void* v, long long ks, long long vs,
                   const int* slots, const int* positions, int N, int* err, cudaStream_t s) {
     using namespace jl;
-    return launch_rows<HD, T, 8>(k_kv4_append<HD, T, 1>, k_kv4_append<HD, T, kKvSteps>, c.KH, N, s, c, l, (const T*)k,
+    return launch_rows<HD, T, 8, kKvAppendRows>(k_kv4_append<HD, T, 1>, k_kv4_append<HD, T, kKvAppendRows>, c.KH, N, s, c, l, (const T*)k,
                                  (const T*)v, ks, vs, slots, positions, N, err);
 }
 
@@ -211,7 +235,7 @@ template <int HD, typename T>
 int launch_read(const jl::kv4_dims& c, int l, const int* slots, const int* positions, int N, void* k, void* v,
                 int* err, cudaStream_t s) {
     using namespace jl;
-    return launch_rows<HD, T, 16 / sizeof(T)>(k_kv4_read<HD, T, 1>, k_kv4_read<HD, T, kKvSteps>, c.KH, N, s, c, l, (T*)k,
+    return launch_rows<HD, T, 16 / sizeof(T), kKvReadRows>(k_kv4_read<HD, T, 1>, k_kv4_read<HD, T, kKvReadRows>, c.KH, N, s, c, l, (T*)k,
                                               (T*)v, slots, positions, N, err);
 }
 

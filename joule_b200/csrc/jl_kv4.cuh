@@ -63,36 +63,65 @@ inline __device__ __noinline__ uint32_t kv4_codes_div(float4 x, float4 y, float 
     return w;
 }
 
+// max of |a|, |b| and m that keeps a NaN.
+__device__ __forceinline__ float kv4_max_nan(float m, float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+
 // Quantises a group of 64 values held by 8 consecutive lanes (lane u of the 8 has
 // word u: values 8u .. 8u + 7, x then y) and stores it as (row r, group g) of block
-// `blk` when `store`. A code is the step nearest to the exact x / s. Its first guess
-// is the product with 1 / s, rounded by adding 1.5 * 2^23 + 8; the guess n stands when
-// what is left, x - (n - 8) s (exact: 11 by 4 bits from a value of the same size), is
-// clearly below half a step, and the lane divides when it is not (a tie or nearly one,
-// a NaN, an infinity, a scale of 0, a value past the largest scale). Beyond the
-// record's own rules: a scale that fp16 cannot hold stays at its largest number
-// (values past 7 * 65504 saturate) and a NaN becomes zero, so what the cache holds is
-// always finite. All lanes of the warp call it.
+// `blk` when `store`. A code is the step nearest to the exact x / s, ties to even. Its
+// first guess k is the product with about 1 / s, rounded by adding 1.5 * 2^23 + 8; it
+// stands when what is left, x - k s, is below half a step. That remainder is exact
+// (11 by 4 bits from a value of the same size), so a value past half or at half of a
+// step moves by one (one bf16 value in 700 is at half). The lane divides for a NaN, an infinity, and a
+// scale past the largest or of less than 8 of fp16's smallest steps, whose rounding can
+// leave amax above 7.5 steps. amax / 7 is the product with 1 / 7 corrected once by its
+// exact remainder (Markstein's correction; equal to the IEEE quotient for every
+// significand). Beyond the record's own rules: a scale that fp16 cannot hold stays at
+// its largest number (values past 7 * 65504 saturate) and a NaN becomes zero, so what
+// the cache holds is always finite. All lanes of the warp call it.
 __device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, int r, int g, int u, float4 x, float4 y,
                                                 bool store) {
-    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    const float2 v[4] = {make_float2(x.x, x.y), make_float2(x.z, x.w), make_float2(y.x, y.y), make_float2(y.z, y.w)};
     float amax = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(v[j]));
+    for (int j = 0; j < 4; j++) amax = fmaxf(amax, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
 #pragma unroll
     for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const __half sh = __float2half_rn(fminf(__fdiv_rn(fmaxf(amax, 1e-12f), 7.0f), 65504.0f));
-    const float s = __half2float(sh), inv = __frcp_rn(s), bound = 0.4999f * s;
-    uint32_t w = 0;
-    bool sure = s >= 0x1p-21f && s < 65504.0f;  // (others can leave values past 7.5 steps)
+    amax = fmaxf(amax, 1e-12f);
+    const float seventh = 1.0f / 7.0f, q0 = amax * seventh;  // (an infinity becomes a NaN, and the largest scale)
+    const __half sh = __float2half_rn(fminf(fmaf(fmaf(-7.0f, q0, amax), seventh, q0), 65504.0f));
+    const float s = __half2float(sh);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const float2 inv2 = make_float2(inv, inv), s2 = make_float2(s, s), magic = make_float2(12582920.0f, 12582920.0f);
+    float2 d[4];  // -k
+    float left = s >= 0x1p-21f && s < 65504.0f ? 0.0f : INFINITY;  // (others can be more than 7.5 steps)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float q = fmaf(v[j], inv, 12582920.0f);
-        const float left = fmaf(12582920.0f - q, s, v[j]);
-        sure = sure && fabsf(left) <= bound;
-        w |= (__float_as_uint(q) & 15u) << (4 * j);
+    for (int j = 0; j < 4; j++) {
+        d[j] = __ffma2_rn(__ffma2_rn(v[j], inv2, magic), make_float2(-1.0f, -1.0f), magic);
+        const float2 e = __ffma2_rn(d[j], s2, v[j]);
+        left = kv4_max_nan(left, e.x, e.y);
     }
-    if (!sure) w = kv4_codes_div(x, y, s);
+    // four codes k + 8 as the low 16 bits of 2^23 + 0x8888 + sum of 16^j k
+    auto four = [](float2 a, float2 b) {
+        const float f = fmaf(fmaf(fmaf(b.y, 16.0f, b.x), 16.0f, a.y), 16.0f, a.x);
+        return __float_as_uint(8388608.0f + 34952.0f - f);
+    };
+    if (!(left <= 0.499998f * s) && left <= s) {  // near a tie: one step on from past half, and from half to even
+        const float half = 0.5f * s;
+        auto nearest = [&](float& d, float v) {
+            const float e = fmaf(d, s, v), a = fabsf(e);
+            if (a > half || (a == half && (__float_as_uint(magic.x - d) & 1))) d -= copysignf(1.0f, e);
+        };
+#pragma unroll
+        for (int j = 0; j < 4; j++) nearest(d[j].x, v[j].x), nearest(d[j].y, v[j].y);
+    }
+    uint32_t w = __byte_perm(four(d[0], d[1]), four(d[2], d[3]), 0x5410);
+    if (!(left <= s)) w = kv4_codes_div(x, y, s);
     if (!store) return;
     *reinterpret_cast<uint32_t*>(blk + kv4_word_off(hd, is_v, r, g, u)) = w;
     if (u == 0) *reinterpret_cast<uint16_t*>(blk + kv4_scale_off(hd, is_v, r, g)) = __half_as_ushort(sh);

@@ -146,7 +146,7 @@ static PyObject* read_back(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         return pass();
     PyObject *shape = Py_BuildValue("(Lii)", s.dim[0], c.n_kv, c.hd), *device = PyLong_FromLong(dev), *k = NULL, *v = NULL, *r = NULL;
     long long pk, pv;
-    if (shape && device && (k = empty(shape, a[4], device)) && (v = empty(shape, a[4], device)) &&
+    if (shape && device && (k = empty(shape, a[4], device)) && (v = PyObject_CallOneArg(f_empty_like, k)) &&
         int_of(method(k, n_data_ptr), &pk) && int_of(method(v, n_data_ptr), &pv)) {
         Py_BEGIN_ALLOW_THREADS;
         rc = p_read(&c, l, (const int*)s.p, p, (int)s.dim[0], (void*)(uintptr_t)pk, (void*)(uintptr_t)pv, kind, NULL, stream);
