@@ -431,6 +431,40 @@ def test_a_step_captured_and_replayed():
             _check(outs[w][i][:, None], q[w, i][:, None].astype(np.float64), ks, vs, hd ** -0.5, "f32")
 
 
+def test_graphs_of_all_kinds_of_calls_follow_their_inputs():
+    """A warp or a block per sequence, a cut, a chunk in splits and a full one: each
+    captured at short lengths, replayed in turns after q, lengths and cache changed."""
+    from joule_b200 import kv4
+    rng = np.random.default_rng(31)
+    calls = [(300, 1, 8, 8, 64, 250), (20, 1, 8, 2, 128, 700), (60, 1, 16, 4, 128, 1900), (1, 90, 32, 2, 128, 1500),
+             (3, 900, 8, 2, 64, 1000)]
+    made = []
+    for B, T, H, kv, hd, maxT in calls:
+        cache = kv4.kv4_cache(B, 1, kv, hd, maxT)
+        k, v = (_to(rng.standard_normal((B * maxT, kv, hd)), "bf16") for _ in range(2))
+        at = np.arange(B * maxT)
+        kv4.kv4_append(cache, 0, k, v, _i32(at // maxT), _i32(at % maxT))
+        q = _to(rng.standard_normal((B, T, H, hd)), "f32")
+        slots, lens = _i32(rng.permutation(B)), _i32(np.minimum(T, maxT) + np.zeros(B))
+        kw = dict(longest=maxT)
+        kv4.kv4_attention(cache, 0, q, slots, lens, **kw)
+        g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            out = kv4.kv4_attention(cache, 0, q, slots, lens, **kw)
+        made.append((g, out, cache, q, slots, lens, kw, maxT))
+    for turn in range(3):
+        for g, out, cache, q, slots, lens, kw, maxT in made:
+            q.copy_(torch.randn_like(q) * (turn + 1))
+            lens.copy_(torch.randint(0, maxT + 1, lens.shape, device="cuda").int())
+            lens[0] = maxT
+        for m in made:
+            m[0].replay()
+        torch.cuda.synchronize()
+        for g, out, cache, q, slots, lens, kw, maxT in made:
+            assert torch.equal(out, kv4.kv4_attention(cache, 0, q, slots, lens, **kw))
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_compiled_and_interpreted_calls_agree(t):
     """A call with a status word goes through the Python function, one without
