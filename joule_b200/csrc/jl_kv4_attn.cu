@@ -656,7 +656,8 @@ __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args 
         if (cut.start(b1) > last) b1--;
         if (nw == 1) b0 = b1 = w1 + 1;  // (a unit per block)
         else if (b1 <= b0) b0 = b1 = max(w0 / nw + 1, w1 / nw);
-        const int c0 = w0 / nw, head = nw == 1 ? w1 + 1 - w0 : b0 > c0 ? min(w1 + 1, c0 * nw + (int)cut.warps(c0)) - w0 : 0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
+        const int c0 = w0 / nw, first_end = c0 * nw + (int)cut.warps(c0);  // past the first block's warps
+        const int head = nw == 1 ? w1 + 1 - w0 : b0 > c0 ? min(w1 + 1, first_end) - w0 : 0, tail = max(0, w1 + 1 - b1 * nw), n = head + b1 - b0 + tail;
         const int g = blockIdx.y * RB + warp % RB, lanes = 8 / RB, pl = warp / RB;
         const float* ws = static_cast<const float*>(a.ws) + g * HD;
         // warp w0 began the segment: its part 1

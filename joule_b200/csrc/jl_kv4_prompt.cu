@@ -522,35 +522,35 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                     pr_fold<HD>(to, ref, held, LO && nb > kPrFold);
                     pr_part<HD>::stats(held->out)[threadIdx.x] = make_float2(ref, ls);
                 } else {
-                if (LO && nb > kPrFold) pr_unfold<HD>(to, ref, held);
-                const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
-                constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
-                T* st = reinterpret_cast<T*>(qs) + (warp & 3) * 32 * HD;
+                    if (LO && nb > kPrFold) pr_unfold<HD>(to, ref, held);
+                    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                    // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
+                    constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
+                    T* st = reinterpret_cast<T*>(qs) + (warp & 3) * 32 * HD;
 #pragma unroll 1
-                for (int q = 0; q < NG * 4; q++) {
-                    float o[16];
-                    tc_ld16(to + 16 * q, o);
+                    for (int q = 0; q < NG * 4; q++) {
+                        float o[16];
+                        tc_ld16(to + 16 * q, o);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = ls == 0.0f ? 0.0f : o[i] * inv;
+                        for (int i = 0; i < 16; i++) o[i] = ls == 0.0f ? 0.0f : o[i] * inv;
 #pragma unroll
-                    for (int i = 0; i < 16; i += VPC) {
-                        const int p = (16 * q + i) / VPC;
-                        store_piece(st + (lane * CPR + (p ^ (lane & 7))) * VPC, o + i);
+                        for (int i = 0; i < 16; i += VPC) {
+                            const int p = (16 * q + i) / VPC;
+                            store_piece(st + (lane * CPR + (p ^ (lane & 7))) * VPC, o + i);
+                        }
+                        if (a.outT && row < rows)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) a.outT[(size_t)(h * HD + 16 * q + i) * a.outT_ld + orow] = o[i];
                     }
-                    if (a.outT && row < rows)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) a.outT[(size_t)(h * HD + 16 * q + i) * a.outT_ld + orow] = o[i];
-                }
-                __syncwarp();  // (and the warp has taken what `out` held)
+                    __syncwarp();  // (and the warp has taken what `out` held)
 #pragma unroll 4
-                for (int i = lane; i < 32 * CPR; i += 32) {
-                    const int r = i / CPR, p = i % CPR, g = row0 + warp * 32 + r;
-                    if (g >= rows) break;
-                    const long long to_row = (long long)b * a.T + g / gsz;
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (to_row * a.H + kh * gsz + g % gsz) * HD + p * VPC) =
-                        *reinterpret_cast<const uint4*>(st + (r * CPR + (p ^ (r & 7))) * VPC);
-                }
+                    for (int i = lane; i < 32 * CPR; i += 32) {
+                        const int r = i / CPR, p = i % CPR, g = row0 + warp * 32 + r;
+                        if (g >= rows) break;
+                        const long long to_row = (long long)b * a.T + g / gsz;
+                        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (to_row * a.H + kh * gsz + g % gsz) * HD + p * VPC) =
+                            *reinterpret_cast<const uint4*>(st + (r * CPR + (p ^ (r & 7))) * VPC);
+                    }
                 }
             }
         }
