@@ -734,7 +734,8 @@ __global__ void __launch_bounds__(kAttnThreads) k_qk_prep(attn_args a) {
             const int ng = hd / 64, gr = tid / 8 % ng, u = tid % 8, is_v = tid / 8 / ng;
             const float4* src = reinterpret_cast<const float4*>((is_v ? v_s : k_s) + gr * 64 + 8 * u);
             uint8_t* blk = a.kv4.run(slot, a.l, g) + (size_t)(pos / kKv4Rows) * kv4_block_bytes(hd);
-            kv4_store_group(blk, hd, is_v, pos % kKv4Rows, gr, u, src[0], src[1], tid < 16 * ng);
+            const float4 x[2] = {src[0], src[1]};
+            kv4_store_group<1>(blk, hd, is_v, pos % kKv4Rows, gr, u, x, tid < 16 * ng);
         }
         return;
     }

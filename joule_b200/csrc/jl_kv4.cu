@@ -58,33 +58,37 @@ __device__ __forceinline__ void to_fp32(const kv4_eight<__nv_bfloat16>& v, float
 // head by HD / values-per-lane lanes, several rows of a lane in flight. (An index of one
 // flat item per lane took three times the instructions and bound both kernels by
 // issue: 8,179 rows x 16 heads 65 + 47 us under ncu.) Rows in flight in long calls:
-// append 4 (8: 35 us against 26, by registers), read 8 (4: 27 us against 24).
-constexpr int kKvAppendRows = 4, kKvReadRows = 8;
+// append 4 of fp32 at head dim 128 (8 by registers 35 us against 26, 2 27.5), else 2 (4:
+// bf16 27 us against 23, fp32 at head dim 64 16.3 against 14.7), read 8 (4: 27 against 24).
+constexpr int kKvReadRows = 8;
+template <int HD, typename T>
+constexpr int kKvAppendRows = HD * sizeof(T) == 512 ? 4 : 2;
 
-// Append: a lane has one code word (8 values); the 8 lanes of a group reduce its
-// maximum by shuffles and store its record. 8,179 rows of 16 heads of 128: fp32 26 us
-// (23 at the copy rate), bound by HBM and issue alike; bf16 27 us, by issue (some 180
-// instructions for 8 values of each lane).
+// Append: a lane has 32 bytes of a row, W code words (8 values each); the 8 / W lanes of
+// a group reduce its maximum by shuffles and store its record. 8,179 rows of 16 heads of 128: fp32 26 us
+// (23 at the copy rate), bound by HBM and issue alike; bf16 23 us (13), by issue (a word
+// a lane: 27).
 template <int HD, typename T, int STEPS>
 __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, const T* __restrict__ k,
                                                            const T* __restrict__ v, long long ks, long long vs,
                                                            const int* __restrict__ slots,
                                                            const int* __restrict__ positions, int N, int* err) {
-    constexpr int LPR = HD / 8, ROWS = kKvThreads / LPR;  // lanes per row, rows per step
+    constexpr int W = 4 / sizeof(T), LPR = HD / (8 * W), ROWS = kKvThreads / LPR;  // lanes per row, rows per step
     griddep_wait();
     griddep_launch_dependents();
     const int hv = blockIdx.x % (2 * c.KH), chunk = blockIdx.x / (2 * c.KH);
-    const int is_v = hv & 1, h = hv >> 1, w = threadIdx.x % LPR, g = w / 8, u = w % 8;
+    const int is_v = hv & 1, h = hv >> 1, w = threadIdx.x % LPR * W, g = w / 8, u = w % 8;
     const long long stride = is_v ? vs : ks;
     const int n0 = chunk * ROWS * STEPS + threadIdx.x / LPR;
     const T* src = (is_v ? v : k) + h * HD + 8 * w;
-    kv4_eight<T> raw[STEPS];
+    kv4_eight<T> raw[STEPS][W];
     int slot[STEPS], pos[STEPS];
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {  // (rows past the last: the last, not stored)
         const int n = min(n0 + j * ROWS, N - 1);
         slot[j] = __ldg(slots + n), pos[j] = __ldg(positions + n);
-        load8<(STEPS > 1)>(src + n * stride, raw[j]);
+#pragma unroll
+        for (int i = 0; i < W; i++) load8<(STEPS > 1)>(src + n * stride + 8 * i, raw[j][i]);
     }
     uint8_t* base = c.run(0, l, h);
     const size_t per_slot = (size_t)c.L * c.KH * c.nb * kv4_block_bytes(HD);
@@ -93,9 +97,10 @@ __global__ void __launch_bounds__(kKvThreads) k_kv4_append(kv4_dims c, int l, co
         const bool in = n0 + j * ROWS < N, ok = in && (unsigned)slot[j] < (unsigned)c.slots && (unsigned)pos[j] < (unsigned)c.maxT;
         if (in && !ok && hv == 0 && w == 0 && err) atomicOr(err, kErrKvIndex);
         uint8_t* blk = base + (unsigned)slot[j] * per_slot + (size_t)((unsigned)pos[j] / kKv4Rows) * kv4_block_bytes(HD);
-        float4 x, y;
-        to_fp32(raw[j], x, y);
-        kv4_store_group(blk, HD, is_v, pos[j] % kKv4Rows, g, u, x, y, ok);
+        float4 x[2 * W];
+#pragma unroll
+        for (int i = 0; i < W; i++) to_fp32(raw[j][i], x[2 * i], x[2 * i + 1]);
+        kv4_store_group<W>(blk, HD, is_v, pos[j] % kKv4Rows, g, u, x, ok);
     }
 }
 
@@ -227,7 +232,7 @@ template <int HD, typename T>
 int launch_append(const jl::kv4_dims& c, int l, const void* k, const void* v, long long ks, long long vs,
                   const int* slots, const int* positions, int N, int* err, cudaStream_t s) {
     using namespace jl;
-    return launch_rows<HD, T, 8, kKvAppendRows>(k_kv4_append<HD, T, 1>, k_kv4_append<HD, T, kKvAppendRows>, c.KH, N, s, c, l, (const T*)k,
+    return launch_rows<HD, T, 32 / sizeof(T), kKvAppendRows<HD, T>>(k_kv4_append<HD, T, 1>, k_kv4_append<HD, T, kKvAppendRows<HD, T>>, c.KH, N, s, c, l, (const T*)k,
                                  (const T*)v, ks, vs, slots, positions, N, err);
 }
 

@@ -70,8 +70,8 @@ __device__ __forceinline__ float kv4_max_nan(float m, float a, float b) {
     return r;
 }
 
-// Quantises a group of 64 values held by 8 consecutive lanes (lane u of the 8 has
-// word u: values 8u .. 8u + 7, x then y) and stores it as (row r, group g) of block
+// Quantises a group of 64 values held by 8 / W consecutive lanes (a lane has the W words
+// from u on: values 8u .. 8u + 8W - 1) and stores it as (row r, group g) of block
 // `blk` when `store`. A code is the step nearest to the exact x / s, ties to even. Its
 // first guess k is the product with about 1 / s, rounded by adding 1.5 * 2^23 + 8; it
 // stands when what is left, x - k s, is below half a step. That remainder is exact
@@ -83,14 +83,17 @@ __device__ __forceinline__ float kv4_max_nan(float m, float a, float b) {
 // significand). Beyond the record's own rules: a scale that fp16 cannot hold stays at
 // its largest number (values past 7 * 65504 saturate) and a NaN becomes zero, so what
 // the cache holds is always finite. All lanes of the warp call it.
-__device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, int r, int g, int u, float4 x, float4 y,
+template <int W>
+__device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, int r, int g, int u, const float4 (&x)[2 * W],
                                                 bool store) {
-    const float2 v[4] = {make_float2(x.x, x.y), make_float2(x.z, x.w), make_float2(y.x, y.y), make_float2(y.z, y.w)};
+    float2 v[4 * W];
+#pragma unroll
+    for (int j = 0; j < 2 * W; j++) v[2 * j] = make_float2(x[j].x, x[j].y), v[2 * j + 1] = make_float2(x[j].z, x[j].w);
     float amax = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) amax = fmaxf(amax, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
+    for (int j = 0; j < 4 * W; j++) amax = fmaxf(amax, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
 #pragma unroll
-    for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = 4 / W; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     amax = fmaxf(amax, 1e-12f);
     const float seventh = 1.0f / 7.0f, q0 = amax * seventh;  // (an infinity becomes a NaN, and the largest scale)
     const __half sh = __float2half_rn(fminf(fmaf(fmaf(-7.0f, q0, amax), seventh, q0), 65504.0f));
@@ -98,10 +101,10 @@ __device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, 
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     const float2 inv2 = make_float2(inv, inv), s2 = make_float2(s, s), magic = make_float2(12582920.0f, 12582920.0f);
-    float2 d[4];  // -k
+    float2 d[4 * W];  // -k
     float left = s >= 0x1p-21f && s < 65504.0f ? 0.0f : INFINITY;  // (others can be more than 7.5 steps)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < 4 * W; j++) {
         d[j] = __ffma2_rn(__ffma2_rn(v[j], inv2, magic), make_float2(-1.0f, -1.0f), magic);
         const float2 e = __ffma2_rn(d[j], s2, v[j]);
         left = kv4_max_nan(left, e.x, e.y);
@@ -118,13 +121,16 @@ __device__ __forceinline__ void kv4_store_group(uint8_t* blk, int hd, int is_v, 
             if (a > half || (a == half && (__float_as_uint(magic.x - d) & 1))) d -= copysignf(1.0f, e);
         };
 #pragma unroll
-        for (int j = 0; j < 4; j++) nearest(d[j].x, v[j].x), nearest(d[j].y, v[j].y);
+        for (int j = 0; j < 4 * W; j++) nearest(d[j].x, v[j].x), nearest(d[j].y, v[j].y);
     }
-    uint32_t w = __byte_perm(four(d[0], d[1]), four(d[2], d[3]), 0x5410);
-    if (!(left <= s)) w = kv4_codes_div(x, y, s);
-    if (!store) return;
-    *reinterpret_cast<uint32_t*>(blk + kv4_word_off(hd, is_v, r, g, u)) = w;
-    if (u == 0) *reinterpret_cast<uint16_t*>(blk + kv4_scale_off(hd, is_v, r, g)) = __half_as_ushort(sh);
+    const bool divide = !(left <= s);
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        uint32_t w = __byte_perm(four(d[4 * i], d[4 * i + 1]), four(d[4 * i + 2], d[4 * i + 3]), 0x5410);
+        if (divide) w = kv4_codes_div(x[2 * i], x[2 * i + 1], s);
+        if (store) *reinterpret_cast<uint32_t*>(blk + kv4_word_off(hd, is_v, r, g, u + i)) = w;
+    }
+    if (store && u == 0) *reinterpret_cast<uint16_t*>(blk + kv4_scale_off(hd, is_v, r, g)) = __half_as_ushort(sh);
 }
 
 }  // namespace jl

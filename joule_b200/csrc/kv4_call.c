@@ -11,9 +11,9 @@
 
 #include "joule_moe.h"
 
-static PyObject *n_shape, *n_dtype, *n_data_ptr, *n_is_contiguous, *n_get_device, *kw_empty;
+static PyObject *n_shape, *n_dtype, *n_data_ptr, *n_is_contiguous, *n_get_device, *n_new_empty, *kw_dtype;
 /* set by bind(): torch's dtypes and functions, the library's entry points */
-static PyObject *t_u8, *t_i32, *t_types[3], *f_empty, *f_empty_like, *f_device, *f_stream;
+static PyObject *t_u8, *t_i32, *t_types[3], *f_empty_like, *f_device, *f_stream;
 static int (*p_append)(const jl_kv4*, int, const void*, const void*, int, long long, long long, const int*, const int*,
                        int, int*, void*);
 static int (*p_read)(const jl_kv4*, int, const int*, const int*, int, void*, void*, int, int*, void*);
@@ -128,9 +128,10 @@ static PyObject* append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     return PyLong_FromLong(rc);
 }
 
-static PyObject* empty(PyObject* shape, PyObject* dtype, PyObject* device) {
-    PyObject* args[3] = {shape, dtype, device};
-    return PyObject_Vectorcall(f_empty, args, 1, kw_empty);
+/* A tensor on the cache's device (half a microsecond less than torch.empty). */
+static PyObject* empty(PyObject* cache, PyObject* shape, PyObject* dtype) {
+    PyObject* args[3] = {cache, shape, dtype};
+    return PyObject_VectorcallMethod(n_new_empty, args, 2, kw_dtype);
 }
 
 /* read(cache, l, slots, positions, dtype): (code, k, v). */
@@ -144,16 +145,16 @@ static PyObject* read_back(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     if (s.dims != 1 || s.dim[0] < 1 || s.dim[0] > INT_MAX || s.dtype != t_i32 || s.dev != dev ||
         !(p = look_index(a[3], s.dim[0], dev)))
         return pass();
-    PyObject *shape = Py_BuildValue("(Lii)", s.dim[0], c.n_kv, c.hd), *device = PyLong_FromLong(dev), *k = NULL, *v = NULL, *r = NULL;
+    PyObject *shape = Py_BuildValue("(Lii)", s.dim[0], c.n_kv, c.hd), *k = NULL, *v = NULL, *r = NULL;
     long long pk, pv;
-    if (shape && device && (k = empty(shape, a[4], device)) && (v = PyObject_CallOneArg(f_empty_like, k)) &&
+    if (shape && (k = empty(a[0], shape, a[4])) && (v = PyObject_CallOneArg(f_empty_like, k)) &&
         int_of(method(k, n_data_ptr), &pk) && int_of(method(v, n_data_ptr), &pv)) {
         Py_BEGIN_ALLOW_THREADS;
         rc = p_read(&c, l, (const int*)s.p, p, (int)s.dim[0], (void*)(uintptr_t)pk, (void*)(uintptr_t)pv, kind, NULL, stream);
         Py_END_ALLOW_THREADS;
         r = Py_BuildValue("(iOO)", rc, k, v);
     }
-    Py_XDECREF(shape), Py_XDECREF(device), Py_XDECREF(k), Py_XDECREF(v);
+    Py_XDECREF(shape), Py_XDECREF(k), Py_XDECREF(v);
     return r; /* NULL: allocation raised */
 }
 
@@ -179,9 +180,9 @@ static PyObject* attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     PyObject *out = PyObject_CallOneArg(f_empty_like, a[2]), *ws = NULL, *r = NULL;
     long long po = 0, pw = 0;
     if (out && need > 0) {
-        PyObject *size = PyLong_FromLongLong(need), *device = PyLong_FromLong(dev);
-        if (size && device) ws = empty(size, t_u8, device);
-        Py_XDECREF(size), Py_XDECREF(device);
+        PyObject* size = PyLong_FromLongLong(need);
+        if (size) ws = empty(a[0], size, t_u8);
+        Py_XDECREF(size);
     }
     if (out && (need <= 0 || (ws && int_of(method(ws, n_data_ptr), &pw))) && int_of(method(out, n_data_ptr), &po)) {
         Py_BEGIN_ALLOW_THREADS;
@@ -194,18 +195,18 @@ static PyObject* attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     return r;
 }
 
-/* bind(uint8, int32, fp32, fp16, bf16, empty, empty_like, current_device, current_stream, append, read, attn, ws) */
+/* bind(uint8, int32, fp32, fp16, bf16, empty_like, current_device, current_stream, append, read, attn, ws) */
 static PyObject* bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
-    PyObject** keep[9] = {&t_u8, &t_i32, &t_types[JL_F32], &t_types[JL_F16], &t_types[JL_BF16], &f_empty, &f_empty_like, &f_device, &f_stream};
-    if (n != 13) {
-        PyErr_SetString(PyExc_TypeError, "bind takes 13 arguments");
+    PyObject** keep[8] = {&t_u8, &t_i32, &t_types[JL_F32], &t_types[JL_F16], &t_types[JL_BF16], &f_empty_like, &f_device, &f_stream};
+    if (n != 12) {
+        PyErr_SetString(PyExc_TypeError, "bind takes 12 arguments");
         return NULL;
     }
     void* at[4];
     for (int i = 0; i < 4; i++)
-        if (!(at[i] = PyLong_AsVoidPtr(a[9 + i]))) return PyErr_Occurred() ? NULL : pass();
+        if (!(at[i] = PyLong_AsVoidPtr(a[8 + i]))) return PyErr_Occurred() ? NULL : pass();
     p_append = at[0], p_read = at[1], p_attn = at[2], p_ws = at[3];
-    for (int i = 0; i < 9; i++) {
+    for (int i = 0; i < 8; i++) {
         Py_INCREF(a[i]);
         Py_XSETREF(*keep[i], a[i]);
     }
@@ -225,7 +226,8 @@ PyMODINIT_FUNC PyInit__kv4_call(void) {
     n_data_ptr = PyUnicode_InternFromString("data_ptr");
     n_is_contiguous = PyUnicode_InternFromString("is_contiguous");
     n_get_device = PyUnicode_InternFromString("get_device");
-    kw_empty = Py_BuildValue("(ss)", "dtype", "device");
-    if (!n_shape || !n_dtype || !n_data_ptr || !n_is_contiguous || !n_get_device || !kw_empty) return NULL;
+    n_new_empty = PyUnicode_InternFromString("new_empty");
+    kw_dtype = Py_BuildValue("(s)", "dtype");
+    if (!n_shape || !n_dtype || !n_data_ptr || !n_is_contiguous || !n_get_device || !n_new_empty || !kw_dtype) return NULL;
     return PyModule_Create(&module);
 }

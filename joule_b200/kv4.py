@@ -59,7 +59,7 @@ def _bind() -> None:
         raise FileNotFoundError("joule_b200/_kv4_call.so is missing: run `python -m joule_b200.build`") from e
     entries = [ctypes.cast(f, ctypes.c_void_p).value
                for f in (dll.jl_kv4_append, dll.jl_kv4_read, dll.jl_kv4_attn, dll.jl_kv4_attn_ws)]
-    _kv4_call.bind(torch.uint8, torch.int32, torch.float32, torch.float16, torch.bfloat16, torch.empty, torch.empty_like,
+    _kv4_call.bind(torch.uint8, torch.int32, torch.float32, torch.float16, torch.bfloat16, torch.empty_like,
                    _current_device, _raw_stream, *entries)
     _dll, _call = dll, _kv4_call
 
