@@ -297,7 +297,7 @@ extern "C" int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, lon
     if (B < 0 || T < 1 || H < 1 || H % d.KH || dtype < JL_F32 || dtype > JL_BF16 || !std::isfinite(scale) ||
         longest < 0 || longest > d.maxT)
         return JL_ERR_INVALID;
-    if ((long long)B * T > INT_MAX / H) return JL_ERR_INVALID;
+    if ((long long)B * T > INT_MAX / H || H > INT_MAX / d.hd) return JL_ERR_INVALID;  // rows, and a row's values
     if (B == 0) return JL_OK;
     const long long unit = dtype == JL_F32 ? 4 : 8, row = (long long)H * d.hd;
     if (!q || !slots || !lens || !out || !aligned16(q) || !aligned16(out) || q_stride % unit ||

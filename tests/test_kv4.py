@@ -94,7 +94,7 @@ def test_bad_arguments_are_refused(dll):
                                  at(longest=-1), at(longest=129), at(B=-1), at(T=0), at(H=3), at(H=0),
                                  at(scale=float("nan")), at(scale=float("inf")), at(out=None), at(out=(1 << 20) + 8),
                                  at(out=4096), at(out=4096 + 2 * 512 * 4 - 16), at(qs=1 << 20, out=1 << 20),
-                                 at(B=2**20, T=2**20)))
+                                 at(B=2**20, T=2**20), at(B=1, H=2**25, out=1 << 40)))
     ws = dll.jl_kv4_attn_ws
     assert all(x == -1 for x in (ws(r, 2, 1, 3, 0), ws(r, 2, 0, 4, 0), ws(r, -1, 1, 4, 0), ws(r, 2, 1, 4, -1),
                                  ws(r, 2, 1, 4, 129), ws(r, 2**20, 2**20, 4, 0)))
