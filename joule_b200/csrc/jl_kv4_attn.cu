@@ -125,8 +125,10 @@ constexpr int kKvWarps = 12;  // warps per block, one block per SM (168 register
 template <int HD>
 struct kv4_smem {
     static constexpr int UNIT = kv4_block_bytes(HD);
-    static constexpr int stat = kKvWarps * kKvRing * UNIT;  // reference, sum [warps][2][8] of the block's sum
-    static constexpr int total = stat + kKvWarps * 2 * kKvTile * 4;
+    // the warps' rings, then (reference, sum) [warps][2][8] of the block's sum
+    __host__ __device__ static constexpr int stat(int warps) { return warps * kKvRing * UNIT; }
+    static constexpr int bytes(int warps) { return stat(warps) + warps * 2 * kKvTile * 4; }
+    static constexpr int total = bytes(kKvWarps);
     static_assert(kKvRing * UNIT >= kKvTile * HD * 4, "a warp's ring holds its sums");
 };
 
@@ -407,12 +409,14 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
 // of two whole cache blocks, filled by 16-byte asynchronous copies (17 instructions a
 // block; a bulk copy held its issuing warp for hundreds of ns); no barrier between
 // warps but for the sum of a block that is inside one segment.
-// BLOCK: a segment per block, whose warps share it and join here; no cut, no second kernel.
+// BLOCK: a segment per block (of 12 warps or, two and three to an SM, of 6 and 4), whose
+// warps share it and join here; no cut, no second kernel.
 template <int HD, typename T, bool BLOCK>
 __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l, jl_kv4_attn_args a, int R, int whole) {
     extern __shared__ __align__(128) uint8_t smem[];
     using SM = kv4_smem<HD>;
-    constexpr int UNIT = SM::UNIT, NG = HD / 64, NW = kKvWarps;
+    constexpr int UNIT = SM::UNIT, NG = HD / 64;
+    const int NW = BLOCK ? blockDim.x >> 5 : kKvWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kKvRing * UNIT;
     griddep_wait();
@@ -556,7 +560,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             } else {
                 float* part = joined ? reinterpret_cast<float*>(ring)
                                      : static_cast<float*>(a.ws) + ((size_t)(blockIdx.x * nw + warp) * 2 + from_start) * kv4_part_floats(HD);
-                float* ml = joined ? reinterpret_cast<float*>(smem + SM::stat) + warp * 2 * kKvTile : part + kKvTile * HD;
+                float* ml = joined ? reinterpret_cast<float*>(smem + SM::stat(NW)) + warp * 2 * kKvTile : part + kKvTile * HD;
 #pragma unroll
                 for (int cc = 0; cc < 2; cc++) {
 #pragma unroll
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
     // the warps' sums, in their order
     const int joining = (BLOCK ? NW : used) * 32;
     asm volatile("bar.sync 1, %0;" ::"r"(joining) : "memory");
-    const float* ml = reinterpret_cast<const float*>(smem + SM::stat);
+    const float* ml = reinterpret_cast<const float*>(smem + SM::stat(NW));
     float* part = static_cast<float*>(a.ws) +
                   ((size_t)blockIdx.x * nw * 2 + (c0 == seg0)) * kv4_part_floats(HD);
     for (int x = threadIdx.x; x < kKvTile * HD / 4; x += joining) {
@@ -753,7 +757,8 @@ int sm_count() {
 
 int row_tiles(const jl::kv4_dims& c, int T, int H) { return (T * (H / c.KH) + jl::kKvTile - 1) / jl::kKvTile; }
 
-// How a call is run: kernel, splits of a unit (tcgen05 form), workspace.
+// How a call is run: kernel, splits of a unit (tcgen05 form) or blocks to an SM (block
+// form), workspace.
 enum class kv4_form { whole, block, cut, prompt, none };
 struct kv4_plan {
     kv4_form form;
@@ -788,17 +793,24 @@ kv4_plan plan(const jl::kv4_dims& c, int B, int T, int H, int longest, int sms) 
     if (segs > INT_MAX || segs * nb > INT_MAX) return {kv4_form::none, 0, 0};  // the cut counts in 32 bits
     // Three ways to share the segments' blocks out, with what they take in fp32 at head
     // dim 128, in units of 0.35 us (a block alone takes a warp 2 us, with all warps busy 4):
-    // a warp per segment, a thread block per segment, or all blocks cut evenly and a second
-    // kernel that adds up. 32/4 heads, 1 / 32 / 64 / 256 sequences, us: over 128 positions
-    // 7.8 / 8.6 / 9.1 / 12.9 by warps, 6.2 / 6.8 / 12.4 / 42 by blocks, over 512 8.4 / 12.6 /
-    // 17.5 / 35 cut, 6.8 / 7.4 / 13.7 / 46 by blocks, over 2,048 9.2 / 20.5 / 30 / 86 and
-    // 15 / 16 / 30 / 110. Lengths are taken as even up to 3/4 of the longest for the cut,
-    // whose work follows them; a block of head dim 64 takes half.
+    // a warp per segment, a thread block per segment (one to three to an SM), or all blocks
+    // cut evenly and a second kernel that adds up. 32/4 heads, 8 / 32 / 64 / 256 sequences,
+    // us: over 128 positions 8.4 / 8.6 / 9.1 / 12.9 by warps, 5.6 / 5.9 / 6.4 / 18.5 by
+    // blocks, over 512 11.6 / 12.6 / 17.5 / 35 cut, 7.0 / 7.3 / 11.3 / 32 by blocks, over
+    // 2,048 12.7 / 20.5 / 30 / 86 and 15.5 / 16 / 27 / 85 (lengths spread evenly: 11.5 / 16.4 /
+    // 22 / 61 and 15 / 15.5 / 26 / 64). The cut's work follows the lengths and is counted at
+    // 3/4 of the longest; a block of head dim 64 takes half.
     const double per_sm = (double)segs / sms, work = c.hd == 64 ? 0.5 * nb : nb, u = per_sm * work;
     const double whole = 10 + work * (6 + std::min(per_sm, 12.0) / 2) * std::max(1.0, std::ceil(per_sm / kKvWarps));
-    const double block = (double)((segs - 1) / sms + 1) * (12 + work), cut = 24 + std::min(9.0, 6 * u) + 0.75 * u;
-    if (longest <= 256) return {whole < block ? kv4_form::whole : kv4_form::block, 1, 0};
-    if (block < cut) return {kv4_form::block, 1, 0};
+    const double cut = 24 + std::min(9.0, 6 * u) + 0.75 * u;
+    double block = INFINITY;
+    int to_sm = 1;  // blocks that share an SM take longer each, and fewer of them wait
+    for (int k = 1; k <= 3; k++) {
+        const double t = (double)((segs - 1) / ((long long)k * sms) + 1) * (12 + k * work);
+        if (t < block) block = t, to_sm = k;
+    }
+    if (longest <= 256 && whole < block) return {kv4_form::whole, 1, 0};
+    if (longest <= 256 || block < cut) return {kv4_form::block, to_sm, 0};
     // two parts for each warp that has blocks (blocks x warps of a cut: below its units + blocks)
     const long long warps = std::min<long long>((long long)sms * kKvWarps, 2 * segs * nb);
     return {kv4_form::cut, 1, warps * 2 * kv4_part_floats(c.hd) * (long long)sizeof(float)};
@@ -821,25 +833,27 @@ int attn_attrs() {
 }
 
 template <int HD, typename T>
-int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, kv4_form form, int sms, cudaStream_t s) {
+int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, const kv4_plan& p, int sms, cudaStream_t s) {
     using namespace jl;
     const int R = row_tiles(c, a.T, a.H);
     const unsigned segs = (unsigned)((long long)a.B * R * c.KH);
-    const dim3 threads(kKvWarps * 32);
-    const size_t smem = kv4_smem<HD>::total;
-    if (form == kv4_form::block) return launch(k_kv4_attn<HD, T, true>, dim3(segs), threads, smem, s, c, l, a, R, 0);
-    const int rc = launch(k_kv4_attn<HD, T, false>, dim3(sms), threads, smem, s, c, l, a, R, (int)(form == kv4_form::whole));
-    if (rc || form == kv4_form::whole) return rc;
+    if (p.form == kv4_form::block) {
+        const int warps = kKvWarps / p.S;
+        return launch(k_kv4_attn<HD, T, true>, dim3(segs), dim3(warps * 32), (size_t)kv4_smem<HD>::bytes(warps), s, c, l, a, R, 0);
+    }
+    const int rc = launch(k_kv4_attn<HD, T, false>, dim3(sms), dim3(kKvWarps * 32), (size_t)kv4_smem<HD>::total, s, c, l, a, R,
+                          (int)(p.form == kv4_form::whole));
+    if (rc || p.form == kv4_form::whole) return rc;
     const int RB = segs >= (unsigned)sms ? 8 : segs * 4 >= (unsigned)sms ? 2 : 1, per = (int)((segs - 1) / (4 * sms) + 1);
     if (per == 1) return launch(k_kv4_merge<HD, T, false>, dim3(segs, kKvTile / RB), dim3(256), 0, s, c, a, R, sms, RB, 1);
     return launch(k_kv4_merge<HD, T, true>, dim3((segs - 1) / per + 1), dim3(256), 0, s, c, a, R, sms, 8, per);
 }
 
 template <int HD>
-int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, kv4_form form, int sms, cudaStream_t s) {
-    if (a.dtype == JL_F32) return launch_t<HD, float>(c, l, a, form, sms, s);
-    if (a.dtype == JL_F16) return launch_t<HD, __half>(c, l, a, form, sms, s);
-    return launch_t<HD, __nv_bfloat16>(c, l, a, form, sms, s);
+int launch_hd(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, const kv4_plan& p, int sms, cudaStream_t s) {
+    if (a.dtype == JL_F32) return launch_t<HD, float>(c, l, a, p, sms, s);
+    if (a.dtype == JL_F16) return launch_t<HD, __half>(c, l, a, p, sms, s);
+    return launch_t<HD, __nv_bfloat16>(c, l, a, p, sms, s);
 }
 
 }  // namespace
@@ -867,5 +881,5 @@ int jl_launch_kv4_attn(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, 
         return r ? r : attn_attrs<128>();
     });
     if (rc) return rc;
-    return c.hd == 64 ? launch_hd<64>(c, l, a, p.form, sms, s) : launch_hd<128>(c, l, a, p.form, sms, s);
+    return c.hd == 64 ? launch_hd<64>(c, l, a, p, sms, s) : launch_hd<128>(c, l, a, p, sms, s);
 }
