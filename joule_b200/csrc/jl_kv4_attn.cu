@@ -271,10 +271,8 @@ __device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, f
 
 // Weights of positions r0 .. r0 + 15 from their scores, and the weighted values
 // onto the sums. V's scale multiplies the weight in fp32. MASK: row g does not see
-// positions from n on (in the block's numbering); those may hold any scale. LO: the
-// weights' lo parts too; without them a weight is off by 2^-12 of itself at most,
-// random from weight to weight, which a 16-bit output (2^-11, 2^-8) does not show.
-template <int HD, bool MASK, bool LO>
+// positions from n on (in the block's numbering); those may hold any scale.
+template <int HD, bool MASK>
 __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], float ref, int n) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -294,8 +292,7 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
                 if (r0 + 8 * h + 2 * t >= n) w.x = 0.0f;
                 if (r0 + 8 * h + 2 * t + 1 >= n) w.y = 0.0f;
             }
-            if (LO) split2(w, bh[gr][h], bl[gr][h]);
-            else bh[gr][h] = h2bits(__float22half2_rn(w));
+            split2(w, bh[gr][h], bl[gr][h]);
         }
     }
     // thread (g, t) unpacks values 8 g .. 8 g + 7 of each group at positions 2t, 2t + 1, 2t + 8, 2t + 9
@@ -324,44 +321,36 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
                 f[gr][i][2] = code_even(i ? y >> 8 : y), f[gr][i][3] = code_odd(i ? y >> 8 : y);
             }
         }
-        if constexpr (!LO) {
+        // The instruction's sums are cut off, not rounded: 16 positions start from zero and
+        // are added here, or a long run's outputs shrink (by 1.3e-6 of themselves after 18
+        // blocks, and on with the length).
+        float acc[NG][2][4];
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++)
+        for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    mma16816(st.o[gr][2 * q + i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bh[gr][0], bh[gr][1]);
-        } else {
-            // The instruction's sums are cut off, not rounded: 16 positions start from zero and
-            // are added here, or a long run's outputs shrink (by 1.3e-6 of themselves after 18
-            // blocks, and on with the length).
-            float acc[NG][2][4];
+            for (int i = 0; i < 2; i++)
+                mma16816_0(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bl[gr][0], bl[gr][1]);
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++)
+        for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    mma16816_0(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bl[gr][0], bl[gr][1]);
+            for (int i = 0; i < 2; i++)
+                mma16816(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bh[gr][0], bh[gr][1]);
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++)
+        for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    mma16816(acc[gr][i], f[gr][i][0], f[gr][i][1], f[gr][i][2], f[gr][i][3], bh[gr][0], bh[gr][1]);
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    float (&o)[4] = st.o[gr][2 * q + i];
-                    const float2 x0 = __fadd2_rn(make_float2(o[0], o[1]), make_float2(acc[gr][i][0], acc[gr][i][1]));
-                    const float2 x1 = __fadd2_rn(make_float2(o[2], o[3]), make_float2(acc[gr][i][2], acc[gr][i][3]));
-                    o[0] = x0.x, o[1] = x0.y, o[2] = x1.x, o[3] = x1.y;
-                }
-        }
+            for (int i = 0; i < 2; i++) {
+                float (&o)[4] = st.o[gr][2 * q + i];
+                const float2 x0 = __fadd2_rn(make_float2(o[0], o[1]), make_float2(acc[gr][i][0], acc[gr][i][1]));
+                const float2 x1 = __fadd2_rn(make_float2(o[2], o[3]), make_float2(acc[gr][i][2], acc[gr][i][3]));
+                o[0] = x0.x, o[1] = x0.y, o[2] = x1.x, o[3] = x1.y;
+            }
     }
 }
 
 // One block (j0 = its first position's number): rows see all positions below n_min
 // and none from n_max on. A block that all rows see whole is one stretch of code
 // with one branch; others go by 16 positions.
-template <int HD, bool LO>
+template <int HD>
 __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_min, int n_max) {
     constexpr int NG = HD / 64;
     const int lane = threadIdx.x & 31, t = lane & 3;
@@ -385,7 +374,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
         if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
         const float ref = st.ref == -INFINITY ? 0.0f : -st.ref;
 #pragma unroll
-        for (int k = 0; k < 4; k++) kv4_values<HD, false, LO>(st, blk, 16 * k, s[k], ref, 0);
+        for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], ref, 0);
         return;
     }
     const int n = st.n - j0;
@@ -400,7 +389,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
         }
         const float mx = fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[1].x, s[1].y));
         if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
-        kv4_values<HD, true, LO>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
+        kv4_values<HD, true>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
     }
 }
 
@@ -526,7 +515,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         cp_async_wait<kKvRing - 1>();  // this unit's copies, by every lane
         __syncwarp();
         const int j0 = co.j * kKvUnit;
-        if (j0 < n_max) kv4_block<HD, sizeof(T) == 4>(st, ring + i % kKvRing * UNIT, j0, n_min, n_max);
+        if (j0 < n_max) kv4_block<HD>(st, ring + i % kKvRing * UNIT, j0, n_min, n_max);
         __syncwarp();
         issue();
         const bool ends = co.j == co.nu - 1;

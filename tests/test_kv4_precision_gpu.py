@@ -1,0 +1,130 @@
+"""The digits of the 4-bit cache's attention, against its definition in 64 bits
+over the values that the cache holds (read back, which is exact).
+
+With e = 2^-24. Scores: as in tests/test_kv4_gpu.py, |ds| <= scale * (16 + 4 (hd + 16)) e
+(|q| . |k|) + 8 e |s|. What a weight is off by is measured against the sum that it is
+part of: M = sum_t p_t amax_t, p the exact weights and amax_t the largest value of the
+position's group of 64, because a product of a weight and a scale is rounded before
+the code multiplies it. Weights times scales are held in 22 bits, sums in fp32, so an
+output is off by at most (4 |ds| + (2 n + 64) e) M plus half a step of its type. The
+roundings being independent, the root mean square of error / M over all outputs is
+held to RMS = 64 e max(1, max|s|).
+
+Results in 16 bits are the nearest to a value that is off by that much. One of them
+differs from the nearest to the exact value only where that value lies within the
+error of the middle of two steps, so of many results at most a share 2 RMS M / step each
+does, plus five standard deviations of their count.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+E = 2.0 ** -24
+
+
+def _i32(x):
+    return torch.as_tensor(np.asarray(x, np.int32)).cuda()
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _cache(rows, maxT=None):
+    """A cache of the sequences' rows [(k, v)] (each [n, kv, hd] fp32), slot b for sequence b."""
+    from joule_b200 import kv4
+    kv, hd = rows[0][0].shape[1:]
+    cache = kv4.kv4_cache(len(rows), 1, kv, hd, maxT or max(max(k.shape[0] for k, _ in rows), 1))
+    cache.random_(0, 256)
+    for b, (k, v) in enumerate(rows):
+        n = k.shape[0]
+        if n:
+            kv4.kv4_append(cache, 0, k, v, _i32([b] * n), _i32(range(n)))
+    return cache
+
+
+def _held(cache, slot, n):
+    from joule_b200 import kv4
+    k, v = kv4.kv4_read(cache, 0, _i32([slot] * n), _i32(range(n)))
+    return k.double(), v.double()
+
+
+def _exact(q, k, v, scale, rows=None):
+    """q [T, H, hd] over k, v [n, kv, hd] (64 bits): out, M, the bound of |ds| [., H, .]
+    of the given rows of T, and the largest |score|."""
+    T, H, hd = q.shape
+    n, kv = k.shape[:2]
+    rows = torch.arange(T, device="cuda") if rows is None else rows
+    out, M, ds = (torch.zeros(len(rows), H, hd, dtype=torch.float64, device="cuda") for _ in range(3))
+    top = 0.0
+    amax = v.unflatten(-1, (-1, 64)).abs().amax(-1, keepdim=True).expand(n, kv, hd // 64, 64).flatten(-2)
+    for h in range(H):
+        g = h // (H // kv)
+        for a in range(0, len(rows), 64):
+            r = rows[a:a + 64]
+            x = q[r, h].double()
+            s = scale * (x @ k[:, g].T)
+            seen = torch.arange(n, device="cuda")[None] < (n - T + 1 + r)[:, None]
+            some = seen.any(1)
+            s = torch.where(seen, s, -math.inf)
+            p = torch.where(some[:, None], torch.softmax(torch.where(some[:, None], s, 0.0), -1), 0.0)
+            out[a:a + 64, h] = p @ v[:, g]
+            M[a:a + 64, h] = p @ amax[:, g]
+            big = torch.where(seen, s.abs(), 0.0).amax()
+            ab = torch.where(seen, x.abs() @ k[:, g].abs().T, 0.0).amax(1)
+            ds[a:a + 64, h] = (abs(scale) * (16 + 4 * (hd + 16)) * E * ab + 8 * E * big)[:, None]
+            top = max(top, float(big))
+    return out, M, ds, top
+
+
+def _step_of(x, t):
+    """The distance of the type's numbers around x."""
+    e = torch.frexp(x.abs().clamp_min(1e-30))[1].double() - 1
+    bits, low = {"f16": (10, -14), "bf16": (7, -126)}[t]
+    return torch.exp2(e.clamp_min(low) - bits)
+
+
+def _nearest(got, want, M, ds, top, n, t):
+    """16-bit results are the nearest ones but for the share that the bound allows."""
+    step = _step_of(want, t)
+    err = (got.double() - want).abs()
+    assert not (err > step / 2 * (1 + 2.0 ** -20) + (4 * ds + (2 * n + 64) * E) * M).any()
+    share = (2 * 64 * E * max(1.0, top) * M / step).clamp_max(1.0)
+    off = (got != want.to(DT[t])).double()
+    allowed = share.sum().item()
+    assert off.sum().item() <= allowed + 5 * math.sqrt(allowed) + 3, (off.sum().item(), allowed, off.numel())
+
+
+# ---------------------------------------------------------------------------
+# 16-bit calls
+
+STEPS16 = [  # B, T, H, kv, hd, lens: a warp per sequence and head, a block, a cut, drafts
+    (300, 1, 8, 8, 64, [1 + (31 * b) % 40 for b in range(300)]), (8, 1, 32, 4, 128, [9 + 5 * b for b in range(8)]),
+    (40, 1, 16, 4, 128, [(211 * b) % 1501 for b in range(40)]), (5, 5, 10, 2, 64, [40, 5, 7, 30, 21]),
+]
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", STEPS16)
+def test_16_bit_results_are_the_nearest(B, T, H, kv, hd, lens, t):
+    """q, weights and sums of a 16-bit call have as many digits as those of a fp32 one:
+    over values of one sign (outputs of the size of M) the results are the exact
+    ones rounded once."""
+    from joule_b200 import kv4
+    g = _gen(B + T)
+    rows = [(torch.randn(n, kv, hd, device="cuda", generator=g), torch.rand(n, kv, hd, device="cuda", generator=g) + 0.5)
+            for n in lens]
+    cache = _cache(rows)
+    q = (torch.randn(B, T, H, hd, device="cuda", generator=g) * 0.5).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32(range(B)), _i32(lens))
+    parts = [_exact(q[b], *_held(cache, b, n), hd ** -0.5) for b, n in enumerate(lens) if n]
+    at = [b for b, n in enumerate(lens) if n]
+    want, M, ds = (torch.cat([p[i] for p in parts]) for i in range(3))
+    _nearest(torch.cat([got[b] for b in at]), want, M, ds, max(p[3] for p in parts), max(lens), t)
