@@ -5,8 +5,9 @@
 // one (sequence, kv head) form tiles of 128, two of them per block. Per cache
 // block of 64 positions and tile: S = q K^T, softmax by the thread that owns the
 // row (= TMEM lane), O += P V, both products on the tensor cores with fp32 sums
-// in TMEM. Codes enter as n - 8, which fp16 holds exactly; q and the weights in
-// fp32 calls as hi and lo parts (22 bits), two instructions onto the same sums.
+// in TMEM. Codes enter as n - 8, which fp16 holds exactly, as it does a 16-bit q
+// (down to 2^-34 of a row's largest value); q and the weights in fp32 calls are hi
+// and lo parts (22 bits), two instructions onto the same sums.
 // K's scales multiply the finished sums of a 64-value group (one accumulator per
 // group), V's the weights of a group, both in fp32. The exponents' reference
 // moves only when a weight times its scale would pass 2^15 (jl_kv4_dev.cuh), and
@@ -29,6 +30,7 @@
 // shared memory) and by the softmax's issue slots in 16 bits. 2,047 rows of 32/4 heads
 // of 128 over 4,100 positions, fp32: 313 us; 123 at the measured bf16 rate.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "jl_internal.h"
@@ -136,10 +138,12 @@ __device__ __forceinline__ float4 load4(const T* p) {
     return make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
 }
 
-// The warp's 32 q rows, scaled to base-2 scores and by a power of two each (the
-// largest value in [2^10, 2^11)), into the operand's hi and lo parts from row r0 on;
-// returns the inverse of the power of row `lane`. HD / 4 lanes read a row (a row per
-// thread touched 32 lines a load and took 13 us a block). src(i): row i.
+// The warp's 32 q rows, by a power of two each (the largest value in [2^10, 2^11)) and
+// the scale's sign, into the operand from row r0 on: 16-bit values exactly, fp32 ones as
+// hi and lo parts. Returns what makes base-2 scores of row `lane`'s sums: the inverse of
+// its power times |scale| log2 e (not 0, which would undo a masked score of -infinity).
+// HD / 4 lanes read a row (a row per thread touched 32 lines a load and took 13 us a
+// block). src(i): row i.
 template <int HD, bool LO, typename T, typename F>
 __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int r0) {
     constexpr int LPR = HD / 4, RPW = 32 / LPR, ROWS = 8;  // rows of a lane in flight
@@ -154,14 +158,14 @@ __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             const int row = i0 + i * RPW + lane / LPR;
-            const float k = scale * 1.4426950408889634f;
-            float4 y = make_float4(x[i].x * k, x[i].y * k, x[i].z * k, x[i].w * k);
+            float4 y = x[i];
             float mx = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
 #pragma unroll
             for (int o = LPR / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             int e = (int)(__float_as_uint(mx) >> 23);
             e = min(max(e, 11), 253);
-            const float inv = __uint_as_float((uint32_t)(264 - e) << 23), fr = __uint_as_float((uint32_t)(e - 10) << 23);
+            const float inv = copysignf(__uint_as_float((uint32_t)(264 - e) << 23), scale);
+            const float fr = __uint_as_float((uint32_t)(e - 10) << 23);
 #pragma unroll
             for (int q = 0; q < RPW; q++) {
                 const float fq = __shfl_sync(0xffffffffu, fr, q * LPR);
@@ -179,7 +183,7 @@ __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int
             if (LO) *reinterpret_cast<uint2*>(p + SM::QTILE) = lo;
         }
     }
-    return f;
+    return fminf(fmaxf(f * (fabsf(scale) * 1.4426950408889634f), FLT_MIN), FLT_MAX);
 }
 
 // 16 bytes of values.

@@ -128,3 +128,45 @@ def test_16_bit_results_are_the_nearest(B, T, H, kv, hd, lens, t):
     at = [b for b, n in enumerate(lens) if n]
     want, M, ds = (torch.cat([p[i] for p in parts]) for i in range(3))
     _nearest(torch.cat([got[b] for b in at]), want, M, ds, max(p[3] for p in parts), max(lens), t)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("T,H,kv,lens,size", [(700, 16, 4, [720, 705], 4.0), (700, 16, 4, [720, 705], 1.5), (40, 32, 2, [3000, 2999], 4.0)])
+def test_q_of_a_16_bit_prompt_is_not_rounded(T, H, kv, lens, size, t):
+    """A 16-bit q is exact in the product of the scores whatever the scale: its error is
+    that of sums of hd products, 16 at a time, each cut off at 2 e of the largest score at
+    most: 16 e in all. The norm of the results' errors is that of the exact results rounded
+    once and of weights off by so much (and by 64 e as they are in all calls)."""
+    from joule_b200 import kv4
+    g, hd, B, scale = _gen(T), 128, len(lens), 0.0931
+    rows = [tuple(torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2)) for n in lens]
+    cache = _cache(rows)
+    q = (torch.randn(B, T, H, hd, device="cuda", generator=g) * size).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32(range(B)), _i32(lens), scale=scale)
+    parts = [_exact(q[b], *_held(cache, b, n), scale) for b, n in enumerate(lens)]
+    want, M = (torch.cat([p[i] for p in parts]) for i in range(2))
+    top = max(p[3] for p in parts)
+    once = (want.to(DT[t]).double() - want).norm()
+    err = (got.flatten(0, 1).double() - want).norm()
+    assert err <= once + (64 + 16 * top) * E * M.norm(), (err / want.norm(), once / want.norm(), top)
+
+
+@pytest.mark.parametrize("T", [1, 9, 720])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-42, 3e-39, -1e-30, 1e30])
+def test_any_finite_scale(T, t, scale):
+    """Scales of either sign, of zero, and of the ends of fp32's range, with q so large
+    and so small that the scores are ordinary or vanish."""
+    from joule_b200 import kv4
+    g, n, kv, hd, H = _gen(T), 900, 2, 64, 32
+    k, v = (torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2))
+    cache = _cache([(k, v)])
+    size = min(max(0.3 / abs(scale), 1e-30), 1e30) if scale else 1.0
+    size = min(max(size, 2e-4), 2e3) if t == "f16" else size
+    q = (torch.randn(1, T, H, hd, device="cuda", generator=g) * size).to(DT[t])
+    if t == "f16" and scale == 1e30:
+        q.zero_()
+    got = kv4.kv4_attention(cache, 0, q, _i32([0]), _i32([n]), scale=scale)
+    want, M, ds, top = _exact(q[0], *_held(cache, 0, n), float(np.float32(scale)))
+    half = _step_of(want, t) / 2 * (1 + 2.0 ** -20) if t == "f16" else E * want.abs()
+    assert not ((got[0].double() - want).abs() > half + (4 * ds + (2 * n + 64) * E) * M).any()
