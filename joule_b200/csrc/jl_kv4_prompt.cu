@@ -6,8 +6,8 @@
 // block of 64 positions and tile: S = q K^T, softmax by the thread that owns the
 // row (= TMEM lane), O += P V, both products on the tensor cores with fp32 sums
 // in TMEM. Codes enter as n - 8, which fp16 holds exactly, as it does a 16-bit q
-// (down to 2^-34 of a row's largest value); q and the weights in fp32 calls are hi
-// and lo parts (22 bits), two instructions onto the same sums.
+// (down to 2^-34 of a row's largest value); a fp32 q and the weights are hi and lo
+// parts (22 bits), two instructions onto the same sums.
 // K's scales multiply the finished sums of a 64-value group (one accumulator per
 // group), V's the weights of a group, both in fp32. The exponents' reference
 // moves only when a weight times its scale would pass 2^15 (jl_kv4_dev.cuh), and
@@ -41,13 +41,14 @@ namespace jl {
 
 constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 12 * 32, kPrUnpack = 3;  // unpacking warps
 // The tensor cores' sums are cut off, not rounded: over n blocks they come out short by
-// about 1e-7 n of themselves. In fp32 calls the sums therefore move to the rows of `out`
-// every kPrFold blocks, which hold them until the end, and TMEM starts anew. 2,047 rows
-// of 32/4 heads of 128 over 4,100 positions: error 1.6e-6 and 309 us (never: 7.4e-6,
-// 264 us; every 12: 2.0e-6, every 16: 2.5e-6); over 23,000: 1.9e-6 (never: 4.7e-5).
-// 16-bit calls have half the instructions per block and no room in `out`: their sums
-// stay in TMEM and are short by half a step of fp16 after some 480,000 positions.
-constexpr int kPrFold = 8;
+// about 1e-7 n of themselves. The sums therefore move to the rows of `out` (16-bit calls:
+// their lower halves; the upper ones to shared memory) every kPrFold blocks, which hold
+// them until the end, and TMEM starts anew. fp32, 2,047 rows of 32/4 heads of 128 over
+// 4,100 positions: error 1.6e-6 and 309 us (never: 7.4e-6, 264 us; every 12: 2.0e-6, every
+// 16: 2.5e-6); over 23,000: 1.9e-6 (never: 4.7e-5). In 16-bit calls 32 blocks' 3e-6 are
+// far below a step of the output.
+template <bool F32>
+constexpr int kPrFold = F32 ? 8 : 32;
 constexpr int kPrCore = 144;  // bytes between V's core matrices (128 of data: stores without bank conflicts)
 
 struct pr_bars {
@@ -59,27 +60,59 @@ struct pr_bars {
 };
 
 struct pr_held {
-    float* out;
-    int H, gsz, row0, rows;  // out: the sequence's first token, the kv head's first head
+    void* out;               // the sequence's first token, the kv head's first head
+    int H, gsz, row0, rows;
     float ref[kPrPair];      // of what a row's places hold
+    template <typename P>    // P: what four values of a row are there
     struct place {
-        float4* p;
+        P* p;
         int left, run, rest, gap;  // pieces left in the run; a run's; of a step past whole runs; between runs
         long long step;
-        __device__ float4* next() {
-            float4* at = p;
+        __device__ P* next() {
+            P* at = p;
             p += step;
             if ((left -= rest) <= 0) left += run, p += gap;
             return at;
         }
     };
     __device__ bool mine() const { return row0 + (int)threadIdx.x < rows; }
-    template <int HD>
-    __device__ place first() const {
+    template <int HD, typename P>
+    __device__ place<P> first() const {
         const int r0 = row0 + (int)(threadIdx.x & ~31u), nv = min(32, rows - r0), run = gsz * (HD / 4), gap = (H - gsz) * (HD / 4);
         const int at = r0 % gsz * (HD / 4) + (int)(threadIdx.x & 31), left = run - at % run;
-        float4* p = reinterpret_cast<float4*>(out + (long long)(r0 / gsz + at / run) * H * HD) + (run - left);
-        return place{p, left, run, nv % run, gap, nv + (long long)(nv / run) * gap};
+        P* p = static_cast<P*>(out) + (long long)(r0 / gsz + at / run) * H * (HD / 4) + (run - left);
+        return place<P>{p, left, run, nv % run, gap, nv + (long long)(nv / run) * gap};
+    }
+};
+
+// A thread's places in turn. HALF: 16-bit rows hold the lower halves of the four values,
+// shared memory behind pr_held ([piece][thread]) the upper ones.
+template <int HD, bool HALF>
+struct pr_places;
+template <int HD>
+struct pr_places<HD, false> {
+    pr_held::place<float4> at;
+    __device__ pr_places(pr_held* held) : at(held->first<HD, float4>()) {}
+    __device__ float4 get() { return *at.next(); }
+    __device__ void put(float4 x) { *at.next() = x; }
+};
+template <int HD>
+struct pr_places<HD, true> {
+    pr_held::place<uint2> at;
+    uint2* upper;
+    __device__ pr_places(pr_held* held)
+        : at(held->first<HD, uint2>()), upper(reinterpret_cast<uint2*>(held + 1) + threadIdx.x) {}
+    __device__ float4 get() {
+        const uint2 lo = *at.next(), hi = *upper;
+        upper += kPrPair;
+        return make_float4(__uint_as_float(__byte_perm(lo.x, hi.x, 0x5410)), __uint_as_float(__byte_perm(lo.x, hi.x, 0x7632)),
+                           __uint_as_float(__byte_perm(lo.y, hi.y, 0x5410)), __uint_as_float(__byte_perm(lo.y, hi.y, 0x7632)));
+    }
+    __device__ void put(float4 x) {
+        const uint32_t a = __float_as_uint(x.x), b = __float_as_uint(x.y), c = __float_as_uint(x.z), d = __float_as_uint(x.w);
+        *at.next() = make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+        *upper = make_uint2(__byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
+        upper += kPrPair;
     }
 };
 
@@ -92,9 +125,9 @@ struct pr_part {
     __device__ static float2* stats(float* part) { return reinterpret_cast<float2*>(part + kPrPair * HD); }
 };
 
-template <int HD, bool LO>
+template <int HD, bool F32>
 struct pr_smem {
-    static constexpr int NG = HD / 64, PARTS = LO ? 2 : 1;
+    static constexpr int NG = HD / 64, PARTS = F32 ? 2 : 1;  // parts of q
     static constexpr int QCHUNK = kPrTile * 16 + 16;  // bytes of 8 values of all rows (16 more: stores spread over the banks)
     static constexpr int QTILE = HD / 8 * QCHUNK, KTILE = kKv4Rows * HD * 2, VTILE = NG * 64 * kPrCore;
     static constexpr int sc = 512;                       // fp32 scales [2 buffers][K g0, K g1, V g0, V g1][64]
@@ -103,9 +136,9 @@ struct pr_smem {
     static constexpr int v = k + 2 * KTILE;              // [buffer][group][8 positions' chunk][8 values' core]
     static constexpr int raw = v + 2 * VTILE;
     static constexpr int held = raw + 2 * kv4_block_bytes(HD);
-    static constexpr int total = held + (int)sizeof(pr_held);
+    static constexpr int total = held + (int)sizeof(pr_held) + (F32 ? 0 : kPrPair * HD * 2);
     static constexpr int SCOLS = NG * 64, TCOLS = 2 * SCOLS;  // TMEM columns of a tile: S (then P), O
-    static_assert(sizeof(pr_bars) <= 512 && total <= 227 * 1024, "shared memory");
+    static_assert(sizeof(pr_bars) <= 512 && sizeof(pr_held) % 8 == 0 && total <= 227 * 1024, "shared memory");
 };
 
 // A wait of a whole warp, bounded; false when it ran out or another role gave up.
@@ -144,10 +177,10 @@ __device__ __forceinline__ float4 load4(const T* p) {
 // its power times |scale| log2 e (not 0, which would undo a masked score of -infinity).
 // HD / 4 lanes read a row (a row per thread touched 32 lines a load and took 13 us a
 // block). src(i): row i.
-template <int HD, bool LO, typename T, typename F>
+template <int HD, bool F32, typename T, typename F>
 __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int r0) {
     constexpr int LPR = HD / 4, RPW = 32 / LPR, ROWS = 8;  // rows of a lane in flight
-    using SM = pr_smem<HD, LO>;
+    using SM = pr_smem<HD, F32>;
     const int lane = threadIdx.x & 31, w = lane % LPR;
     float f = 0.0f;
 #pragma unroll 1
@@ -180,7 +213,7 @@ __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int
             split2(odd ? make_float2(sb, y.w) : make_float2(y.y, sb), hi.y, lo.y);
             uint8_t* p = dst + w / 2 * SM::QCHUNK + (r0 + row) * 16 + (w & 1) * 8;
             *reinterpret_cast<uint2*>(p) = hi;
-            if (LO) *reinterpret_cast<uint2*>(p + SM::QTILE) = lo;
+            if (F32) *reinterpret_cast<uint2*>(p + SM::QTILE) = lo;
         }
     }
     return fminf(fmaxf(f * (fabsf(scale) * 1.4426950408889634f), FLT_MIN), FLT_MAX);
@@ -268,23 +301,24 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
     }
 }
 
-// Moves the finished sums in TMEM (HD columns from `to`) to `out`, onto what earlier
-// calls put there, rescaled to the reference `ref`. Places: pieces (4 values) of the
-// warp's rows in turn over the rows' own part of `out` (runs of the kv head's heads,
-// one run a token). A call of its own that finds its arguments in shared memory:
-// inlined it took the softmax's registers (chunk below: 326 us inlined, 309 so).
-template <int HD>
+// Moves the finished sums in TMEM (HD columns from `to`) to their places, onto what
+// earlier calls put there, rescaled to the reference `ref`. Places: pieces (4 values) of
+// the warp's rows in turn over the rows' own part of `out` (runs of the kv head's heads,
+// one run a token) or of the workspace. A call of its own that finds its arguments in
+// shared memory: inlined it took the softmax's registers (chunk below: 326 us inlined,
+// 309 so).
+template <int HD, bool HALF>
 __device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool holds) {
     const float href = held->ref[threadIdx.x], al = ex2(href - (ref == -INFINITY ? 0.0f : ref));
     const bool mine = held->mine();
     held->ref[threadIdx.x] = ref;
-    pr_held::place st = held->first<HD>(), ld = st;
+    pr_places<HD, HALF> st(held), ld(held);
 #pragma unroll 1
     for (int q = 0; q < HD; q += 32) {
         float4 y[8];
         if (holds && mine)
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = *ld.next();
+            for (int i = 0; i < 8; i++) y[i] = ld.get();
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             float o[16];
@@ -296,23 +330,23 @@ __device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool
                     float4 x = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     const float4 z = y[4 * p + i];
                     if (holds) x = make_float4(fmaf(z.x, al, x.x), fmaf(z.y, al, x.y), fmaf(z.z, al, x.z), fmaf(z.w, al, x.w));
-                    *st.next() = x;
+                    st.put(x);
                 }
         }
     }
 }
 
 // At the end: what the places hold, back onto the last sums in TMEM.
-template <int HD>
+template <int HD, bool HALF>
 __device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
     const float al = ex2(held->ref[threadIdx.x] - (ref == -INFINITY ? 0.0f : ref));
-    pr_held::place at = held->first<HD>();
+    pr_places<HD, HALF> at(held);
 #pragma unroll 1
     for (int q = 0; q < HD; q += 16) {
         float4 y[4] = {};
         if (held->mine())
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = *at.next();
+            for (int i = 0; i < 4; i++) y[i] = at.get();
         float o[16];
         __syncwarp();
         tc_ld16(to + q, o);
@@ -329,8 +363,9 @@ __device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l, jl_kv4_attn_args a, int pairs, int S) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr bool LO = sizeof(T) == 4;
-    using SM = pr_smem<HD, LO>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int FOLD = kPrFold<F32>;
+    using SM = pr_smem<HD, F32>;
     constexpr int NG = SM::NG, PARTS = SM::PARTS, BLK = kv4_block_bytes(HD);
     pr_bars& sh = *reinterpret_cast<pr_bars*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -370,8 +405,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         sh.abort = 0;
         if (S > 1) {
             held->out = pr_part<HD>::of(a.ws, blockIdx.x), held->H = held->gsz = 1, held->row0 = 0, held->rows = kPrPair;
-        } else if (LO) {
-            held->out = static_cast<float*>(a.out) + ((long long)b * a.T * a.H + kh * gsz) * HD;
+        } else {
+            held->out = static_cast<T*>(a.out) + ((long long)b * a.T * a.H + kh * gsz) * HD;
             held->H = a.H, held->gsz = gsz, held->row0 = row0, held->rows = rows;
         }
         for (int i = 0; i < 2; i++) {
@@ -396,7 +431,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    auto starts = [](int j) { return LO ? j % kPrFold == 0 : j == 0; };  // blocks at which TMEM's sums start anew
+    auto starts = [](int j) { return j % FOLD == 0; };  // blocks at which TMEM's sums start anew
     volatile int* abort = &sh.abort;
 
     if (warp < 8) {
@@ -404,7 +439,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         const int t = warp >> 2;
         if (t < tiles) {
             uint8_t* qs = smem + SM::q + t * PARTS * SM::QTILE;
-            const float f = pr_load_q<HD, LO, T>(
+            const float f = pr_load_q<HD, F32, T>(
                 [&](int i) {
                     const int r = min(row0 + warp * 32 + i, rows - 1);
                     return static_cast<const T*>(a.q) + ((long long)b * a.T + r / gsz) * a.q_stride + (kh * gsz + r % gsz) * HD;
@@ -423,8 +458,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 // the scales (kv_full), then the scores
                 if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) || !pr_wait(&sh.s_full[t], j & 1, a.err, abort)) break;
                 tc_fence_after();
-                if (LO && j > 0 && starts(j)) {  // S was issued after the last block's values: the sums are complete
-                    pr_fold<HD>(to, ref, held, j > kPrFold);
+                if (j > 0 && starts(j)) {  // S was issued after the last block's values: the sums are complete
+                    if (F32 || S > 1) pr_fold<HD, false>(to, ref, held, j > FOLD);
+                    else pr_fold<HD, true>(to, ref, held, j > FOLD);
                 }
                 const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
                 float2 x[32];
@@ -499,18 +535,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                         lsum = __fadd2_rn(lsum, p);
                         const float4 w0 = v0[i / 2], w1 = NG == 2 ? v1[i / 2] : w0;
                         const float2 y0 = __fmul2_rn(p, i & 1 ? make_float2(w0.z, w0.w) : make_float2(w0.x, w0.y));
-                        if (LO) split2(y0, hi[0][i], lo[0][i]);
-                        else hi[0][i] = h2bits(__float22half2_rn(y0));
+                        split2(y0, hi[0][i], lo[0][i]);
                         if (NG == 2) {
                             const float2 y1 = __fmul2_rn(p, i & 1 ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
-                            if (LO) split2(y1, hi[NG - 1][i], lo[NG - 1][i]);
-                            else hi[NG - 1][i] = h2bits(__float22half2_rn(y1));
+                            split2(y1, hi[NG - 1][i], lo[NG - 1][i]);
                         }
                     }
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         tc_st8(ts + 64 * g + 8 * q, hi[g]);
-                        if (LO) tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
+                        tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
                     }
                 }
                 tc_wait_st();
@@ -523,10 +557,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 const float ls = lsum.x + lsum.y;
                 griddep_launch_dependents();  // not before: the next kernel's blocks, the merge's, would poll beside this one's
                 if (S > 1) {
-                    pr_fold<HD>(to, ref, held, LO && nb > kPrFold);
-                    pr_part<HD>::stats(held->out)[threadIdx.x] = make_float2(ref, ls);
+                    pr_fold<HD, false>(to, ref, held, nb > FOLD);
+                    pr_part<HD>::stats(static_cast<float*>(held->out))[threadIdx.x] = make_float2(ref, ls);
                 } else {
-                    if (LO && nb > kPrFold) pr_unfold<HD>(to, ref, held);
+                    if (nb > FOLD) pr_unfold<HD, !F32>(to, ref, held);
                     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
                     // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
                     constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
@@ -636,7 +670,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
 #pragma unroll
                     for (int g = 0; g < NG; g++)
 #pragma unroll
-                        for (int p = 0; p < PARTS; p++)
+                        for (int p = 0; p < 2; p++)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 tc_mma_ts(to + 64 * g, ts + 64 * g + 32 * p + 8 * k,

@@ -170,3 +170,44 @@ def test_any_finite_scale(T, t, scale):
     want, M, ds, top = _exact(q[0], *_held(cache, 0, n), float(np.float32(scale)))
     half = _step_of(want, t) / 2 * (1 + 2.0 ** -20) if t == "f16" else E * want.abs()
     assert not ((got[0].double() - want).abs() > half + (4 * ds + (2 * n + 64) * E) * M).any()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("B,T,H,kv,hd,lens,maxT", [(2, 700, 16, 4, 128, [700, 700], 720), (3, 900, 6, 2, 64, [900, 905, 1000], 1000),
+                                                   (1, 64, 32, 4, 128, [70], 4096), (1, 70, 32, 2, 64, [71], 3000)])
+def test_weights_of_a_16_bit_prompt(B, T, H, kv, hd, lens, maxT, t):
+    """The first 60 rows of a prompt, over a few positions each, whole and in splits (most
+    of them empty)."""
+    from joule_b200 import kv4
+    g = _gen(B + T)
+    rows = [(torch.randn(n, kv, hd, device="cuda", generator=g), torch.rand(n, kv, hd, device="cuda", generator=g) + 0.5)
+            for n in lens]
+    cache = _cache(rows, maxT)
+    q = (torch.randn(B, T, H, hd, device="cuda", generator=g) * 0.1).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32(range(B)), _i32(lens))[:, :60]
+    first = torch.arange(60, device="cuda")
+    parts = [_exact(q[b], *_held(cache, b, n), hd ** -0.5, first) for b, n in enumerate(lens)]
+    want, M, ds = (torch.cat([p[i] for p in parts]) for i in range(3))
+    _nearest(got.flatten(0, 1), want, M, ds, 1.0, 160, t)
+    assert max(p[3] for p in parts) < 1.0
+
+
+@pytest.mark.parametrize("T,H,kv,hd,n", [(1184, 32, 4, 128, 23000), (1, 32, 4, 128, 60000), (300, 8, 1, 64, 23000), (2500, 16, 4, 64, 23000),
+                                         (2100, 24, 3, 128, 2900)])
+def test_sums_of_16_bit_calls_do_not_shrink(T, H, kv, hd, n):
+    """Values of one sign over many positions. The part of the results along the exact ones
+    is off by no more than products cut off rather than rounded over at most 32 blocks make
+    (1.6e-7 each, half of that on the way), fp32 sums (64 e), and five standard deviations of
+    the mean of the results' own roundings."""
+    from joule_b200 import kv4
+    g = _gen(T)
+    k, v = torch.randn(n, kv, hd, device="cuda", generator=g), torch.rand(n, kv, hd, device="cuda", generator=g) + 0.5
+    cache = _cache([(k, v)])
+    q = torch.randn(1, T, H, hd, device="cuda", generator=g).half()
+    got = kv4.kv4_attention(cache, 0, q, _i32([0]), _i32([n]))[0]
+    r = torch.unique(torch.linspace(0, T - 1, min(24, T)).long()).cuda()
+    want, M, ds, top = _exact(q[0], *_held(cache, 0, n), hd ** -0.5, r)
+    err = got[r].double() - want
+    assert (err.abs() <= _step_of(want, "f16") / 2 * (1 + 2.0 ** -20) + (4 * ds + (2 * n + 64) * E) * M).all()
+    bias = ((err * want).sum() / (want * want).sum()).item()
+    assert abs(bias) <= 32 * 0.8e-7 + 64 * E + 5 * 2.0 ** -11 / math.sqrt(3 * err.numel()), bias
