@@ -30,7 +30,6 @@
 // shared memory) and by the softmax's issue slots in 16 bits. 2,047 rows of 32/4 heads
 // of 128 over 4,100 positions, fp32: 313 us; 123 at the measured bf16 rate.
 #include <algorithm>
-#include <cfloat>
 #include <climits>
 
 #include "jl_internal.h"
@@ -171,14 +170,14 @@ __device__ __forceinline__ float4 load4(const T* p) {
     return make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
 }
 
-// The warp's 32 q rows, by a power of two each (the largest value in [2^10, 2^11)) and
-// the scale's sign, into the operand from row r0 on: 16-bit values exactly, fp32 ones as
-// hi and lo parts. Returns what makes base-2 scores of row `lane`'s sums: the inverse of
-// its power times |scale| log2 e (not 0, which would undo a masked score of -infinity).
-// HD / 4 lanes read a row (a row per thread touched 32 lines a load and took 13 us a
-// block). src(i): row i.
+// The warp's 32 q rows, by a power of two each (the largest value in [2^10, 2^11)), into
+// the operand from row r0 on: 16-bit values exactly, fp32 ones as hi and lo parts. Returns
+// the inverse of the power of row `lane` (what else makes base-2 scores of the sums is in
+// K's scales: a factor that is no power of two would round scores that weights are
+// differences of). HD / 4 lanes read a row (a row per thread touched 32 lines a load and
+// took 13 us a block). src(i): row i.
 template <int HD, bool F32, typename T, typename F>
-__device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int r0) {
+__device__ __forceinline__ float pr_load_q(F src, uint8_t* dst, int r0) {
     constexpr int LPR = HD / 4, RPW = 32 / LPR, ROWS = 8;  // rows of a lane in flight
     using SM = pr_smem<HD, F32>;
     const int lane = threadIdx.x & 31, w = lane % LPR;
@@ -197,8 +196,7 @@ __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int
             for (int o = LPR / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             int e = (int)(__float_as_uint(mx) >> 23);
             e = min(max(e, 11), 253);
-            const float inv = copysignf(__uint_as_float((uint32_t)(264 - e) << 23), scale);
-            const float fr = __uint_as_float((uint32_t)(e - 10) << 23);
+            const float inv = __uint_as_float((uint32_t)(264 - e) << 23), fr = __uint_as_float((uint32_t)(e - 10) << 23);
 #pragma unroll
             for (int q = 0; q < RPW; q++) {
                 const float fq = __shfl_sync(0xffffffffu, fr, q * LPR);
@@ -216,7 +214,7 @@ __device__ __forceinline__ float pr_load_q(F src, float scale, uint8_t* dst, int
             if (F32) *reinterpret_cast<uint2*>(p + SM::QTILE) = lo;
         }
     }
-    return fminf(fmaxf(f * (fabsf(scale) * 1.4426950408889634f), FLT_MIN), FLT_MAX);
+    return f;
 }
 
 // 16 bytes of values.
@@ -232,9 +230,9 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
 }
 
 // Unpacks one cache block (kPrUnpack warps, tid from 0) into operand tiles and fp32
-// scales; positions from n on (never written) get scales of 0.
+// scales (K's times `factor`); positions from n on (never written) get scales of 0.
 template <int HD>
-__device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, float* top, int n, int tid) {
+__device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, float* top, float factor, int n, int tid) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = tid & 31, w = tid >> 5;
     // K: lane (t, position of 8) takes words 2t, 2t + 1 of the groups
@@ -292,7 +290,7 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const uint32_t b = tid < n ? vs[g] : 0;
-            sc[g * kKv4Rows + tid] = tid < n ? half_bits_to_f32(ks[g]) : 0.0f;
+            sc[g * kKv4Rows + tid] = tid < n ? half_bits_to_f32(ks[g]) * factor : 0.0f;
             sc[(2 + g) * kKv4Rows + tid] = half_bits_to_f32((uint16_t)b);
             bits = max(bits, b);
         }
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                     const int r = min(row0 + warp * 32 + i, rows - 1);
                     return static_cast<const T*>(a.q) + ((long long)b * a.T + r / gsz) * a.q_stride + (kh * gsz + r % gsz) * HD;
                 },
-                a.scale, qs, (warp & 3) * 32);
+                qs, (warp & 3) * 32);
             fence_proxy_async_smem();  // before the tensor cores read it
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full);
@@ -595,6 +593,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     } else if (warp < 8 + kPrUnpack) {
         // ---------------- unpack, and the copies of the cache's blocks
         const int tid = threadIdx.x - 256, w = warp - 8;
+        const float factor = a.scale * 1.4426950408889634f;
         const uint8_t* src = c.run(a.slots[b], l, kh) + (size_t)jb * BLK;
         uint8_t* raw = smem + SM::raw;
         auto issue = [&](int j) {
@@ -610,7 +609,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             if (!pr_wait(&sh.raw_full[s], j >> 1 & 1, a.err, abort)) break;
             if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, a.err, abort)) break;
             pr_unpack<HD>(raw + s * BLK, smem + SM::k + s * SM::KTILE, smem + SM::v + s * SM::VTILE,
-                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], len - off - j * kKv4Rows, tid);
+                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], factor, len - off - j * kKv4Rows, tid);
             fence_proxy_async_smem();  // the operands to the tensor cores, the reads before the next copy
             __syncwarp();
             if (lane == 0) {

@@ -211,3 +211,25 @@ def test_sums_of_16_bit_calls_do_not_shrink(T, H, kv, hd, n):
     assert (err.abs() <= _step_of(want, "f16") / 2 * (1 + 2.0 ** -20) + (4 * ds + (2 * n + 64) * E) * M).all()
     bias = ((err * want).sum() / (want * want).sum()).item()
     assert abs(bias) <= 32 * 0.8e-7 + 64 * E + 5 * 2.0 ** -11 / math.sqrt(3 * err.numel()), bias
+
+
+@pytest.mark.parametrize("T", [1, 30, 720])
+@pytest.mark.parametrize("size", [1e4, 1e6])
+def test_scores_past_the_fraction_of_a_float(T, size):
+    """One key ahead of all others by thousands at scores of 1e6 to 1e10: its values."""
+    from joule_b200 import kv4
+    g = _gen(44)
+    n, kv, hd, H = 800, 2, 128, 16
+    k, v = (torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2))
+    v *= 0.01
+    k[:, :, 0] = 7.0
+    k[3, :, 0] = 14.0
+    k *= size / 100
+    q = torch.zeros(1, T, H, hd, device="cuda")
+    q[..., 0] = size
+    got = kv4.kv4_attention(_cache([(k, v)]), 0, q, _i32([0]), _i32([n]), scale=1.0)
+    c = _cache([(k, v)])
+    kk, vv = _held(c, 0, n)
+    assert (kk[3, :, 0] > kk[torch.arange(n) != 3][:, :, 0].amax()).all()
+    want = vv[3].repeat_interleave(H // kv, 0)
+    assert (got[0].double() - want).abs().amax() <= 8 * E * want.abs().amax()
