@@ -145,7 +145,7 @@ struct kv4_state {
     static constexpr int NG = HD / 64;
     uint32_t qf[NG * 4][4];  // q of row g per step of 16 values
     float f;                 // accumulator -> score in base 2 (a power of two)
-    float ref;               // reference of row g's exponents, base 2
+    kv4_ref<NG == 2> r;      // row g's references
     float2 l;                // this thread's sum of row g's weights
     float o[NG][4][4];       // o[gr][i][c]: value 64 gr + 8 g + 2 i + c / 2 of row 2 t + c % 2
     int n;                   // positions that row g sees
@@ -194,7 +194,7 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
 #pragma unroll
             for (int c = 0; c < 4; c++) st.o[g][i][c] = 0.0f;
     }
-    st.ref = -INFINITY;
+    st.r.clear();
     st.l = f2(0.0f);
 }
 
@@ -246,34 +246,35 @@ __device__ __forceinline__ void kv4_scores(const kv4_state<HD>& st, const uint8_
     }
 }
 
-// A weight past the limit (or the first of a row): its row takes a new reference,
-// and its sums are brought to it. mx: this thread's largest score of row g.
+// A product past the limit (or the first of a row): its row takes new references, and
+// its sums are brought to them. mx, b0, b1 (kv4_ref): this thread's part of row g.
 template <int HD>
-__device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, float top) {
+__device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, float b0, float b1) {
     const int t = threadIdx.x & 3;
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    float al = 1.0f;
-    if (mx - st.ref > kTop - top) {
-        mx += top - (kTop - kHeadroom);
-        al = ex2(st.ref - mx);  // the first time: 0
-        st.ref = mx;
-    }
-    st.l = __fmul2_rn(st.l, f2(al));
-    const float2 ac = make_float2(__shfl_sync(0xffffffffu, al, 8 * t), __shfl_sync(0xffffffffu, al, 8 * t + 4));
 #pragma unroll
-    for (int gr = 0; gr < HD / 64; gr++)
+    for (int o = 1; o <= 2; o <<= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, o));
+        if (HD == 128) b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, o));
+    }
+    const float2 al = st.r.past(mx, b0, b1) ? st.r.move(mx, b0, b1) : f2(1.0f);
+    st.l = __fmul2_rn(st.l, f2(al.x));
+#pragma unroll
+    for (int gr = 0; gr < HD / 64; gr++) {
+        const float x = gr ? al.y : al.x;
+        const float2 ac = make_float2(__shfl_sync(0xffffffffu, x, 8 * t), __shfl_sync(0xffffffffu, x, 8 * t + 4));
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) st.o[gr][i][c] *= c & 1 ? ac.y : ac.x;
+    }
 }
 
 // Weights of positions r0 .. r0 + 15 from their scores, and the weighted values
 // onto the sums. V's scale multiplies the weight in fp32. MASK: row g does not see
 // positions from n on (in the block's numbering); those may hold any scale.
 template <int HD, bool MASK>
-__device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], float ref, int n) {
+__device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], int n) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t bh[NG][2], bl[NG][2];
@@ -281,13 +282,14 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
     for (int h = 0; h < 2; h++) {
         float2 sc[NG];
         scale_pairs<NG>(blk + kv4_vscale(HD), r0 + 8 * h + 2 * t, sc);
-        s[h] = __fadd2_rn(s[h], f2(ref));
+        s[h] = __fadd2_rn(s[h], f2(st.r.minus()));
         s[h].x = ex2(s[h].x);
         s[h].y = ex2(s[h].y);
         st.l = __fadd2_rn(st.l, s[h]);
 #pragma unroll
         for (int gr = 0; gr < NG; gr++) {
             float2 w = __fmul2_rn(s[h], sc[gr]);
+            if (gr) w = __fmul2_rn(w, f2(st.r.more()));
             if (MASK) {
                 if (r0 + 8 * h + 2 * t >= n) w.x = 0.0f;
                 if (r0 + 8 * h + 2 * t + 1 >= n) w.y = 0.0f;
@@ -348,34 +350,31 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
 }
 
 // One block (j0 = its first position's number): rows see all positions below n_min
-// and none from n_max on. A block that all rows see whole is one stretch of code
-// with one branch; others go by 16 positions.
+// and none from n_max on. A block that all rows see whole, with scales of about one
+// size, is one stretch of code with one branch; others go by 16 positions.
 template <int HD>
 __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk, int j0, int n_min, int n_max) {
     constexpr int NG = HD / 64;
     const int lane = threadIdx.x & 31, t = lane & 3;
-    // 2^top: the power of two above the block's largest V scale that a row sees
-    uint32_t bits = 0;
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-        if (j0 + 32 * h + lane < n_max) {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(blk + kv4_vscale(HD)) + (32 * h + lane) * NG;
-            bits = max(bits, (uint32_t)(NG == 2 ? max(p[0], p[NG - 1]) : p[0]));
-        }
-    const float top = (float)((int)(__reduce_max_sync(0xffffffffu, bits) >> 10) - 14);
     if (j0 + kKv4Rows <= n_min) {
-        float2 s[4][2];
-        float mx = -INFINITY;
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(blk + kv4_vscale(HD)) + lane * NG;
+        uint32_t most = max(p[0], p[32 * NG]), least = min(p[0], p[32 * NG]);
+        if (NG == 2) most = max(most, max(p[1], p[32 * NG + 1])), least = min(least, min(p[1], p[32 * NG + 1]));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (!kv4_spread(most, __reduce_min_sync(0xffffffffu, least))) {
+            const float top = kv4_top(most);
+            float2 s[4][2];
+            float mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            kv4_scores<HD>(st, blk, 16 * k, s[k]);
-            mx = fmaxf(mx, fmaxf(fmaxf(s[k][0].x, s[k][0].y), fmaxf(s[k][1].x, s[k][1].y)));
+            for (int k = 0; k < 4; k++) {
+                kv4_scores<HD>(st, blk, 16 * k, s[k]);
+                mx = fmaxf(mx, fmaxf(fmaxf(s[k][0].x, s[k][0].y), fmaxf(s[k][1].x, s[k][1].y)));
+            }
+            if (__any_sync(0xffffffffu, st.r.past(mx, top, top))) kv4_new_reference<HD>(st, mx, top, top);
+#pragma unroll
+            for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], 0);
+            return;
         }
-        if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
-        const float ref = st.ref == -INFINITY ? 0.0f : -st.ref;
-#pragma unroll
-        for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], ref, 0);
-        return;
     }
     const int n = st.n - j0;
 #pragma unroll 1
@@ -387,9 +386,19 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
             if (r0 + 8 * h + 2 * t >= n) s[h].x = -INFINITY;
             if (r0 + 8 * h + 2 * t + 1 >= n) s[h].y = -INFINITY;
         }
-        const float mx = fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[1].x, s[1].y));
-        if (__any_sync(0xffffffffu, mx - st.ref > kTop - top)) kv4_new_reference<HD>(st, mx, top);
-        kv4_values<HD, true>(st, blk, r0, s, st.ref == -INFINITY ? 0.0f : -st.ref, n);
+        float mx = fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[1].x, s[1].y)), b[2] = {kLeast, kLeast};
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // (an unseen position's score stays -infinity whatever its scale's bits are)
+            float2 sc[NG];
+            scale_pairs<NG>(blk + kv4_vscale(HD), r0 + 8 * h + 2 * t, sc);
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+                b[gr] = fmaxf(b[gr], fmaxf((s[h].x - mx) + exponent_of(sc[gr].x), (s[h].y - mx) + exponent_of(sc[gr].y)));
+        }
+        if (__any_sync(0xffffffffu, st.r.past(mx, b[0], b[1]))) kv4_new_reference<HD>(st, mx, b[0], b[1]);
+        kv4_values<HD, true>(st, blk, r0, s, n);
     }
 }
 
@@ -524,6 +533,13 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
             lrow += __shfl_xor_sync(0xffffffffu, lrow, 1);
             lrow += __shfl_xor_sync(0xffffffffu, lrow, 2);
             const float2 lsum = make_float2(__shfl_sync(0xffffffffu, lrow, 8 * t), __shfl_sync(0xffffffffu, lrow, 8 * t + 4));
+            if (NG == 2) {  // both groups' sums on one scale
+                const float x = st.r.less(), x0 = __shfl_sync(0xffffffffu, x, 8 * t), x1 = __shfl_sync(0xffffffffu, x, 8 * t + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) st.o[NG - 1][j][c] *= c & 1 ? x1 : x0;
+            }
             const bool from_start = i >= co.j;  // the segment's first unit is in this warp's run
             if (ends && from_start) {
 #pragma unroll
@@ -561,7 +577,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
                     }
                 }
                 if (t == 0) {
-                    ml[g] = st.ref;
+                    ml[g] = st.r.ref;
                     ml[kKvTile + g] = lrow;
                 }
             }

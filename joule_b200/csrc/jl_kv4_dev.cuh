@@ -8,10 +8,19 @@
 
 namespace jl {
 
-// Weights times V's scales are kept at or below 2^kTop in fp16; a new reference
-// puts the largest at 2^(kTop - kHeadroom), so that the sums are not rescaled at
-// every new maximum (most units of a short run have one in some row).
-constexpr float kTop = 15.0f, kHeadroom = 4.0f;
+// Weights times V's scales enter the second product as fp16 hi and lo parts: 22 bits of
+// a product of 2^-2 and more, down to steps of 2^-24 below. So the largest product of a
+// row has to be near the top of fp16's range whatever the scales are, in each 64-value
+// group by itself (kv4_ref): products are kept at or below 2^kTop, and a new reference
+// puts the largest at 2^(kTop - kHeadroom), so that the sums are not rescaled at every
+// new maximum (most units of a short run have one in some row).
+//
+// How large the products of a block are: its largest score times its largest scale is a
+// bound, at most 2^kSpread above the truth when the scales of all its positions and
+// groups are within that (kv4_spread), and then costs nothing. Else, and in blocks that
+// not all rows see whole, the maximum is taken over the products that the row has.
+constexpr float kTop = 15.0f, kHeadroom = 4.0f, kLeast = -40.0f;  // 2^kLeast: taken for products of 0
+constexpr int kSpread = 10;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -67,10 +76,63 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// 2^e is above x >= 0 (by at most 2): e, at least kLeast.
+__device__ __forceinline__ float exponent_of(float x) {
+    return fmaxf((float)((int)(__float_as_uint(x) >> 23) - 126), kLeast);
+}
+
+// From the largest and smallest scale's bits: the exponent that bounds them, and whether
+// some are zero, subnormal or smaller by more than 2^kSpread.
+__device__ __forceinline__ float kv4_top(uint32_t most) { return (float)((int)(most >> 10) - 14); }
+__device__ __forceinline__ bool kv4_spread(uint32_t most, uint32_t least) {
+    return least < 1024 || most - least > (uint32_t)kSpread << 10;
+}
+
+// A row's references: weights are 2^(score - ref), and those of a head's second group
+// (G1) may take a power of two more into the product, so that each group's largest
+// product is near the top: 2^lift would bring it there, and lifts of 0 to kNoLift are
+// left out: `ref` goes by the larger group unless the second is larger by more, so
+// that ordinary rows have no other. `ref` is a score plus a whole number.
+constexpr float kNoLift = 8.0f;
+template <bool G1>
+struct kv4_ref {
+    float ref, lift;
+    __device__ __forceinline__ void clear() { ref = -INFINITY, lift = 0.0f; }
+    __device__ __forceinline__ bool lifted() const { return G1 && !(lift >= 0.0f && lift <= kNoLift); }
+    __device__ __forceinline__ float log_more() const { return lifted() ? lift : 0.0f; }
+    // the second group's factor, and what brings its sums to a scale without it
+    __device__ __forceinline__ float more() const { return __uint_as_float((uint32_t)((int)log_more() + 127) << 23); }
+    __device__ __forceinline__ float less() const { return __uint_as_float((uint32_t)(127 - (int)log_more()) << 23); }
+    __device__ __forceinline__ float minus() const { return ref == -INFINITY ? 0.0f : -ref; }
+    // Does a product of at most 2^(b0 + score - mx) of group 0, or 2^(b1 + ...) of group 1, pass the limit?
+    __device__ __forceinline__ bool past(float mx, float b0, float b1) const {
+        return (mx - ref) + (G1 ? fmaxf(b0, b1 + log_more()) : b0) > kTop;
+    }
+    // Brings the references to a row's largest score mx (its products below 2^b0 and 2^b1 of
+    // that weight) and returns the factors of the sums: of the weights and group 0, of group 1.
+    // A reference that fp32 cannot hold to within 1 (scores past 2^24) is the score itself.
+    __device__ __forceinline__ float2 move(float mx, float b0, float b1) {
+        const float old = ref, was = log_more(), b = G1 && b1 - b0 <= kNoLift ? fmaxf(b0, b1) : b0;
+        if ((mx - ref) + b > kTop) {
+            const float k = ceilf(b - (kTop - kHeadroom));
+            ref = mx + k;
+            if (!(fabsf((ref - mx) - k) <= 1.0f)) ref = mx;
+        }
+        const float al = ex2(old - ref);  // the first time: 0
+        if (!G1) return make_float2(al, al);
+        const float at = (mx - ref) + b1, most = floorf((kTop - kHeadroom) - at);
+        lift = old == -INFINITY ? most : lift + floorf(ref - old);
+        if (at + log_more() > kTop) lift = most;
+        lift = fminf(fmaxf(lift, -100.0f), 100.0f);
+        return make_float2(al, ex2((old - ref) + (log_more() - was)));
+    }
+};
+
 __device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// A pair as fp16 pairs, hi the nearest and lo what hi misses: 22 bits down to
-// fp16's smallest steps of 2^-24 (callers scale what they split to 2^10 and more).
+// A pair as fp16 pairs, hi the nearest and lo what hi misses: 22 bits of values of 2^-2
+// and more, steps of 2^-24 of smaller ones (the callers' largest are 2^1 and more: a
+// row's q by a power of two, products by kv4_ref).
 __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __float22half2_rn(x);
     const float2 f = __half22float2(h);

@@ -9,9 +9,9 @@
 // (down to 2^-34 of a row's largest value); a fp32 q and the weights are hi and lo
 // parts (22 bits), two instructions onto the same sums.
 // K's scales multiply the finished sums of a 64-value group (one accumulator per
-// group), V's the weights of a group, both in fp32. The exponents' reference
-// moves only when a weight times its scale would pass 2^15 (jl_kv4_dev.cuh), and
-// the sums are then rescaled in TMEM.
+// group), V's the weights of a group, both in fp32. The exponents' references
+// (kv4_ref) move only when a weight times its scale would pass 2^15, and the sums
+// are then rescaled in TMEM.
 //
 // Roles (12 warps, so that the softmax has 168 registers a thread): 0-3 and 4-7
 // softmax of tile 0 and 1, 8-10 unpack the cache block into the two operands (K as
@@ -55,7 +55,7 @@ struct pr_bars {
     uint64_t s_full[2], p_full[2], pv_done[2], fin;
     uint32_t tmem;
     int abort;
-    float top[2][2];  // per buffer, per warp of positions: 2^top is above V's scales
+    uint2 range[2][2];  // per buffer, per warp of positions: bits of V's largest and smallest scale
 };
 
 struct pr_held {
@@ -232,7 +232,7 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
 // Unpacks one cache block (kPrUnpack warps, tid from 0) into operand tiles and fp32
 // scales (K's times `factor`); positions from n on (never written) get scales of 0.
 template <int HD>
-__device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, float* top, float factor, int n, int tid) {
+__device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8_t* vt, float* sc, uint2* range, float factor, int n, int tid) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = tid & 31, w = tid >> 5;
     // K: lane (t, position of 8) takes words 2t, 2t + 1 of the groups
@@ -286,27 +286,28 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
     if (tid < kKv4Rows) {
         const uint16_t* ks = reinterpret_cast<const uint16_t*>(raw + kv4_kscale(HD)) + tid * NG;
         const uint16_t* vs = reinterpret_cast<const uint16_t*>(raw + kv4_vscale(HD)) + tid * NG;
-        uint32_t bits = 0;
+        uint32_t most = 0, least = 0xFFFFu;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const uint32_t b = tid < n ? vs[g] : 0;
             sc[g * kKv4Rows + tid] = tid < n ? half_bits_to_f32(ks[g]) * factor : 0.0f;
             sc[(2 + g) * kKv4Rows + tid] = half_bits_to_f32((uint16_t)b);
-            bits = max(bits, b);
+            most = max(most, b), least = min(least, b);
         }
-        bits = __reduce_max_sync(0xffffffffu, bits);
-        if (lane == 0) top[w] = (float)((int)(bits >> 10) - 14);
+        most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) range[w] = make_uint2(most, least);
     }
 }
 
-// Moves the finished sums in TMEM (HD columns from `to`) to their places, onto what
-// earlier calls put there, rescaled to the reference `ref`. Places: pieces (4 values) of
+// Moves the finished sums in TMEM (HD columns from `to`; less: what brings the second
+// group's to the first's scale) to their places, onto what earlier calls put there,
+// rescaled to the reference `ref`. Places: pieces (4 values) of
 // the warp's rows in turn over the rows' own part of `out` (runs of the kv head's heads,
 // one run a token) or of the workspace. A call of its own that finds its arguments in
 // shared memory: inlined it took the softmax's registers (chunk below: 326 us inlined,
 // 309 so).
 template <int HD, bool HALF>
-__device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool holds) {
+__device__ __noinline__ void pr_fold(uint32_t to, float ref, float less, pr_held* held, bool holds) {
     const float href = held->ref[threadIdx.x], al = ex2(href - (ref == -INFINITY ? 0.0f : ref));
     const bool mine = held->mine();
     held->ref[threadIdx.x] = ref;
@@ -322,10 +323,11 @@ __device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool
             float o[16];
             __syncwarp();
             tc_ld16(to + q + 16 * p, o);
+            const float m = q < 64 ? 1.0f : less;
             if (mine)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float4 x = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    float4 x = make_float4(o[4 * i] * m, o[4 * i + 1] * m, o[4 * i + 2] * m, o[4 * i + 3] * m);
                     const float4 z = y[4 * p + i];
                     if (holds) x = make_float4(fmaf(z.x, al, x.x), fmaf(z.y, al, x.y), fmaf(z.z, al, x.z), fmaf(z.w, al, x.w));
                     st.put(x);
@@ -334,10 +336,11 @@ __device__ __noinline__ void pr_fold(uint32_t to, float ref, pr_held* held, bool
     }
 }
 
-// At the end: what the places hold, back onto the last sums in TMEM.
+// At the end: what the places hold, back onto the last sums in TMEM (more: the second
+// group's factor).
 template <int HD, bool HALF>
-__device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
-    const float al = ex2(held->ref[threadIdx.x] - (ref == -INFINITY ? 0.0f : ref));
+__device__ __noinline__ void pr_unfold(uint32_t to, float ref, float more, pr_held* held) {
+    const float al0 = ex2(held->ref[threadIdx.x] - (ref == -INFINITY ? 0.0f : ref));
     pr_places<HD, HALF> at(held);
 #pragma unroll 1
     for (int q = 0; q < HD; q += 16) {
@@ -348,6 +351,7 @@ __device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
         float o[16];
         __syncwarp();
         tc_ld16(to + q, o);
+        const float al = q < 64 ? al0 : al0 * more;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             o[4 * i] = fmaf(y[i].x, al, o[4 * i]), o[4 * i + 1] = fmaf(y[i].y, al, o[4 * i + 1]);
@@ -356,6 +360,190 @@ __device__ __noinline__ void pr_unfold(uint32_t to, float ref, pr_held* held) {
         tc_st16(to + q, o);
     }
     tc_wait_st();
+}
+
+// Scores (but for the row's power of two) of positions 16 q .. 16 q + 15 from the sums in
+// TMEM and K's scales.
+template <int HD>
+__device__ __forceinline__ void pr_scores(uint32_t ts, const float* sc, int q, float2* x) {
+    constexpr int NG = HD / 64;
+    float a0[16], a1[16];
+    if (NG == 2) tc_ld16x2(ts + 16 * q, ts + 64 + 16 * q, a0, a1);
+    else tc_ld16(ts + 16 * q, a0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float4 k0 = *reinterpret_cast<const float4*>(sc + 16 * q + 4 * i);
+        float2 u = __fmul2_rn(make_float2(a0[4 * i], a0[4 * i + 1]), make_float2(k0.x, k0.y));
+        float2 v = __fmul2_rn(make_float2(a0[4 * i + 2], a0[4 * i + 3]), make_float2(k0.z, k0.w));
+        if (NG == 2) {
+            const float4 k1 = *reinterpret_cast<const float4*>(sc + kKv4Rows + 16 * q + 4 * i);
+            u = __ffma2_rn(make_float2(a1[4 * i], a1[4 * i + 1]), make_float2(k1.x, k1.y), u);
+            v = __ffma2_rn(make_float2(a1[4 * i + 2], a1[4 * i + 3]), make_float2(k1.z, k1.w), v);
+        }
+        x[2 * i] = u;
+        x[2 * i + 1] = v;
+    }
+}
+// Scores of positions from n on: -infinity.
+template <int COUNT>
+__device__ __forceinline__ void pr_mask(float2* x, int n) {
+#pragma unroll
+    for (int i = 0; i < COUNT / 2; i++) {
+        if (2 * i >= n) x[i].x = -INFINITY;
+        if (2 * i + 1 >= n) x[i].y = -INFINITY;
+    }
+}
+
+// Weights of a block, 16 positions at a time, times V's scales of a group (MORE: and the
+// second group's factor), hi and lo, into S's place; adds them to lsum.
+template <int HD, bool MORE>
+__device__ __forceinline__ void pr_weights(uint32_t ts, const float* sc, const float2 (&x)[32], float f, float minus, float more,
+                                           float2& lsum) {
+    constexpr int NG = HD / 64;
+    const float2 nr = f2(minus), ff = f2(f);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        float4 v0[4], v1[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v0[i] = *reinterpret_cast<const float4*>(sc + 2 * kKv4Rows + 16 * q + 4 * i);
+            if (NG == 2) v1[i] = *reinterpret_cast<const float4*>(sc + 3 * kKv4Rows + 16 * q + 4 * i);
+        }
+        uint32_t hi[NG][8], lo[NG][8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float2 p = __ffma2_rn(x[8 * q + i], ff, nr);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            lsum = __fadd2_rn(lsum, p);
+            const float4 w0 = v0[i / 2], w1 = NG == 2 ? v1[i / 2] : w0;
+            const float2 y0 = __fmul2_rn(p, i & 1 ? make_float2(w0.z, w0.w) : make_float2(w0.x, w0.y));
+            split2(y0, hi[0][i], lo[0][i]);
+            if (NG == 2) {
+                float2 y1 = __fmul2_rn(p, i & 1 ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
+                if (MORE) y1 = __fmul2_rn(y1, f2(more));
+                split2(y1, hi[NG - 1][i], lo[NG - 1][i]);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            tc_st8(ts + 64 * g + 8 * q, hi[g]);
+            tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
+        }
+    }
+}
+
+// Exponents above a row's products with the scales of each group in a block (kv4_ref), from
+// the sums in TMEM: n positions are seen. 16 at a time, brought to the largest score. A call
+// of its own, before the softmax's registers are in use: inlined on its scores it made every
+// block slower (8 % of a prompt).
+template <int HD>
+__device__ __noinline__ float2 pr_products(uint32_t ts, float f, const float* sc, int n) {
+    constexpr int NG = HD / 64;
+    float mx = -INFINITY, b0 = kLeast, b1 = kLeast;
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        float2 x[8];
+        __syncwarp();
+        pr_scores<HD>(ts, sc, q, x);
+        pr_mask<16>(x, n - 16 * q);
+        float m = -INFINITY, m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fmaxf(x[i].x, x[i].y));
+        m *= f;
+        const float2 nm = f2(m == -INFINITY ? 0.0f : -m);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float2 p = __ffma2_rn(x[i], f2(f), nm);
+            p.x = ex2(p.x), p.y = ex2(p.y);
+            const float2 y0 = __fmul2_rn(p, *reinterpret_cast<const float2*>(sc + 2 * kKv4Rows + 16 * q + 2 * i));
+            m0 = fmaxf(m0, fmaxf(y0.x, y0.y));
+            if (NG == 2) {
+                const float2 y1 = __fmul2_rn(p, *reinterpret_cast<const float2*>(sc + 3 * kKv4Rows + 16 * q + 2 * i));
+                m1 = fmaxf(m1, fmaxf(y1.x, y1.y));
+            }
+        }
+        const float to = fmaxf(mx, m), up = to == -INFINITY ? 0.0f : mx - to, down = to == -INFINITY ? 0.0f : m - to;
+        b0 = fmaxf(fmaxf(b0 + up, exponent_of(m0) + down), kLeast);
+        b1 = fmaxf(fmaxf(b1 + up, exponent_of(m1) + down), kLeast);
+        mx = to;
+    }
+    return make_float2(b0, b1);
+}
+
+// The softmax of a thread's row over blocks from st.j on: ends at nb, at a wait that ran out
+// (st.j = -1), or, without MORE, at a block whose weights need a factor in some row of the
+// warp (its references are moved then, its sums folded and rescaled).
+template <int HD>
+struct pr_run {
+    kv4_ref<HD == 128> r;
+    float2 lsum;
+    int j;  // -1: not ok
+};
+template <int HD, bool F32, bool MORE>
+__device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t, uint32_t ts, float f, int nb, int S, int n_row,
+                                                 int n_min, pr_run<HD> st) {
+    using SM = pr_smem<HD, F32>;
+    constexpr int NG = SM::NG, FOLD = kPrFold<F32>;
+    pr_bars& sh = *reinterpret_cast<pr_bars*>(smem);
+    pr_held* held = reinterpret_cast<pr_held*>(smem + SM::held);
+    const uint32_t to = ts + SM::SCOLS;
+    const int from = st.j;
+    for (; st.j < nb; st.j++) {
+        const int j = st.j, s = j & 1, j0 = j * kKv4Rows;
+        // the scales (kv_full), then the scores
+        if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, err, &sh.abort) || !pr_wait(&sh.s_full[t], j & 1, err, &sh.abort)) {
+            st.j = -1;
+            return st;
+        }
+        tc_fence_after();
+        const bool starts = j % FOLD == 0;  // TMEM's sums start anew
+        if (j > 0 && starts && !(MORE && j == from)) {  // S was issued after the last block's values: the sums are complete
+            if (F32 || S > 1) pr_fold<HD, false>(to, st.r.ref, st.r.less(), held, j > FOLD);
+            else pr_fold<HD, true>(to, st.r.ref, st.r.less(), held, j > FOLD);
+        }
+        const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
+        const uint32_t most = max(sh.range[s][0].x, sh.range[s][1].x), least = min(sh.range[s][0].y, sh.range[s][1].y);
+        float2 bound = f2(kv4_top(most));
+        if (j0 + kKv4Rows > n_min || kv4_spread(most, least)) bound = pr_products<HD>(ts, f, sc, n_row - j0);
+        float2 x[32];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; q++) pr_scores<HD>(ts, sc, q, x + 8 * q);
+        if (j0 + kKv4Rows > n_min) pr_mask<64>(x, n_row - j0);
+#pragma unroll
+        for (int i = 0; i < 32; i++) mx = fmaxf(mx, fmaxf(x[i].x, x[i].y));
+        mx *= f;
+        const bool past = st.r.past(mx, bound.x, bound.y);  // a product past the limit, or the row's first
+        if (__any_sync(0xffffffffu, past)) {
+            const float2 al = past ? st.r.move(mx, bound.x, bound.y) : f2(1.0f);
+            st.lsum = __fmul2_rn(st.lsum, f2(al.x));
+            if (!starts) {  // the sums of earlier blocks are complete (S was issued after them)
+#pragma unroll 1
+                for (int q = 0; q < NG * 4; q++) {
+                    float o[16];
+                    tc_ld16(to + 16 * q, o);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] *= q < 4 ? al.x : al.y;
+                    tc_st16(to + 16 * q, o);
+                }
+                tc_wait_st();
+            }
+            if (NG == 2 && !MORE && __any_sync(0xffffffffu, st.r.lifted())) break;
+        }
+        pr_weights<HD, MORE>(ts, sc, x, f, st.r.minus(), MORE ? st.r.more() : 1.0f, st.lsum);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_full[t]);
+    }
+    return st;
+}
+// With factors: a call of its own (multiplying by them in all blocks took 4 % of a prompt).
+template <int HD, bool F32>
+__device__ __noinline__ pr_run<HD> pr_softmax_lifted(uint8_t* smem, int* err, int t, uint32_t ts, float f, int nb, int S, int n_row,
+                                                     int n_min, pr_run<HD> st) {
+    return pr_softmax<HD, F32, true>(smem, err, t, ts, f, nb, S, n_row, n_min, st);
 }
 
 template <int HD, typename T>
@@ -448,117 +636,25 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             if (lane == 0) mbar_arrive(&sh.q_full);
             const int n_row = sees(row) - off, n_min = sees(row0 + t * kPrTile) - off;
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * SM::TCOLS, to = ts + SM::SCOLS;
-            float ref = -INFINITY;
-            float2 lsum = f2(0.0f);
-            int j = 0;
-            for (; j < nb; j++) {
-                const int s = j & 1, j0 = j * kKv4Rows;
-                // the scales (kv_full), then the scores
-                if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, a.err, abort) || !pr_wait(&sh.s_full[t], j & 1, a.err, abort)) break;
-                tc_fence_after();
-                if (j > 0 && starts(j)) {  // S was issued after the last block's values: the sums are complete
-                    if (F32 || S > 1) pr_fold<HD, false>(to, ref, held, j > FOLD);
-                    else pr_fold<HD, true>(to, ref, held, j > FOLD);
-                }
-                const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
-                float2 x[32];
-                float mx = -INFINITY;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    float a0[16], a1[16];
-                    if (NG == 2) tc_ld16x2(ts + 16 * q, ts + 64 + 16 * q, a0, a1);
-                    else tc_ld16(ts + 16 * q, a0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float4 k0 = *reinterpret_cast<const float4*>(sc + 16 * q + 4 * i);
-                        float2 u = __fmul2_rn(make_float2(a0[4 * i], a0[4 * i + 1]), make_float2(k0.x, k0.y));
-                        float2 v = __fmul2_rn(make_float2(a0[4 * i + 2], a0[4 * i + 3]), make_float2(k0.z, k0.w));
-                        if (NG == 2) {
-                            const float4 k1 = *reinterpret_cast<const float4*>(sc + kKv4Rows + 16 * q + 4 * i);
-                            u = __ffma2_rn(make_float2(a1[4 * i], a1[4 * i + 1]), make_float2(k1.x, k1.y), u);
-                            v = __ffma2_rn(make_float2(a1[4 * i + 2], a1[4 * i + 3]), make_float2(k1.z, k1.w), v);
-                        }
-                        x[8 * q + 2 * i] = u;
-                        x[8 * q + 2 * i + 1] = v;
-                    }
-                }
-                if (j0 + kKv4Rows > n_min) {
-                    const int n = n_row - j0;
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        if (2 * i >= n) x[i].x = -INFINITY;
-                        if (2 * i + 1 >= n) x[i].y = -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) mx = fmaxf(mx, fmaxf(x[i].x, x[i].y));
-                mx *= f;
-                const float top = fmaxf(sh.top[s][0], sh.top[s][1]);
-                const bool past = mx - ref > kTop - top;  // a weight past the limit, or the row's first
-                if (__any_sync(0xffffffffu, past)) {
-                    float al = 1.0f;
-                    if (past) {
-                        const float nref = mx + top - (kTop - kHeadroom);
-                        al = ex2(ref - nref);
-                        ref = nref;
-                    }
-                    lsum = __fmul2_rn(lsum, f2(al));
-                    if (!starts(j)) {  // the sums of earlier blocks are complete (S was issued after them)
-#pragma unroll 1
-                        for (int q = 0; q < NG * 4; q++) {
-                            float o[16];
-                            tc_ld16(to + 16 * q, o);
-#pragma unroll
-                            for (int i = 0; i < 16; i++) o[i] *= al;
-                            tc_st16(to + 16 * q, o);
-                        }
-                        tc_wait_st();
-                    }
-                }
-                const float2 nr = f2(ref == -INFINITY ? 0.0f : -ref), ff = f2(f);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {  // 16 positions: weights, times V's scales of a group, hi and lo, into S's place
-                    float4 v0[4], v1[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        v0[i] = *reinterpret_cast<const float4*>(sc + 2 * kKv4Rows + 16 * q + 4 * i);
-                        if (NG == 2) v1[i] = *reinterpret_cast<const float4*>(sc + 3 * kKv4Rows + 16 * q + 4 * i);
-                    }
-                    uint32_t hi[NG][8], lo[NG][8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        float2 p = __ffma2_rn(x[8 * q + i], ff, nr);
-                        p.x = ex2(p.x);
-                        p.y = ex2(p.y);
-                        lsum = __fadd2_rn(lsum, p);
-                        const float4 w0 = v0[i / 2], w1 = NG == 2 ? v1[i / 2] : w0;
-                        const float2 y0 = __fmul2_rn(p, i & 1 ? make_float2(w0.z, w0.w) : make_float2(w0.x, w0.y));
-                        split2(y0, hi[0][i], lo[0][i]);
-                        if (NG == 2) {
-                            const float2 y1 = __fmul2_rn(p, i & 1 ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
-                            split2(y1, hi[NG - 1][i], lo[NG - 1][i]);
-                        }
-                    }
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        tc_st8(ts + 64 * g + 8 * q, hi[g]);
-                        tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
-                    }
-                }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
-            }
-            if (j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
+            pr_run<HD> st;
+            st.r.clear(), st.lsum = f2(0.0f), st.j = 0;
+            st = pr_softmax<HD, F32, false>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
+            if (st.j >= 0 && st.j < nb) st = pr_softmax_lifted<HD, F32>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
+            const kv4_ref<NG == 2> r = st.r;
+            const float2 lsum = st.lsum;
+            if (st.j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
                 tc_fence_after();
                 const float ls = lsum.x + lsum.y;
+                int tx = threadIdx.x;
+                asm volatile("" : "+r"(tx));  // the row's place again (kept over the loop it took registers)
+                const int row = row0 + tx, rc = min(row, rows - 1), h = kh * gsz + rc % gsz;
+                const long long orow = (long long)b * a.T + rc / gsz;
                 griddep_launch_dependents();  // not before: the next kernel's blocks, the merge's, would poll beside this one's
                 if (S > 1) {
-                    pr_fold<HD, false>(to, ref, held, nb > FOLD);
-                    pr_part<HD>::stats(static_cast<float*>(held->out))[threadIdx.x] = make_float2(ref, ls);
+                    pr_fold<HD, false>(to, r.ref, r.less(), held, nb > FOLD);
+                    pr_part<HD>::stats(static_cast<float*>(held->out))[threadIdx.x] = make_float2(r.ref, ls);
                 } else {
-                    if (nb > FOLD) pr_unfold<HD, !F32>(to, ref, held);
+                    if (nb > FOLD) pr_unfold<HD, !F32>(to, r.ref, r.more(), held);
                     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
                     // through the tile's q (no longer read), 16 bytes at a time, so that whole rows are written at once
                     constexpr int VPC = 16 / sizeof(T), CPR = HD / VPC;  // values of a piece, pieces of a row
@@ -568,7 +664,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                         float o[16];
                         tc_ld16(to + 16 * q, o);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = ls == 0.0f ? 0.0f : o[i] * inv;
+                        for (int i = 0; i < 16; i++) o[i] = ls == 0.0f ? 0.0f : o[i] * (q < 4 ? inv : inv * r.less());
 #pragma unroll
                         for (int i = 0; i < 16; i += VPC) {
                             const int p = (16 * q + i) / VPC;
@@ -609,7 +705,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             if (!pr_wait(&sh.raw_full[s], j >> 1 & 1, a.err, abort)) break;
             if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, a.err, abort)) break;
             pr_unpack<HD>(raw + s * BLK, smem + SM::k + s * SM::KTILE, smem + SM::v + s * SM::VTILE,
-                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.top[s], factor, len - off - j * kKv4Rows, tid);
+                          reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.range[s], factor, len - off - j * kKv4Rows, tid);
             fence_proxy_async_smem();  // the operands to the tensor cores, the reads before the next copy
             __syncwarp();
             if (lane == 0) {

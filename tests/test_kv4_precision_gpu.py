@@ -84,6 +84,16 @@ def _exact(q, k, v, scale, rows=None):
     return out, M, ds, top
 
 
+def _close(got, want, M, ds, top, n):
+    """fp32 results within both bounds."""
+    err, some = (got.double() - want).abs(), M > 0
+    assert torch.isfinite(got).all() and (err[~some] == 0).all()
+    bad = err > (4 * ds + (2 * n + 64) * E) * M + E * want.abs()
+    assert not bad.any(), (bad.sum().item(), (err / M.clamp_min(1e-300)).amax().item())
+    rms = (err / torch.where(some, M, 1.0)).pow(2).mean().sqrt().item()
+    assert rms <= 64 * E * max(1.0, top), rms
+
+
 def _step_of(x, t):
     """The distance of the type's numbers around x."""
     e = torch.frexp(x.abs().clamp_min(1e-30))[1].double() - 1
@@ -100,6 +110,12 @@ def _nearest(got, want, M, ds, top, n, t):
     off = (got != want.to(DT[t])).double()
     allowed = share.sum().item()
     assert off.sum().item() <= allowed + 5 * math.sqrt(allowed) + 3, (off.sum().item(), allowed, off.numel())
+
+
+def _sampled(B, T, rows):
+    b = torch.tensor([0, B - 1] if B > 1 else [0])
+    r = torch.unique(torch.linspace(0, T - 1, min(rows, T)).long()).cuda()
+    return b, r
 
 
 # ---------------------------------------------------------------------------
@@ -233,3 +249,115 @@ def test_scores_past_the_fraction_of_a_float(T, size):
     assert (kk[3, :, 0] > kk[torch.arange(n) != 3][:, :, 0].amax()).all()
     want = vv[3].repeat_interleave(H // kv, 0)
     assert (got[0].double() - want).abs().amax() <= 8 * E * want.abs().amax()
+
+
+# ---------------------------------------------------------------------------
+# V rows of very different size
+
+FORMS = [  # B, T, H, kv, hd, lens
+    (2, 1, 8, 2, 128, [333, 90]), (2, 1, 8, 2, 64, [333, 90]), (200, 1, 8, 8, 64, [20 + (31 * b) % 231 for b in range(200)]),
+    (40, 1, 16, 4, 128, [20 + (211 * b) % 1481 for b in range(40)]), (3, 24, 8, 2, 128, [500, 90, 30]),
+    (2, 90, 32, 2, 128, [1500, 1000]), (1, 90, 32, 2, 64, [1500]), (2, 720, 8, 2, 128, [1333, 730]),
+    (3, 1000, 16, 4, 64, [1100, 1000, 1024]),
+]
+
+
+def _spread_case(B, T, H, kv, hd, lens, seed, make):
+    """Attention of one row's size of scores over rows that make(v, n) scales; key 5 of every
+    sequence (and what make returns as hidden) has a score of some -130 in base 2."""
+    from joule_b200 import kv4
+    g = _gen(seed)
+    rows = []
+    for n in lens:
+        k = torch.randn(n, kv, hd, device="cuda", generator=g) * 0.5
+        v = torch.randn(n, kv, hd, device="cuda", generator=g)
+        k[..., 0] = 0.0
+        for j, x in make(v, n).items():
+            k[j, :, 0] = x
+        rows.append((k, v))
+    cache = _cache(rows)
+    q = torch.randn(B, T, H, hd, device="cuda", generator=g)
+    q[..., 0] = 1.0
+    got = kv4.kv4_attention(cache, 0, q, _i32(range(B)), _i32(lens), scale=0.1)
+    for b, n in enumerate(lens):
+        # (the keys with an outlier are exact in element 0 alone; scores are those of the held keys)
+        want, M, ds, top = _exact(q[b], *_held(cache, b, n), 0.1)
+        yield got[b], want, M, ds, n
+
+
+def _check_spread(B, T, H, kv, hd, lens, seed, make):
+    for got, want, M, ds, n in _spread_case(B, T, H, kv, hd, lens, seed, make):
+        # the hidden keys' scores carry no weight: those of the others are below 4
+        err, some = (got.double() - want).abs(), M > 0
+        assert torch.isfinite(got).all()
+        assert not (err > (4 * ds + (2 * n + 64) * E) * M + E * want.abs()).any(), (err / M).amax()
+        rms = (err / torch.where(some, M, 1.0)).pow(2).mean().sqrt().item()
+        assert rms <= 64 * E * 4.0, rms
+
+
+@pytest.mark.parametrize("factor", [1e3, 1e5, 1e7, 1e9])
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", FORMS)
+def test_a_large_row_without_weight(B, T, H, kv, hd, lens, factor):
+    """A V row of 1e5 whose weight is nothing beside rows smaller by the factor."""
+    def make(v, n):
+        v *= 1e5 / factor
+        v[5] = v[5].sign() * 1e5
+        return {5: -1000.0}
+    _check_spread(B, T, H, kv, hd, lens, 40, make)
+
+
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", FORMS)
+def test_groups_of_different_size(B, T, H, kv, hd, lens):
+    """The two groups of a head, and the kv heads, differ by 1e8; rows by powers of ten."""
+    def make(v, n):
+        v *= 10 ** torch.linspace(-1, 1, n, device="cuda")[torch.randperm(n, device="cuda", generator=_gen(n))][:, None, None]
+        v[..., 64:] *= 1e-4
+        v[..., :64] *= 1e4
+        v[:, ::2] *= 0.01
+        return {5: -1000.0}
+    _check_spread(B, T, H, kv, hd, lens, 41, make)
+
+
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", FORMS)
+def test_a_key_of_all_weight_with_values_of_zero(B, T, H, kv, hd, lens):
+    """The first position takes the weight by a factor of e^20 and has no value; what is
+    left is that small sum of the others' values."""
+    def make(v, n):
+        v[0] = 0.0
+        return {0: 200.0}
+    for got, want, M, ds, n in _spread_case(B, T, H, kv, hd, lens, 42, make):
+        err = (got.double() - want).abs()
+        assert not (err > (4 * ds + (2 * n + 64) * E) * M + E * want.abs()).any()
+        rms = (err / torch.where(M > 0, M, 1.0)).pow(2).mean().sqrt().item()
+        assert rms <= 64 * E * 24.0, rms
+
+
+@pytest.mark.parametrize("T,H,kv,hd,n", [(5, 8, 2, 128, 300), (24, 8, 1, 64, 70), (90, 32, 2, 128, 1500), (720, 32, 4, 128, 1333)])
+def test_a_later_row_does_not_change_an_earlier_result(T, H, kv, hd, n):
+    """Query i's digits do not depend on the values of positions that it does not see."""
+    from joule_b200 import kv4
+    g = _gen(43)
+    k, v = (torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2))
+    q = torch.randn(1, T, H, hd, device="cuda", generator=g)
+    got = []
+    for x in (1.0, 1e5):
+        v[n - 3:] *= x
+        got.append(kv4.kv4_attention(_cache([(k, v)]), 0, q, _i32([0]), _i32([n])))
+    assert torch.equal(got[0][:, :T - 3], got[1][:, :T - 3])
+    assert not torch.equal(got[0][:, T - 3:], got[1][:, T - 3:])
+
+
+@pytest.mark.parametrize("B,T,H,kv,hd,n", [(1, 1, 32, 4, 128, 131072), (1, 64, 32, 4, 128, 50000), (1, 1184, 32, 4, 128, 23000)])
+def test_sizes_that_change_from_block_to_block(B, T, H, kv, hd, n):
+    """V's size rises and falls by 2^10 from one block to the next, so that references move
+    by V's scales alone, across folds and joins."""
+    from joule_b200 import kv4
+    g = _gen(n)
+    k, v = (torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2))
+    v *= torch.exp2(10.0 * ((torch.arange(n, device="cuda") // 64 * 7919) % 11 % 3 - 1).float())[:, None, None]
+    cache = _cache([(k, v)])
+    q = torch.randn(B, T, H, hd, device="cuda", generator=g)
+    got = kv4.kv4_attention(cache, 0, q, _i32([0] * B), _i32([n] * B))
+    _, r = _sampled(B, T, 16)
+    want, M, ds, top = _exact(q[0], *_held(cache, 0, n), hd ** -0.5, r)
+    _close(got[0][r], want, M, ds, top, n)
