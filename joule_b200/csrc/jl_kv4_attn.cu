@@ -146,7 +146,7 @@ struct kv4_state {
     uint32_t qf[NG * 4][4];  // q of row g per step of 16 values
     float f;                 // accumulator -> score in base 2 (a power of two)
     kv4_ref<NG == 2> r;      // row g's references
-    float2 l;                // this thread's sum of row g's weights
+    kv4_sum l;               // this thread's sum of row g's weights
     float o[NG][4][4];       // o[gr][i][c]: value 64 gr + 8 g + 2 i + c / 2 of row 2 t + c % 2
     int n;                   // positions that row g sees
 };
@@ -195,7 +195,7 @@ __device__ __forceinline__ void kv4_load_q(kv4_state<HD>& st, const T* q, float 
             for (int c = 0; c < 4; c++) st.o[g][i][c] = 0.0f;
     }
     st.r.clear();
-    st.l = f2(0.0f);
+    st.l.clear();
 }
 
 // Scores in base 2 of positions r0 .. r0 + 15 of a block: s[h] = those of
@@ -258,7 +258,7 @@ __device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, f
         if (HD == 128) b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, o));
     }
     const float2 al = st.r.past(mx, b0, b1) ? st.r.move(mx, b0, b1) : f2(1.0f);
-    st.l = __fmul2_rn(st.l, f2(al.x));
+    st.l.scale(al.x);
 #pragma unroll
     for (int gr = 0; gr < HD / 64; gr++) {
         const float x = gr ? al.y : al.x;
@@ -271,10 +271,10 @@ __device__ __forceinline__ void kv4_new_reference(kv4_state<HD>& st, float mx, f
 }
 
 // Weights of positions r0 .. r0 + 15 from their scores, and the weighted values
-// onto the sums. V's scale multiplies the weight in fp32. MASK: row g does not see
+// onto the sums; adds the weights to l. V's scale multiplies the weight in fp32. MASK: row g does not see
 // positions from n on (in the block's numbering); those may hold any scale.
 template <int HD, bool MASK>
-__device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], int n) {
+__device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk, int r0, float2 (&s)[2], float2& l, int n) {
     constexpr int NG = HD / 64, ROW = HD / 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t bh[NG][2], bl[NG][2];
@@ -285,7 +285,7 @@ __device__ __forceinline__ void kv4_values(kv4_state<HD>& st, const uint8_t* blk
         s[h] = __fadd2_rn(s[h], f2(st.r.minus()));
         s[h].x = ex2(s[h].x);
         s[h].y = ex2(s[h].y);
-        st.l = __fadd2_rn(st.l, s[h]);
+        l = __fadd2_rn(l, s[h]);
 #pragma unroll
         for (int gr = 0; gr < NG; gr++) {
             float2 w = __fmul2_rn(s[h], sc[gr]);
@@ -363,7 +363,7 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
         most = __reduce_max_sync(0xffffffffu, most);
         if (!kv4_spread(most, __reduce_min_sync(0xffffffffu, least))) {
             const float top = kv4_top(most);
-            float2 s[4][2];
+            float2 s[4][2], l = f2(0.0f);
             float mx = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -372,14 +372,15 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
             }
             if (__any_sync(0xffffffffu, st.r.past(mx, top, top))) kv4_new_reference<HD>(st, mx, top, top);
 #pragma unroll
-            for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], 0);
+            for (int k = 0; k < 4; k++) kv4_values<HD, false>(st, blk, 16 * k, s[k], l, 0);
+            st.l.add(l);
             return;
         }
     }
     const int n = st.n - j0;
 #pragma unroll 1
     for (int r0 = 0; r0 < min(kKv4Rows, n_max - j0); r0 += 16) {
-        float2 s[2];
+        float2 s[2], l = f2(0.0f);
         kv4_scores<HD>(st, blk, r0, s);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -398,7 +399,8 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
                 b[gr] = fmaxf(b[gr], fmaxf((s[h].x - mx) + exponent_of(sc[gr].x), (s[h].y - mx) + exponent_of(sc[gr].y)));
         }
         if (__any_sync(0xffffffffu, st.r.past(mx, b[0], b[1]))) kv4_new_reference<HD>(st, mx, b[0], b[1]);
-        kv4_values<HD, true>(st, blk, r0, s, n);
+        kv4_values<HD, true>(st, blk, r0, s, l, n);
+        st.l.add(l);
     }
 }
 
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
         issue();
         const bool ends = co.j == co.nu - 1;
         if (ends || i == units - 1) {
-            float lrow = st.l.x + st.l.y;
+            float lrow = st.l.total();
             lrow += __shfl_xor_sync(0xffffffffu, lrow, 1);
             lrow += __shfl_xor_sync(0xffffffffu, lrow, 2);
             const float2 lsum = make_float2(__shfl_sync(0xffffffffu, lrow, 8 * t), __shfl_sync(0xffffffffu, lrow, 8 * t + 4));

@@ -395,12 +395,12 @@ __device__ __forceinline__ void pr_mask(float2* x, int n) {
 }
 
 // Weights of a block, 16 positions at a time, times V's scales of a group (MORE: and the
-// second group's factor), hi and lo, into S's place; adds them to lsum.
+// second group's factor), hi and lo, into S's place; returns their sum.
 template <int HD, bool MORE>
-__device__ __forceinline__ void pr_weights(uint32_t ts, const float* sc, const float2 (&x)[32], float f, float minus, float more,
-                                           float2& lsum) {
+__device__ __forceinline__ float2 pr_weights(uint32_t ts, const float* sc, const float2 (&x)[32], float f, float minus, float more) {
     constexpr int NG = HD / 64;
     const float2 nr = f2(minus), ff = f2(f);
+    float2 sum;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         float4 v0[4], v1[4];
@@ -415,7 +415,7 @@ __device__ __forceinline__ void pr_weights(uint32_t ts, const float* sc, const f
             float2 p = __ffma2_rn(x[8 * q + i], ff, nr);
             p.x = ex2(p.x);
             p.y = ex2(p.y);
-            lsum = __fadd2_rn(lsum, p);
+            sum = q + i ? __fadd2_rn(sum, p) : p;
             const float4 w0 = v0[i / 2], w1 = NG == 2 ? v1[i / 2] : w0;
             const float2 y0 = __fmul2_rn(p, i & 1 ? make_float2(w0.z, w0.w) : make_float2(w0.x, w0.y));
             split2(y0, hi[0][i], lo[0][i]);
@@ -431,6 +431,7 @@ __device__ __forceinline__ void pr_weights(uint32_t ts, const float* sc, const f
             tc_st8(ts + 64 * g + 32 + 8 * q, lo[g]);
         }
     }
+    return sum;
 }
 
 // Exponents above a row's products with the scales of each group in a block (kv4_ref), from
@@ -477,7 +478,7 @@ __device__ __noinline__ float2 pr_products(uint32_t ts, float f, const float* sc
 template <int HD>
 struct pr_run {
     kv4_ref<HD == 128> r;
-    float2 lsum;
+    kv4_sum lsum;
     int j;  // -1: not ok
 };
 template <int HD, bool F32, bool MORE>
@@ -517,7 +518,7 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t,
         const bool past = st.r.past(mx, bound.x, bound.y);  // a product past the limit, or the row's first
         if (__any_sync(0xffffffffu, past)) {
             const float2 al = past ? st.r.move(mx, bound.x, bound.y) : f2(1.0f);
-            st.lsum = __fmul2_rn(st.lsum, f2(al.x));
+            st.lsum.scale(al.x);
             if (!starts) {  // the sums of earlier blocks are complete (S was issued after them)
 #pragma unroll 1
                 for (int q = 0; q < NG * 4; q++) {
@@ -531,7 +532,7 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t,
             }
             if (NG == 2 && !MORE && __any_sync(0xffffffffu, st.r.lifted())) break;
         }
-        pr_weights<HD, MORE>(ts, sc, x, f, st.r.minus(), MORE ? st.r.more() : 1.0f, st.lsum);
+        st.lsum.add(pr_weights<HD, MORE>(ts, sc, x, f, st.r.minus(), MORE ? st.r.more() : 1.0f));
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -637,14 +638,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             const int n_row = sees(row) - off, n_min = sees(row0 + t * kPrTile) - off;
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * SM::TCOLS, to = ts + SM::SCOLS;
             pr_run<HD> st;
-            st.r.clear(), st.lsum = f2(0.0f), st.j = 0;
+            st.r.clear(), st.lsum.clear(), st.j = 0;
             st = pr_softmax<HD, F32, false>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
             if (st.j >= 0 && st.j < nb) st = pr_softmax_lifted<HD, F32>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
             const kv4_ref<NG == 2> r = st.r;
-            const float2 lsum = st.lsum;
             if (st.j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
                 tc_fence_after();
-                const float ls = lsum.x + lsum.y;
+                const float ls = st.lsum.total();
                 int tx = threadIdx.x;
                 asm volatile("" : "+r"(tx));  // the row's place again (kept over the loop it took registers)
                 const int row = row0 + tx, rc = min(row, rows - 1), h = kh * gsz + rc % gsz;

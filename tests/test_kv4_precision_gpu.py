@@ -361,3 +361,41 @@ def test_sizes_that_change_from_block_to_block(B, T, H, kv, hd, n):
     _, r = _sampled(B, T, 16)
     want, M, ds, top = _exact(q[0], *_held(cache, 0, n), hd ** -0.5, r)
     _close(got[0][r], want, M, ds, top, n)
+
+
+# ---------------------------------------------------------------------------
+# long histories
+
+LONG = [  # B, T, H, kv, hd, n: a cut (few and many blocks to a warp), a prompt in splits, two whole ones
+    (1, 1, 32, 4, 128, 131072), (64, 1, 32, 4, 128, 131072), (8, 1, 8, 8, 64, 50000), (1, 64, 32, 4, 128, 131072),
+    (1, 1184, 32, 4, 128, 23000), (1, 2368, 16, 4, 64, 131072),
+]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("B,T,H,kv,hd,n", LONG)
+def test_nothing_grows_with_the_length(B, T, H, kv, hd, n, t):
+    """One key ahead and all others equal: every weight of the sum rounds the same way.
+    The output's part along the exact one is off by no more than a fixed bound: sums of 64
+    weights (32 roundings in a row, 16 e), the block's into a total that keeps what it
+    rounds off, products cut off rather than rounded over at most 8 blocks (16-bit calls:
+    32) of 64 positions, measured at 1.6e-7 a block: 4e-6 in fp32; 16 bits add 6e-6."""
+    from joule_b200 import kv4
+    g = _gen(n + T)
+    k = torch.randn(1, kv, hd, device="cuda", generator=g).expand(n, kv, hd).contiguous()
+    k[7] *= 1.5
+    v = torch.rand(n, kv, hd, device="cuda", generator=g) + 0.5
+    cache = _cache([(k, v)])
+    kk, vv = _held(cache, 0, n)
+    q = (kk[0].float().repeat_interleave(H // kv, 0) * 0.05 * (1 + torch.rand(B, T, H, 1, device="cuda", generator=g))).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32([0] * B), _i32([n] * B), scale=1.0)
+    bs, r = _sampled(B, T, 24)
+    num = den = 0.0
+    for b in bs.tolist():
+        want = _exact(q[b], kk, vv, 1.0, r)[0]
+        num += ((got[b][r].double() - want) * want).sum().item()
+        den += (want * want).sum().item()
+        if t == "f32":
+            assert ((got[b][r].double() - want).abs() <= 2e-5 * want.abs()).all()
+    # 16-bit results of equal weights repeat from row to row: kv * hd independent roundings
+    assert abs(num / den) <= 4e-6 + (6e-6 + 5 * 2.0 ** -12 / math.sqrt(3 * kv * hd) if t == "f16" else 0.0), num / den
