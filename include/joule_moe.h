@@ -553,7 +553,8 @@ int jl_kv4_read(const jl_kv4* c, int l, const int* slots, const int* positions, 
  * that sees nothing is 0. T = 1 is a decode step, T > 1 a piece of a prompt.
  * `longest` is a bound that the caller knows of the lens (0: maxT); a length
  * outside [0, longest] or a slot outside the cache gives zeros and the status
- * bit (and a wait inside the call that ran out sets bit 1, with out undefined).
+ * bit. A wait inside the call that ran out leaves out undefined and sets bit 1
+ * of dev_status, or, in a call without one, is reported by jl_kv4_check.
  * out does not overlap q's rows or what lies between them, nor the other buffers.
  * ws: jl_kv4_attn_ws(c, B, T, H, longest) bytes of device memory (asked on the
  * call's device; 0: none, as where longest is 1 to 256), 16-byte aligned, used
@@ -565,6 +566,17 @@ int jl_kv4_attn(const jl_kv4* c, int l, const void* q, int dtype, long long q_st
                 const int* slots, const int* lens, int longest, int B, int T, int H,
                 float scale, void* out, void* ws, long long ws_bytes, int* dev_status,
                 void* stream);
+
+/* Waits for the stream's calls; JL_ERR_TIMEOUT when a wait inside a jl_kv4_attn
+ * call without dev_status on the current device has run out since the last
+ * check (whose output is then not valid), JL_OK otherwise. */
+int jl_kv4_check(void* stream);
+
+/* Bound of each wait inside jl_kv4_attn's kernels, in nanoseconds, for calls
+ * launched from then on (default about 2 s; 0: every wait gives up at once,
+ * to test what is done about it). The waits are on the kernel's own copies and
+ * products, microseconds away. */
+int jl_kv4_set_wait_limit(long long ns);
 
 /* The cache of a decoder created with JL_DEC_KV4 (its buffer stays the
  * decoder's), for jl_kv4_read and the like. */

@@ -220,6 +220,7 @@ struct jl_kv4_attn_args {
     int* err;      // status word (kErrKvIndex), or null
     float scale;
     int dtype, len_add, longest, B, T, H, outT_ld;
+    long long wait_limit;  // SM cycles of a wait inside the tcgen05 form (set at its launch)
 };
 // The workspace of one call on the current device, and the most that any call on c needs.
 long long jl_kv4_attn_ws_bytes(const jl::kv4_dims& c, int B, int T, int H, int longest);

@@ -30,6 +30,7 @@
 // shared memory) and by the softmax's issue slots in 16 bits. 2,047 rows of 32/4 heads
 // of 128 over 4,100 positions, fp32: 313 us; 123 at the measured bf16 rate.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "jl_internal.h"
@@ -55,6 +56,8 @@ struct pr_bars {
     uint64_t s_full[2], p_full[2], pv_done[2], fin;
     uint32_t tmem;
     int abort;
+    int* err;         // of waits that ran out
+    long long limit;  // of a wait, in cycles
     uint2 range[2][2];  // per buffer, per warp of positions: bits of V's largest and smallest scale
 };
 
@@ -140,19 +143,23 @@ struct pr_smem {
     static_assert(sizeof(pr_bars) <= 512 && sizeof(pr_held) % 8 == 0 && total <= 227 * 1024, "shared memory");
 };
 
+// Where waits that ran out are recorded when the call has no status word.
+__device__ int g_kv4_status;
+
 // A wait of a whole warp, bounded; false when it ran out or another role gave up.
 // (mbarrier.test_wait in place of try_wait, polling without a suspension, was 6 %
 // slower: the polls take the softmax's issue slots.)
-__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
+__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, pr_bars& sh) {
     bool ok = mbar_try_wait(bar, parity);
     if (!ok) {
         const long long t0 = clock64();
         for (int i = 1; !ok; i++) {
             ok = mbar_try_wait(bar, parity);
             if (!ok && (i & 63) == 0) {
+                volatile int* abort = &sh.abort;
                 if (*abort) break;
-                if (clock64() - t0 > kWaitLimitCycles) {
-                    if (err) atomicOr(err, kErrTimeout);
+                if (clock64() - t0 > sh.limit) {
+                    atomicOr(sh.err, kErrTimeout);
                     *abort = 1;
                     break;
                 }
@@ -482,7 +489,7 @@ struct pr_run {
     int j;  // -1: not ok
 };
 template <int HD, bool F32, bool MORE>
-__device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t, uint32_t ts, float f, int nb, int S, int n_row,
+__device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int t, uint32_t ts, float f, int nb, int S, int n_row,
                                                  int n_min, pr_run<HD> st) {
     using SM = pr_smem<HD, F32>;
     constexpr int NG = SM::NG, FOLD = kPrFold<F32>;
@@ -493,7 +500,7 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t,
     for (; st.j < nb; st.j++) {
         const int j = st.j, s = j & 1, j0 = j * kKv4Rows;
         // the scales (kv_full), then the scores
-        if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, err, &sh.abort) || !pr_wait(&sh.s_full[t], j & 1, err, &sh.abort)) {
+        if (!pr_wait(&sh.kv_full[s], j >> 1 & 1, sh) || !pr_wait(&sh.s_full[t], j & 1, sh)) {
             st.j = -1;
             return st;
         }
@@ -542,9 +549,9 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int* err, int t,
 }
 // With factors: a call of its own (multiplying by them in all blocks took 4 % of a prompt).
 template <int HD, bool F32>
-__device__ __noinline__ pr_run<HD> pr_softmax_lifted(uint8_t* smem, int* err, int t, uint32_t ts, float f, int nb, int S, int n_row,
+__device__ __noinline__ pr_run<HD> pr_softmax_lifted(uint8_t* smem, int t, uint32_t ts, float f, int nb, int S, int n_row,
                                                      int n_min, pr_run<HD> st) {
-    return pr_softmax<HD, F32, true>(smem, err, t, ts, f, nb, S, n_row, n_min, st);
+    return pr_softmax<HD, F32, true>(smem, t, ts, f, nb, S, n_row, n_min, st);
 }
 
 template <int HD, typename T>
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     }
     pr_held* held = reinterpret_cast<pr_held*>(smem + SM::held);
     if (threadIdx.x == 0) {
-        sh.abort = 0;
+        sh.abort = 0, sh.err = a.err ? a.err : &g_kv4_status, sh.limit = a.wait_limit;
         if (S > 1) {
             held->out = pr_part<HD>::of(a.ws, blockIdx.x), held->H = held->gsz = 1, held->row0 = 0, held->rows = kPrPair;
         } else {
@@ -618,8 +625,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    const bool gives_up = a.wait_limit == 0;  // every role leaves at its first wait
+    if (gives_up && threadIdx.x == 0) atomicOr(sh.err, kErrTimeout);
     auto starts = [](int j) { return j % FOLD == 0; };  // blocks at which TMEM's sums start anew
-    volatile int* abort = &sh.abort;
 
     if (warp < 8) {
         // ---------------- softmax: thread = row of tile t = TMEM lane
@@ -639,10 +647,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * SM::TCOLS, to = ts + SM::SCOLS;
             pr_run<HD> st;
             st.r.clear(), st.lsum.clear(), st.j = 0;
-            st = pr_softmax<HD, F32, false>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
-            if (st.j >= 0 && st.j < nb) st = pr_softmax_lifted<HD, F32>(smem, a.err, t, ts, f, nb, S, n_row, n_min, st);
+            if (gives_up) st.j = -1;
+            else st = pr_softmax<HD, F32, false>(smem, t, ts, f, nb, S, n_row, n_min, st);
+            if (st.j >= 0 && st.j < nb) st = pr_softmax_lifted<HD, F32>(smem, t, ts, f, nb, S, n_row, n_min, st);
             const kv4_ref<NG == 2> r = st.r;
-            if (st.j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, a.err, abort)) {
+            if (st.j == nb && pr_wait(&sh.pv_done[t], (nb - 1) & 1, sh)) {
                 tc_fence_after();
                 const float ls = st.lsum.total();
                 int tx = threadIdx.x;
@@ -702,8 +711,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         __syncwarp();
         for (; j < nb; j++) {
             const int s = j & 1;
-            if (!pr_wait(&sh.raw_full[s], j >> 1 & 1, a.err, abort)) break;
-            if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, a.err, abort)) break;
+            if (gives_up || !pr_wait(&sh.raw_full[s], j >> 1 & 1, sh)) break;
+            if (j >= 2 && !pr_wait(&sh.kv_empty[s], (j >> 1) + 1 & 1, sh)) break;
             pr_unpack<HD>(raw + s * BLK, smem + SM::k + s * SM::KTILE, smem + SM::v + s * SM::VTILE,
                           reinterpret_cast<float*>(smem + SM::sc) + s * 4 * kKv4Rows, sh.range[s], factor, len - off - j * kKv4Rows, tid);
             fence_proxy_async_smem();  // the operands to the tensor cores, the reads before the next copy
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 mbar_arrive(&sh.raw_empty[s]);
             }
             if (w == 0 && j + 2 < nb) {
-                if (!pr_wait(&sh.raw_empty[s], j >> 1 & 1, a.err, abort)) {
+                if (!pr_wait(&sh.raw_empty[s], j >> 1 & 1, sh)) {
                     j++;
                     break;
                 }
@@ -722,7 +731,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             }
         }
         if (tid == 0)
-            for (; j < issued; j++) mbar_wait_bounded(&sh.raw_full[j & 1], j >> 1 & 1, a.err);  // no copy left in flight
+            for (; j < issued; j++) mbar_wait_bounded(&sh.raw_full[j & 1], j >> 1 & 1, sh.err);  // no copy left in flight
     } else {
         // ---------------- the instructions (a whole warp, one elected lane issues). The
         // tiles take turns: a tile's values and its next scores go out together, and
@@ -732,7 +741,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
         const uint64_t kd = umma_desc(smem + SM::k, 1024, 128);
         const uint64_t vd = umma_desc(smem + SM::v, 8 * kPrCore, kPrCore);
         auto scores = [&](int t, int j) {
-            if (!pr_wait(&sh.kv_full[j & 1], j >> 1 & 1, a.err, abort)) return false;
+            if (!pr_wait(&sh.kv_full[j & 1], j >> 1 & 1, sh)) return false;
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t qd = umma_desc(smem + SM::q + t * PARTS * SM::QTILE, SM::QCHUNK, 128);
@@ -749,12 +758,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             __syncwarp();
             return true;
         };
-        bool ok = pr_wait(&sh.q_full, 0, a.err, abort);
+        bool ok = !gives_up && pr_wait(&sh.q_full, 0, sh);
         for (int t = 0; ok && t < tiles; t++) ok = scores(t, 0);
         for (int j = 0; ok && j < nb; j++)
             for (int t = 0; ok && t < tiles; t++) {
                 const int s = j & 1;
-                if (!pr_wait(&sh.p_full[t], j & 1, a.err, abort)) {
+                if (!pr_wait(&sh.p_full[t], j & 1, sh)) {
                     ok = false;
                     break;
                 }
@@ -776,11 +785,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                 }
                 __syncwarp();
                 // the next scores go where these weights are: after the product that reads them
-                if (j + 1 < nb) ok = pr_wait(&sh.pv_done[t], j & 1, a.err, abort) && scores(t, j + 1);
+                if (j + 1 < nb) ok = pr_wait(&sh.pv_done[t], j & 1, sh) && scores(t, j + 1);
             }
         if (elect_one()) tc_commit(&sh.fin);  // no instruction left in flight
         __syncwarp();
-        mbar_wait_bounded(&sh.fin, 0, a.err);
+        mbar_wait_bounded(&sh.fin, 0, sh.err);
     }
     tc_fence_before();
     __syncthreads();
@@ -855,6 +864,8 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_merge(kv4_dims c, jl_kv4_att
 
 namespace {
 
+std::atomic<long long> g_wait_limit{jl::kWaitLimitCycles};
+
 template <int HD, typename T>
 int launch_t(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, int S, cudaStream_t s) {
     using namespace jl;
@@ -888,7 +899,9 @@ long long jl_kv4_prompt_ws_bytes(const jl::kv4_dims& c, long long units, int S) 
     return S > 1 ? units * S * (c.hd == 64 ? jl::pr_part<64>::floats : jl::pr_part<128>::floats) * (long long)sizeof(float) : 0;
 }
 
-int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a, int S, cudaStream_t s) {
+int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& args, int S, cudaStream_t s) {
+    jl_kv4_attn_args a = args;
+    a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
     const int rc = jl_device_once(kOnceKv4Prompt, [] {
         const int r = prompt_attrs<64>();
         return r ? r : prompt_attrs<128>();
@@ -897,4 +910,23 @@ int jl_launch_kv4_prompt(const jl::kv4_dims& c, int l, const jl_kv4_attn_args& a
     if (a.dtype == JL_F32) return c.hd == 64 ? launch_t<64, float>(c, l, a, S, s) : launch_t<128, float>(c, l, a, S, s);
     if (a.dtype == JL_F16) return c.hd == 64 ? launch_t<64, __half>(c, l, a, S, s) : launch_t<128, __half>(c, l, a, S, s);
     return c.hd == 64 ? launch_t<64, __nv_bfloat16>(c, l, a, S, s) : launch_t<128, __nv_bfloat16>(c, l, a, S, s);
+}
+
+extern "C" int jl_kv4_set_wait_limit(long long ns) {
+    if (ns < 0) return JL_ERR_INVALID;
+    // clock64 counts SM cycles; 2 a ns bound a wait by at least `ns` at any SM clock up to 2 GHz
+    g_wait_limit.store(ns > (1ll << 61) ? 1ll << 62 : 2 * ns, std::memory_order_relaxed);
+    return JL_OK;
+}
+
+extern "C" int jl_kv4_check(void* stream) {
+    cudaStream_t s = (cudaStream_t)stream;
+    int err = 0;
+    JL_CUDA(cudaMemcpyFromSymbolAsync(&err, jl::g_kv4_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    JL_CUDA(cudaStreamSynchronize(s));
+    if (!err) return JL_OK;
+    const int zero = 0;
+    JL_CUDA(cudaMemcpyToSymbolAsync(jl::g_kv4_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+    JL_CUDA(cudaStreamSynchronize(s));
+    return JL_ERR_TIMEOUT;
 }

@@ -13,7 +13,10 @@ Calls run on the cache's device, on the current stream there or the one given;
 all of them can be captured into CUDA graphs. Nothing is checked on the
 device's side of a call but what would leave the cache: a slot, position or
 length outside it skips the row (append) or reads as zeros, and sets bit 8 of
-``status`` (an int32 CUDA tensor of one element) when one is given.
+``status`` (an int32 CUDA tensor of one element) when one is given. A wait inside
+an attention kernel that runs out (about 2 s, where microseconds are due) leaves
+the output undefined: it sets bit 1 of ``status``, and without one the next
+``kv4_check`` raises.
 """
 from __future__ import annotations
 
@@ -24,9 +27,11 @@ import torch
 
 from joule_b200.native import BF16, F16, F32, Kv4, check, get_dll
 
-__all__ = ["KV4_BLOCK", "KV4_BAD_INDEX", "kv4_cache", "kv4_append", "kv4_read", "kv4_attention"]
+__all__ = ["KV4_BLOCK", "KV4_TIMEOUT", "KV4_BAD_INDEX", "kv4_cache", "kv4_append", "kv4_read", "kv4_attention",
+           "kv4_check"]
 
 KV4_BLOCK = 64      # positions per block
+KV4_TIMEOUT = 1     # status bit: a wait inside a kernel ran out, the output is not valid
 KV4_BAD_INDEX = 8   # status bit: a slot, position or length outside the cache
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -244,3 +249,15 @@ def kv4_attention(cache: torch.Tensor, l: int, q: torch.Tensor, slots: torch.Ten
     check(_dll.jl_kv4_attn(c, l, pq, kind, row, ps, pl, longest, B, T, H, 1.0 / math.sqrt(hd) if scale is None else scale,
                            out.data_ptr(), ws.data_ptr() if n else None, n, st, _raw_stream(dev)), "jl_kv4_attn")
     return out
+
+
+def kv4_check(device=None, stream=None) -> None:
+    """Wait for the stream (the current one of `device`, the current CUDA device by
+    default) and raise JouleError when a wait inside a kv4_attention call without
+    `status` on the device has run out since the last check."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"kv4_check: a CUDA device, got {device}")
+    with torch.cuda.device(device):
+        s = torch.cuda.current_stream() if stream is None else _other(torch.cuda.current_device(), stream)
+        check(get_dll().jl_kv4_check(s.cuda_stream), "jl_kv4_check")

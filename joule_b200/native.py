@@ -138,6 +138,8 @@ SIGNATURES = {
     "jl_kv4_attn_ws": ([ctypes.POINTER(Kv4), _I, _I, _I, _I], _LL),
     "jl_kv4_attn": ([ctypes.POINTER(Kv4), _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _LL,
                      _P, _P], _I),
+    "jl_kv4_check": ([_P], _I),
+    "jl_kv4_set_wait_limit": ([_LL], _I),
     "jl_dec_kv4": ([_P, ctypes.POINTER(Kv4)], _I),
     "jl_version": ([], ctypes.c_char_p),
     "jl_last_cuda_error": ([], ctypes.c_char_p),

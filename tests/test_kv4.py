@@ -161,3 +161,9 @@ def test_the_compiled_calls_pass_on_what_is_not_regular():
     assert call.read(cache, 0, i, i, torch.float64) is None
     with pytest.raises(TypeError):
         call.bind(1)
+
+
+def test_wait_limits_and_devices_are_checked(dll):
+    assert dll.jl_kv4_set_wait_limit(-1) == -1
+    with pytest.raises(ValueError):
+        kv4.kv4_check("cpu")
