@@ -79,6 +79,7 @@ class Decoder:
                                        1 if src_on_device else 0, DEC_KV4 if kv4 else 0, ctypes.byref(h)),
               "jl_dec_create_ex")
         self.h = h
+        self.device = torch.device("cuda", torch.cuda.current_device())
         moe = ctypes.c_void_p()
         check(self._L.jl_dec_moe(h, ctypes.byref(moe)), "jl_dec_moe")
         self.moe = moe
@@ -142,11 +143,12 @@ class Decoder:
 
     def kv4_cache(self) -> torch.Tensor:
         """The 4-bit cache of a decoder created with kv4=True as the uint8 tensor
-        that joule_b200.kv4 takes (the decoder's own memory, not a copy)."""
+        that joule_b200.kv4 takes (the decoder's own memory, not a copy: not to be
+        used after close())."""
         c = Kv4()
         check(self._L.jl_dec_kv4(self.h, ctypes.byref(c)), "jl_dec_kv4")
         shape = (c.slots, c.L, c.n_kv, -(-c.maxT // 64), 68 * c.hd)
-        return torch.as_tensor(_Buffer(c.base, shape, self), device="cuda")
+        return torch.as_tensor(_Buffer(c.base, shape, self), device=self.device)
 
     # -- the step -----------------------------------------------------------
     def embed(self, tokens: torch.Tensor, x: torch.Tensor, stream=None) -> torch.Tensor:

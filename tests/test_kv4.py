@@ -167,3 +167,24 @@ def test_wait_limits_and_devices_are_checked(dll):
     assert dll.jl_kv4_set_wait_limit(-1) == -1
     with pytest.raises(ValueError):
         kv4.kv4_check("cpu")
+
+
+def test_the_decoders_cache_is_on_its_own_device(monkeypatch):
+    """Decoder.kv4_cache asks for the device that the decoder was created on, whichever is
+    current; with the current one it would be a copy there."""
+    from joule_b200 import decoder
+
+    class Lib:
+        def jl_dec_kv4(self, h, c):
+            c._obj.base, c._obj.slots, c._obj.L, c._obj.n_kv, c._obj.hd, c._obj.maxT = 4096, 2, 1, 2, 64, 65
+            return 0
+
+        def jl_dec_destroy(self, h):
+            return 0
+    d = decoder.Decoder.__new__(decoder.Decoder)
+    d._L, d.h, d.device = Lib(), ctypes.c_void_p(1), torch.device("cuda", 3)
+    seen = {}
+    monkeypatch.setattr(decoder.torch, "as_tensor", lambda x, device=None: seen.update(x=x, device=device))
+    d.kv4_cache()
+    assert torch.device(seen["device"]) == torch.device("cuda", 3)
+    assert seen["x"].__cuda_array_interface__["shape"] == (2, 1, 2, 2, 68 * 64)
