@@ -6,7 +6,8 @@
 Each .cu under csrc/ compiles to an object in parallel; the objects link into
 one shared library with a static CUDA runtime. No torch headers are used:
 the library's ABI is plain C (include/joule_moe.h). csrc/kv4_call.c, which
-needs Python's headers alone, becomes joule_b200/_kv4_call.so.
+needs Python's headers alone, becomes joule_b200/_kv4_call with this interpreter's
+suffix (another one does not load it, and goes without).
 """
 from __future__ import annotations
 
@@ -23,7 +24,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libjoule_moe.so"
-CALL = PKG / "_kv4_call.so"
+CALL = PKG / f"_kv4_call{sysconfig.get_config_var('EXT_SUFFIX')}"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I", str(ROOT / "include"), "-I", str(CSRC)]
@@ -54,6 +55,7 @@ def _compile(src: Path, force: bool, extra: list[str]) -> Path:
 def _call_module(force: bool) -> None:
     src = CSRC / "kv4_call.c"
     deps = [src, ROOT / "include" / "joule_moe.h"]
+    (PKG / "_kv4_call.so").unlink(missing_ok=True)  # one without a suffix would be loaded by any interpreter
     if not force and CALL.exists() and CALL.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
         return
     cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")

@@ -51,6 +51,11 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle 
 _current_device = torch._C._cuda_getDevice
 
 
+class _Interpreted:
+    """In place of the compiled calls where this interpreter has none: nothing is regular."""
+    bind = append = read = attention = staticmethod(lambda *a: None)
+
+
 _call = None  # the compiled form of regular calls (csrc/kv4_call.c), bound at the first one
 _dll = None
 
@@ -60,8 +65,8 @@ def _bind() -> None:
     dll = get_dll()
     try:
         from joule_b200 import _kv4_call
-    except ImportError as e:
-        raise FileNotFoundError("joule_b200/_kv4_call.so is missing: run `python -m joule_b200.build`") from e
+    except ImportError:  # built for another Python: the functions below do all of it, some microseconds slower
+        _kv4_call = _Interpreted
     entries = [ctypes.cast(f, ctypes.c_void_p).value
                for f in (dll.jl_kv4_append, dll.jl_kv4_read, dll.jl_kv4_attn, dll.jl_kv4_attn_ws)]
     _kv4_call.bind(torch.uint8, torch.int32, torch.float32, torch.float16, torch.bfloat16, torch.empty_like,

@@ -188,3 +188,24 @@ def test_the_decoders_cache_is_on_its_own_device(monkeypatch):
     d.kv4_cache()
     assert torch.device(seen["device"]) == torch.device("cuda", 3)
     assert seen["x"].__cuda_array_interface__["shape"] == (2, 1, 2, 2, 68 * 64)
+
+
+def test_the_compiled_calls_belong_to_one_python_and_can_be_missing(monkeypatch):
+    """The module's file carries the interpreter's tag, so that no other one loads it, and
+    without it the Python functions do everything."""
+    import sys
+    import sysconfig
+
+    import joule_b200
+    from joule_b200 import build
+    assert build.CALL.name == "_kv4_call" + sysconfig.get_config_var("EXT_SUFFIX")
+    monkeypatch.delattr(joule_b200, "_kv4_call", raising=False)
+    monkeypatch.setitem(sys.modules, "joule_b200._kv4_call", None)
+    monkeypatch.setattr(kv4, "_call", None)
+    kv4._bind()
+    i, x = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, 64)
+    assert kv4._call is not None and kv4._call.append(x, 0, x, x, i, i) is None
+    for call in (lambda c: kv4.kv4_append(c, 0, x, x, i, i), lambda c: kv4.kv4_read(c, 0, i, i),
+                 lambda c: kv4.kv4_attention(c, 0, x, i, i)):
+        with pytest.raises(ValueError):
+            call(torch.zeros(2, 1, 2, 1, 68 * 64, dtype=torch.uint8))
