@@ -745,13 +745,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t qd = umma_desc(smem + SM::q + t * PARTS * SM::QTILE, SM::QCHUNK, 128);
+                // lo first: half of the cut-off sums are small then (a prompt's error 1.5e-6 -> 1.1e-6)
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
                     for (int p = 0; p < PARTS; p++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            tc_mma_ss(tmem + t * SM::TCOLS + 64 * g, qd + ((p * SM::QTILE + (g * 4 + k) * 2 * SM::QCHUNK) >> 4),
+                            tc_mma_ss(tmem + t * SM::TCOLS + 64 * g, qd + (((PARTS - 1 - p) * SM::QTILE + (g * 4 + k) * 2 * SM::QCHUNK) >> 4),
                                       kd + (((j & 1) * SM::KTILE + (g * 4 + k) * 2048) >> 4), idesc, p + k > 0);
                 tc_commit(&sh.s_full[t]);
             }
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) k_kv4_prompt(kv4_dims c, int l,
                         for (int p = 0; p < 2; p++)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                tc_mma_ts(to + 64 * g, ts + 64 * g + 32 * p + 8 * k,
+                                tc_mma_ts(to + 64 * g, ts + 64 * g + 32 * (1 - p) + 8 * k,
                                           vd + ((s * SM::VTILE + (g * 64 + k * 16) * kPrCore) >> 4), idesc,
                                           p + k > 0 || !fresh);
                     tc_commit(&sh.pv_done[t]);
