@@ -399,3 +399,48 @@ def test_nothing_grows_with_the_length(B, T, H, kv, hd, n, t):
             assert ((got[b][r].double() - want).abs() <= 2e-5 * want.abs()).all()
     # 16-bit results of equal weights repeat from row to row: kv * hd independent roundings
     assert abs(num / den) <= 4e-6 + (6e-6 + 5 * 2.0 ** -12 / math.sqrt(3 * kv * hd) if t == "f16" else 0.0), num / den
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,H,kv,hd,lens", [(4, 640, 15, 3, 128, [2500, 2300, 640, 0]), (6, 500, 14, 2, 64, [2400, 3000, 500, 499, 1, 2111]),
+                                              (1, 3, 1030, 1, 128, [4500])])
+def test_sums_in_places_of_odd_groups(B, T, H, kv, hd, lens, t):
+    """Units whose sums move to their rows of the output and back while they are computed:
+    groups of 5 and 7 heads, rows that end inside a warp, sequences shorter than the chunk."""
+    from joule_b200 import kv4
+    g = _gen(B + T)
+    rows = [tuple(torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2)) for n in lens]
+    cache = _cache(rows)
+    q = torch.randn(B, T, H, hd, device="cuda", generator=g).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32(range(B)), _i32(lens))
+    for b, n in enumerate(lens):
+        assert (got[b, :max(0, T - n)] == 0).all()
+        if n:
+            r = torch.unique(torch.cat([torch.arange(3), torch.linspace(0, T - 1, min(T, 40)).long()]).clamp_max(T - 1)).cuda()
+            want, M, ds, _ = _exact(q[b], *_held(cache, b, n), hd ** -0.5, r)
+            half = E * want.abs() if t == "f32" else _step_of(want, t) / 2 * (1 + 2.0 ** -20)
+            assert not ((got[b][r].double() - want).abs() > half + (4 * ds + (2 * n + 64) * E) * M).any()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T,H,kv,n", [(1, 1, 32, 4, 9000), (1, 90, 32, 2, 9000), (3, 400, 32, 4, 3500), (2, 720, 8, 2, 1333)])
+def test_groups_that_change_places(B, T, H, kv, n, t):
+    """The two groups of a head differ by 1e6 one way in the first part of a history and the
+    other way in the second: factors that come and go across folds, splits and joins."""
+    from joule_b200 import kv4
+    g, hd = _gen(n + T), 128
+    k, v = (torch.randn(n, kv, hd, device="cuda", generator=g) for _ in range(2))
+    turn = (torch.arange(n, device="cuda") * 5 // n % 2 == 0)[:, None, None]
+    v *= torch.where(turn == (torch.arange(hd, device="cuda") < 64), 1e3, 1e-3)
+    k[:, :, :4] += 2.0 * (torch.arange(n, device="cuda") * 5 // n)[:, None, None] / 4
+    cache = _cache([(k, v)])
+    q = torch.randn(B, T, H, hd, device="cuda", generator=g).to(DT[t])
+    got = kv4.kv4_attention(cache, 0, q, _i32([0] * B), _i32([n] * B))
+    r = torch.unique(torch.linspace(0, T - 1, min(T, 30)).long()).cuda()
+    for b in range(B):
+        want, M, ds, top = _exact(q[b], *_held(cache, 0, n), hd ** -0.5, r)
+        if t == "f32":
+            _close(got[b][r], want, M, ds, top, n)
+        else:
+            half = _step_of(want, t) / 2 * (1 + 2.0 ** -20)
+            assert not ((got[b][r].double() - want).abs() > half + (4 * ds + (2 * n + 64) * E) * M).any()
