@@ -404,8 +404,9 @@ __device__ __forceinline__ void kv4_block(kv4_state<HD>& st, const uint8_t* blk,
     }
 }
 
-// Bound by HBM for long caches (the codes and scales are read once, 4.25 bits
-// per value) and by launch and load latency for short ones. Each warp has a ring
+// Bound by issue slots for long caches (1,545 instructions a cache block and tile, two
+// fifths of them taking codes apart; the codes and scales are read once, DRAM at 36 %) and by
+// launch and load latency for short ones. Each warp has a ring
 // of two whole cache blocks, filled by 16-byte asynchronous copies (17 instructions a
 // block; a bulk copy held its issuing warp for hundreds of ns); no barrier between
 // warps but for the sum of a block that is inside one segment.
@@ -628,8 +629,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, 1) k_kv4_attn(kv4_dims c, int l
 // Adds up the parts of segments that several warps shared: block = RB rows of a run
 // of segments, 8 / RB warps per row, each adding every (8 / RB)-th part.
 // RUN: `per` segments a block, where a block each (2 us of latency, four to an SM)
-// took longer than the sums: 256 sequences of 16/16 heads over 512, 105 us against 97.
-// 
+// took longer than the sums (256 sequences of 16/16 heads over 512: 8 us of 98).
 template <int HD, typename T, bool RUN>
 __global__ void __launch_bounds__(256) k_kv4_merge(kv4_dims c, jl_kv4_attn_args a, int R, int ctas, int RB,
                                                    int per) {
@@ -774,8 +774,8 @@ struct kv4_plan {
 };
 
 // Splits of each unit of a call in the tcgen05 form: as many as fill the SMs, of at
-// least kMinSplit cache blocks each (4 in place of 2: 64 tokens of 32/4 heads of 128 over
-// 1,024 25.7 us against 21.3, over 4,096 the same). Calls of at most 256 positions have
+// least kMinSplit cache blocks each (with 4, 64 tokens of 32/4 heads of 128 take as long over
+// 4,096 positions, and were 4 us slower over 1,024). Calls of at most 256 positions have
 // no workspace.
 constexpr int kMinSplit = 2;
 int splits_of(long long units, int longest, int sms) {
@@ -789,9 +789,11 @@ kv4_plan plan(const jl::kv4_dims& c, int B, int T, int H, int longest, int sms) 
     // The tcgen05 kernel takes the time of its units of 256 rows, however few rows fill
     // them, and some 14 us beside (start, q, joining); this file's a time by the rows.
     // fp32, 32/4 heads of 128, here / there: 8 tokens (64 rows a unit) over 16,384
-    // positions 29 / 34 us, 16 of 4 sequences (128 a unit) 145 / 93; 64 tokens (2,048
-    // rows) over 512 14 / 20, over 1,024 21 / 21, over 4,096 47 / 30. Over types, head
-    // dims and lengths the rule is within 0.5 % of the better one (geometric mean).
+    // positions 30 / 36 us, 16 of 4 sequences (128 a unit) 149 / 98; 64 tokens (2,048
+    // rows) over 512 12 / 22, over 1,024 17 / 23, over 2,048 30 / 26, over 4,096 48 / 31.
+    // Over 802 calls of fp32 and bf16, 1 to 16 sequences of 8 to 512 tokens, 3 to 32 heads
+    // of 64 and 128, and 200 to 16,384 positions, the rule is within 0.6 % of the better
+    // one (geometric mean).
     if (rows >= 76 * units && rows * nb >= 310ll * sms) {
         const int S = splits_of(units, longest, sms);
         return {kv4_form::prompt, S, jl_kv4_prompt_ws_bytes(c, units, S)};
@@ -802,10 +804,10 @@ kv4_plan plan(const jl::kv4_dims& c, int B, int T, int H, int longest, int sms) 
     // dim 128, in units of 0.35 us (a block alone takes a warp 2 us, with all warps busy 4):
     // a warp per segment, a thread block per segment (one to three to an SM), or all blocks
     // cut evenly and a second kernel that adds up. 32/4 heads, 8 / 32 / 64 / 256 sequences,
-    // us: over 128 positions 8.4 / 8.6 / 9.1 / 12.9 by warps, 5.6 / 5.9 / 6.4 / 18.5 by
-    // blocks, over 512 11.6 / 12.6 / 17.5 / 35 cut, 7.0 / 7.3 / 11.3 / 32 by blocks, over
-    // 2,048 12.7 / 20.5 / 30 / 86 and 15.5 / 16 / 27 / 85 (lengths spread evenly: 11.5 / 16.4 /
-    // 22 / 61 and 15 / 15.5 / 26 / 64). The cut's work follows the lengths and is counted at
+    // us: over 128 positions 8.7 / 9.0 / 9.4 / 13.1 by warps, 6.0 / 6.3 / 6.8 / 19.2 by
+    // blocks, over 512 11.9 / 12.9 / 17.8 / 36 cut, 7.4 / 7.7 / 11.6 / 31 by blocks, over
+    // 2,048 13.1 / 21 / 30 / 88 and 15.7 / 16 / 27 / 96 (lengths spread evenly: 11.8 / 17.3 /
+    // 24 / 70 and 15.5 / 15.8 / 25 / 65). The cut's work follows the lengths and is counted at
     // 3/4 of the longest; a block of head dim 64 takes half.
     const double per_sm = (double)segs / sms, work = c.hd == 64 ? 0.5 * nb : nb, u = per_sm * work;
     const double whole = 10 + work * (6 + std::min(per_sm, 12.0) / 2) * std::max(1.0, std::ceil(per_sm / kKvWarps));

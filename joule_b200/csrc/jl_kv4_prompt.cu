@@ -22,13 +22,14 @@
 //
 // A unit is the 256 rows of one block. When there are fewer units than SMs, S blocks
 // share a unit's cache blocks; their sums meet in k_kv4_prompt_merge (fp32, 32/4 heads
-// of 128: 64 tokens over 2,048 positions 24 us, 256 over 4,096 68, 512 over 16,384 436;
-// the form for few rows 29, 147 and 1,067).
+// of 128: 64 tokens over 2,048 positions 25 us, 256 over 4,096 67, 512 over 16,384 415;
+// the form for few rows 30, 150 and 1,102).
 //
-// Bound by the tensor cores in fp32 (two passes of each product; a product of 64
-// positions takes 60 to 75 cycles where its arithmetic takes 32, q being read from
-// shared memory) and by the softmax's issue slots in 16 bits. 2,047 rows of 32/4 heads
-// of 128 over 4,100 positions, fp32: 313 us; 123 at the measured bf16 rate.
+// Bound by the tensor cores and the softmax's latency alike: in fp32 two passes of each
+// product (a product of 64 positions takes 60 to 75 cycles where its arithmetic takes 32,
+// q being read from shared memory), in 16 bits one of the scores and two of the values.
+// 2,047 rows of 32/4 heads of 128 over 4,100 positions: fp32 338 us, 123 at the measured
+// bf16 rate, bf16 332, 92 at that rate.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -44,9 +45,9 @@ constexpr int kPrTile = 128, kPrPair = 2 * kPrTile, kPrThreads = 12 * 32, kPrUnp
 // about 1e-7 n of themselves. The sums therefore move to the rows of `out` (16-bit calls:
 // their lower halves; the upper ones to shared memory) every kPrFold blocks, which hold
 // them until the end, and TMEM starts anew. fp32, 2,047 rows of 32/4 heads of 128 over
-// 4,100 positions: error 1.6e-6 and 309 us (never: 7.4e-6, 264 us; every 12: 2.0e-6, every
-// 16: 2.5e-6); over 23,000: 1.9e-6 (never: 4.7e-5). In 16-bit calls 32 blocks' 3e-6 are
-// far below a step of the output.
+// 4,100 positions: error 1.1e-6 and 338 us (never: 6.8e-6, 299 us; every 12: 1.7e-6, 326 us,
+// every 16: 2.2e-6, 319 us); 120 tokens of 96/4 heads over 23,000: 1.2e-6 (never: 1.7e-5).
+// In 16-bit calls 32 blocks' 3e-6 are far below a step of the output.
 template <bool F32>
 constexpr int kPrFold = F32 ? 8 : 32;
 constexpr int kPrCore = 144;  // bytes between V's core matrices (128 of data: stores without bank conflicts)
@@ -311,8 +312,7 @@ __device__ __forceinline__ void pr_unpack(const uint8_t* raw, uint8_t* kt, uint8
 // rescaled to the reference `ref`. Places: pieces (4 values) of
 // the warp's rows in turn over the rows' own part of `out` (runs of the kv head's heads,
 // one run a token) or of the workspace. A call of its own that finds its arguments in
-// shared memory: inlined it took the softmax's registers (chunk below: 326 us inlined,
-// 309 so).
+// shared memory, out of the softmax's registers.
 template <int HD, bool HALF>
 __device__ __noinline__ void pr_fold(uint32_t to, float ref, float less, pr_held* held, bool holds) {
     const float href = held->ref[threadIdx.x], al = ex2(href - (ref == -INFINITY ? 0.0f : ref));
@@ -443,8 +443,8 @@ __device__ __forceinline__ float2 pr_weights(uint32_t ts, const float* sc, const
 
 // Exponents above a row's products with the scales of each group in a block (kv4_ref), from
 // the sums in TMEM: n positions are seen. 16 at a time, brought to the largest score. A call
-// of its own, before the softmax's registers are in use: inlined on its scores it made every
-// block slower (8 % of a prompt).
+// of its own, before the softmax's registers are in use (computed from the softmax's own
+// scores it made every block slower, 8 % of a prompt).
 template <int HD>
 __device__ __noinline__ float2 pr_products(uint32_t ts, float f, const float* sc, int n) {
     constexpr int NG = HD / 64;
