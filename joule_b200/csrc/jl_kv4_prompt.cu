@@ -509,6 +509,7 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int t, uint32_t 
         if (j > 0 && starts && !(MORE && j == from)) {  // S was issued after the last block's values: the sums are complete
             if (F32 || S > 1) pr_fold<HD, false>(to, st.r.ref, st.r.less(), held, j > FOLD);
             else pr_fold<HD, true>(to, st.r.ref, st.r.less(), held, j > FOLD);
+            __syncwarp();
         }
         const float* sc = reinterpret_cast<const float*>(smem + SM::sc) + s * 4 * kKv4Rows;
         const uint32_t most = max(sh.range[s][0].x, sh.range[s][1].x), least = min(sh.range[s][0].y, sh.range[s][1].y);
@@ -526,6 +527,7 @@ __device__ __forceinline__ pr_run<HD> pr_softmax(uint8_t* smem, int t, uint32_t 
         if (__any_sync(0xffffffffu, past)) {
             const float2 al = past ? st.r.move(mx, bound.x, bound.y) : f2(1.0f);
             st.lsum.scale(al.x);
+            __syncwarp();  // (rows part above; the loads below are the whole warp's)
             if (!starts) {  // the sums of earlier blocks are complete (S was issued after them)
 #pragma unroll 1
                 for (int q = 0; q < NG * 4; q++) {
